@@ -2,6 +2,9 @@
 #include "../../include/celebbasis_hip.h"
 #include "cb_models.h"
 #include "cb_gemm_tiles.h"
+#include "cb_seq.h"
+#include <algorithm>
+#include <cmath>
 
 using namespace cb;
 
@@ -23,6 +26,12 @@ struct cb_vae_dec { Ctx* ctx; VaeDec V; };
 struct cb_clip { Ctx* ctx; Clip C; std::unique_ptr<Graph> G; Ten* out = nullptr; Ten* in = nullptr; };
 struct cb_frnet { Ctx* ctx; FrNet F; };
 struct cb_trainer { Ctx* ctx; Trainer T; };
+// bucket of every relative position in [-D, D] (host and device), and the range of positions of every bucket
+struct cb_relpos {
+    int device = -1, D = 0, nb = 0;
+    std::vector<short> map; std::vector<int> range;
+    short* dmap = nullptr; int* drange = nullptr;
+};
 
 static void require(const void* p, const char* what) { CB_CHECK(p != nullptr, CB_ERR_ARG, "%s must not be NULL", what); }
 
@@ -1000,6 +1009,168 @@ int cb_trainer_set_state(cb_trainer* t, const char* name, const float* host_src,
             CB_HIP(hipMemcpy(r.p, host_src, (size_t)r.n * sizeof(float), hipMemcpyHostToDevice));
         }
     }
+    CB_END
+}
+
+// ------------------------------------------------------------------ sequence attention
+// work of a context goes to the context's device, whatever the calling thread's current device is
+struct OnDevice {
+    int prev = -1;
+    explicit OnDevice(const Ctx& c) {
+        if (c.dry) return;
+        int cur = 0;
+        CB_HIP(hipGetDevice(&cur));
+        if (cur != c.device) { CB_HIP(hipSetDevice(c.device)); prev = cur; }
+    }
+    ~OnDevice() { if (prev >= 0) (void)hipSetDevice(prev); }
+};
+int cb_relpos_create(cb_ctx* ctx, int num_buckets, int max_distance, int bidirectional, cb_relpos** out) {
+    CB_TRY
+    require(ctx, "ctx"); require(out, "out");
+    const bool two = bidirectional != 0;
+    CB_CHECK(num_buckets >= (two ? 4 : 2) && num_buckets <= SEQ_MAX_BUCKETS && num_buckets % (two ? 4 : 2) == 0, CB_ERR_ARG,
+             "relpos: num_buckets = %d (2 .. %d, a multiple of %d)", num_buckets, SEQ_MAX_BUCKETS, two ? 4 : 2);
+    const int nb = two ? num_buckets / 2 : num_buckets, E = nb / 2, m = nb - E, D = max_distance;
+    CB_CHECK(D > E && D <= SEQ_MAX_DIST, CB_ERR_ARG, "relpos: max_distance = %d (%d .. %d)", D, E + 1, SEQ_MAX_DIST);
+    std::unique_ptr<cb_relpos> h(new cb_relpos());
+    h->device = ctx->c.dry ? -1 : ctx->c.device; h->D = D; h->nb = num_buckets;
+    // first distance of bucket E + k: the least whole n with n >= E (D/E)^(k/m). A border that is itself whole is found 1e-15 off at most.
+    std::vector<int> first((size_t)m, E);
+    for (int k = 1; k < m; ++k) {
+        const long double x = (long double)E * powl((long double)D / E, (long double)k / m), r = roundl(x);
+        first[(size_t)k] = (int)(fabsl(x - r) < 1e-13L * x ? r : ceill(x));
+    }
+    h->map.resize((size_t)2 * D + 1);
+    h->range.assign((size_t)2 * num_buckets, 0);
+    for (int rel = -D; rel <= D; ++rel) {
+        const int n = two ? abs(rel) : std::max(-rel, 0);
+        int k = n;
+        if (n >= E) { k = E; for (int i = 1; i < m; ++i) k += n >= first[(size_t)i]; }
+        if (two && rel > 0) k += nb;
+        h->map[(size_t)(rel + D)] = (short)k;
+        int* r = &h->range[(size_t)2 * k];
+        if (r[0] == r[1]) r[0] = rel + D;          // every bucket is one run of positions
+        r[1] = rel + D + 1;
+    }
+    if (!ctx->c.dry) {
+        OnDevice on(ctx->c);
+        try {
+            CB_HIP(hipMalloc(&h->dmap, h->map.size() * sizeof(short)));
+            CB_HIP(hipMalloc(&h->drange, h->range.size() * sizeof(int)));
+            CB_HIP(hipMemcpy(h->dmap, h->map.data(), h->map.size() * sizeof(short), hipMemcpyHostToDevice));
+            CB_HIP(hipMemcpy(h->drange, h->range.data(), h->range.size() * sizeof(int), hipMemcpyHostToDevice));
+        } catch (...) { (void)hipFree(h->dmap); (void)hipFree(h->drange); throw; }
+    }
+    *out = h.release();
+    CB_END
+}
+int cb_relpos_destroy(cb_relpos* rp) {
+    CB_TRY
+    if (rp) { if (rp->dmap) (void)hipFree(rp->dmap); if (rp->drange) (void)hipFree(rp->drange); }
+    delete rp;
+    CB_END
+}
+int cb_relpos_bucket(const cb_relpos* rp, int64_t relative, int* bucket) {
+    CB_TRY
+    require(rp, "relpos"); require(bucket, "bucket");
+    const int64_t r = std::min<int64_t>(std::max<int64_t>(relative, -rp->D), rp->D);
+    *bucket = rp->map[(size_t)(r + rp->D)];
+    CB_END
+}
+// a [batch][token][head][d] operand: alignment, strides, and for outputs that no element is written twice
+static SeqT seq_tensor(const cb_seq_tensor& t, const char* what, DType dt, int B, int N, int H, int d, bool written, bool dry) {
+    const int64_t ep = 16 / (int64_t)dt_size(dt);
+    if (!dry && (long)B * N * H > 0) require(t.p, what);
+    CB_CHECK((reinterpret_cast<uintptr_t>(t.p) & 15) == 0, CB_ERR_ARG, "seq attention: %s is not 16-byte aligned", what);
+    CB_CHECK(t.row >= 0 && t.head >= 0 && t.batch >= 0 && t.row % ep == 0 && t.head % ep == 0 && t.batch % ep == 0, CB_ERR_SHAPE,
+             "seq attention: strides of %s (%ld, %ld, %ld) are not multiples of 16 bytes", what, (long)t.row, (long)t.head, (long)t.batch);
+    CB_CHECK(t.row < (1 << 22), CB_ERR_SHAPE, "seq attention: row stride of %s is %ld, at most 2^22 - 1 elements", what, (long)t.row);
+    if (written) {
+        std::vector<std::pair<int64_t, int64_t>> e;          // (stride, extent)
+        if (N > 1) e.push_back({t.row, N});
+        if (H > 1) e.push_back({t.head, H});
+        if (B > 1) e.push_back({t.batch, B});
+        std::sort(e.begin(), e.end());
+        int64_t span = d;
+        for (auto& x : e) {
+            CB_CHECK(x.first >= span, CB_ERR_SHAPE, "seq attention: %s overlaps itself (strides %ld, %ld, %ld)", what, (long)t.row, (long)t.head, (long)t.batch);
+            span = x.first * (x.second - 1) + span;
+        }
+    }
+    SeqT r; r.p = t.p; r.row = t.row; r.head = t.head; r.batch = t.batch;
+    return r;
+}
+static SeqArgs seq_args(const cb_ctx* ctx, const cb_seq_attention_desc* d, bool bwd, bool pointers) {
+    const Ctx& c = ctx->c;
+    CB_CHECK(d->struct_size == (int)sizeof(cb_seq_attention_desc), CB_ERR_ARG, "seq attention: desc.struct_size %d != %d — caller built against "
+             "another header (ABI %d)", d->struct_size, (int)sizeof(cb_seq_attention_desc), CB_ABI_VERSION);
+    CB_CHECK(d->dtype == CB_DTYPE_F32 || d->dtype == CB_DTYPE_BF16, CB_ERR_ARG, "seq attention: unknown desc.dtype %d", d->dtype);
+    CB_CHECK(d->B >= 0 && d->Nq >= 0 && d->Nk >= 0 && d->heads >= 1 && d->kv_heads >= 1 && d->heads % d->kv_heads == 0, CB_ERR_SHAPE,
+             "seq attention: B = %d, Nq = %d, Nk = %d, heads = %d, kv_heads = %d", d->B, d->Nq, d->Nk, d->heads, d->kv_heads);
+    CB_CHECK(d->Nq <= (1 << 24) && d->Nk <= (1 << 24), CB_ERR_SHAPE, "seq attention: at most 2^24 tokens (Nq = %d, Nk = %d)", d->Nq, d->Nk);
+    CB_CHECK((int64_t)d->B * d->heads <= (1 << 20) && (int64_t)d->B * d->heads * cdiv(std::max(d->Nq, d->Nk), 64) < (1ll << 31), CB_ERR_SHAPE,
+             "seq attention: B * heads = %ld with %d tokens is too large for one call", (long)d->B * d->heads, std::max(d->Nq, d->Nk));
+    CB_CHECK(d->d >= 8 && d->d % 8 == 0 && d->d <= SEQ_MAX_D, CB_ERR_SHAPE, "seq attention: head dim %d (a multiple of 8, at most %d)", d->d, SEQ_MAX_D);
+    CB_CHECK(d->scale > 0.f && std::isfinite(d->scale), CB_ERR_ARG, "seq attention: scale = %g must be positive and finite", (double)d->scale);
+    CB_CHECK((d->relpos != nullptr) == (d->table != nullptr), CB_ERR_ARG, "seq attention: relpos and table go together");
+    SeqArgs a;
+    a.dt = (DType)d->dtype; a.B = d->B; a.Nq = d->Nq; a.Nk = d->Nk; a.H = d->heads; a.Hkv = d->kv_heads; a.G = d->heads / d->kv_heads; a.d = d->d;
+    a.scale = d->scale; a.causal = d->causal != 0;
+    a.q_pos = d->q_pos; a.q_len = d->q_len; a.kv_len = d->kv_len; a.mask = d->kv_mask; a.mask_b = d->mask_stride;
+    CB_CHECK(!d->kv_mask || d->mask_stride >= 0, CB_ERR_SHAPE, "seq attention: mask_stride = %ld", (long)d->mask_stride);
+    if (d->relpos) {
+        CB_CHECK(d->relpos->device == (c.dry ? -1 : c.device), CB_ERR_ARG, "seq attention: the relpos handle belongs to device %d", d->relpos->device);
+        a.table = d->table; a.bmap = d->relpos->dmap; a.brange = d->relpos->drange; a.D = d->relpos->D; a.nb = d->relpos->nb;
+    }
+    if (bwd) {
+        CB_CHECK(!d->dtable || d->relpos, CB_ERR_ARG, "seq attention: dtable without a table");
+        a.dtable = d->dtable;
+    }
+    a.lse = d->lse; a.o32 = a.dt == DT_BF16 ? d->out32 : nullptr;
+    if (!pointers) return a;
+    a.q = seq_tensor(d->q, "q", a.dt, d->B, d->Nq, d->heads, d->d, false, c.dry);
+    a.k = seq_tensor(d->k, "k", a.dt, d->B, d->Nk, d->kv_heads, d->d, false, c.dry);
+    a.v = seq_tensor(d->v, "v", a.dt, d->B, d->Nk, d->kv_heads, d->d, false, c.dry);
+    a.o = seq_tensor(d->out, "out", a.dt, d->B, d->Nq, d->heads, d->d, !bwd, c.dry);
+    CB_CHECK((reinterpret_cast<uintptr_t>(d->out32) & 15) == 0, CB_ERR_ARG, "seq attention: out32 is not 16-byte aligned");
+    if (bwd) {
+        a.dout = seq_tensor(d->dout, "dout", a.dt, d->B, d->Nq, d->heads, d->d, false, c.dry);
+        a.dq = seq_tensor(d->dq, "dq", a.dt, d->B, d->Nq, d->heads, d->d, true, c.dry);
+        a.dk = seq_tensor(d->dk, "dk", a.dt, d->B, d->Nk, d->kv_heads, d->d, true, c.dry);
+        a.dv = seq_tensor(d->dv, "dv", a.dt, d->B, d->Nk, d->kv_heads, d->d, true, c.dry);
+        if (!c.dry && (long)d->B * d->Nq > 0) require(d->lse, "lse");
+    }
+    return a;
+}
+static size_t seq_ws(const SeqArgs& a, bool bwd) { return bwd ? seq_bwd_plan(a, a.dtable != nullptr).total : seq_fwd_plan(a).total; }
+static void seq_ws_check(const cb_seq_attention_desc* d, size_t need, bool dry) {
+    CB_CHECK(d->workspace_bytes >= 0 && (size_t)d->workspace_bytes >= need, CB_ERR_ARG, "seq attention: workspace of %ld bytes, %zu needed", (long)d->workspace_bytes, need);
+    if (need && !dry) require(d->workspace, "workspace");
+    CB_CHECK((reinterpret_cast<uintptr_t>(d->workspace) & 15) == 0, CB_ERR_ARG, "seq attention: workspace is not 16-byte aligned");
+}
+int cb_seq_attention_workspace(cb_ctx* ctx, const cb_seq_attention_desc* d, int backward, int64_t* bytes) {
+    CB_TRY
+    require(ctx, "ctx"); require(d, "desc"); require(bytes, "bytes");
+    *bytes = (int64_t)seq_ws(seq_args(ctx, d, backward != 0, false), backward != 0);
+    CB_END
+}
+int cb_seq_attention_fwd(cb_ctx* ctx, const cb_seq_attention_desc* d) {
+    CB_TRY
+    require(ctx, "ctx"); require(d, "desc");
+    const SeqArgs a = seq_args(ctx, d, false, true);
+    seq_ws_check(d, seq_ws(a, false), ctx->c.dry);
+    if ((long)a.B * a.Nq == 0) return CB_STATUS_OK;
+    OnDevice on(ctx->c);
+    seq_forward(ctx->c.launch(), a, d->workspace);
+    CB_END
+}
+int cb_seq_attention_bwd(cb_ctx* ctx, const cb_seq_attention_desc* d) {
+    CB_TRY
+    require(ctx, "ctx"); require(d, "desc");
+    const SeqArgs a = seq_args(ctx, d, true, true);
+    seq_ws_check(d, seq_ws(a, true), ctx->c.dry);
+    OnDevice on(ctx->c);
+    seq_backward(ctx->c.launch(), a, d->workspace);
     CB_END
 }
 

@@ -1,0 +1,266 @@
+// cb_seq.h — attention over sequences with lengths, key masks, shared key / value heads and a learned relative position bias: the
+// arguments of the kernels (cb_seq_fwd.hip, cb_seq_bwd.hip) and the device pieces that they share.
+//
+//   visible(i, j) = i < q_len[b]  and  j < kv_len[b]  and  mask[b][j]  and  (not causal or j <= q_pos[b] + i)
+//   s_ij = scale * q_i . k_j + table[bucket(j - q_pos[b] - i)][h] ;  o_i = sum_j softmax_j(s_ij) v_j  over the visible keys (none: o_i = 0)
+//
+// One code for fp32 and bf16. A fragment is 8 consecutive elements of a row (lane (l15, g) of a wave: row l15, elements 8g .. 8g+7 of a
+// 32-wide group of the head dim): one v_mfma_f32_16x16x32_bf16, or eight v_mfma_f32_16x16x4_f32 whose k index is g and whose i-th call takes
+// element i — a permutation of the sum over the head dim that both operands share. The accumulator of X Y^T (lane: row 4g + r of X, row l15 of
+// Y) is, packed, the second operand of the following product without any movement between lanes.
+#pragma once
+#include "cb_device.h"
+#include <type_traits>
+
+namespace cb {
+
+struct SeqT { void* p = nullptr; long row = 0, head = 0, batch = 0; };       // element strides of one token, one head, one sample
+
+struct SeqArgs {
+    DType dt = DT_F32;
+    int B = 0, Nq = 0, Nk = 0, H = 0, Hkv = 0, G = 1, d = 0;                 // G = H / Hkv query heads share a key / value head
+    SeqT q, k, v, o;
+    float scale = 1.f; int causal = 0;
+    const int* q_pos = nullptr; const int* q_len = nullptr; const int* kv_len = nullptr;
+    const unsigned char* mask = nullptr; long mask_b = 0;
+    const float* table = nullptr; const short* bmap = nullptr; const int* brange = nullptr; int D = 0, nb = 0;   // relative bias (relpos handle)
+    float* lse = nullptr;                                                     // [B][H][Nq], natural logarithm
+    float* o32 = nullptr;                                                     // [B][Nq][H][d]: the unrounded output (bf16, kept for the backward pass)
+    // backward
+    SeqT dout, dq, dk, dv;
+    float* dvec = nullptr;                                                    // [B][H][Nq]: rowsum(dO * O)
+    float* dtable = nullptr;                                                  // [nb][H]
+    float* tpart = nullptr;                                                   // [B][H][blocks of queries][nb]
+    float* part = nullptr; float* ml = nullptr; int nsplit = 1;               // partial results of a split axis (fp32)
+};
+
+struct SeqPlan { int qb = 1, nsplit = 1; size_t part = 0, ml = 0, total = 0; };           // sizes in bytes
+struct SeqBwdPlan { int qb = 1, kb = 1, qsplit = 1, ksplit = 1, nqb = 1; size_t dvec = 0, tpart = 0, part = 0, partq = 0, total = 0; };
+SeqPlan seq_fwd_plan(const SeqArgs& a);
+SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable);
+void seq_forward(const Launch& L, SeqArgs a, void* ws);
+void seq_backward(const Launch& L, SeqArgs a, void* ws);
+
+constexpr int SEQ_MAX_D = 160, SEQ_MAX_DIST = 1024, SEQ_MAX_BUCKETS = 256;
+
+#ifdef __HIPCC__
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4s __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* lds_vp;
+typedef __attribute__((address_space(3))) s16x4* lds_s4;
+
+constexpr float SEQ_L2E = 1.4426950408889634f, SEQ_LN2 = 0.6931471805599453f;
+constexpr int SEQ_OOB = -16;                       // 0xFFFFFFF0 >= num_records: the load returns zeros
+constexpr int SEQ_POS_LIM = 1 << 29;               // positions are held to +-2^29, so that differences stay inside an int
+
+__device__ __forceinline__ float seq_group_max(float v) { v = fmaxf(v, __shfl_xor(v, 16, 64)); return fmaxf(v, __shfl_xor(v, 32, 64)); }
+__device__ __forceinline__ float seq_group_sum(float v) { v += __shfl_xor(v, 16, 64); return v + __shfl_xor(v, 32, 64); }
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t seq_srd(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0x7FFFFFFF, 0x00020000);
+}
+
+template <typename T> struct SeqFrag;
+template <> struct SeqFrag<bf16_t> { bf16x8_t v; };
+template <> struct SeqFrag<float> { f32x4 v[2]; };
+__device__ __forceinline__ f32x4 seq_mma(const SeqFrag<bf16_t>& a, const SeqFrag<bf16_t>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 seq_mma(const SeqFrag<float>& a, const SeqFrag<float>& b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i >> 2][i & 3], b.v[i >> 2][i & 3], c, 0, 0, 0);
+    return c;
+}
+
+// Geometry of one instantiation. A tile is TK rows in LDS, row-major, P pieces of 16 bytes a row, filled by LDS-DMA in lane-linear slots of
+// 256 pieces; piece c of row r lies at place swz(c, r), which puts the 16 rows that a fragment read touches into 16 different bank groups.
+template <typename T, int DT> struct SeqGeo {
+    static constexpr int ES = sizeof(T), EP = 16 / ES;                        // elements of a piece
+    static constexpr int KS = (DT + 1) / 2;                                   // 32-wide groups of the head dim
+    static constexpr int P = KS * 32 / EP;
+    static constexpr int TK = (ES == 4 && DT >= 8) ? 32 : 64;
+    static constexpr int KT = TK / 16;
+    static constexpr int TILE = TK * P * 16, NS = TILE / 4096;
+    static constexpr int DA = ES == 4 ? 2 * KS : DT;                          // 16-wide accumulator tiles across the head dim
+    static __device__ __forceinline__ int swz(int c, int r) {
+        if constexpr (P % 16 == 0) return c ^ (r & 15);
+        else if constexpr (P % 8 == 0) return c ^ ((r >> 1) & 7);
+        else return c ^ ((r >> 2) & 3);
+    }
+};
+
+// per-thread source offsets of a tile's slots (bytes from the tile's first row), and the DMA of one tile: rows whose bit in `live` is
+// clear, and elements at or beyond the head dim, are filled with zeros — masked places may hold anything, NaN included
+template <typename T, int DT> struct SeqSlots {
+    using G = SeqGeo<T, DT>;
+    int off[G::NS];
+    __device__ __forceinline__ void init(long ld, int d, int tid) {
+#pragma unroll
+        for (int i = 0; i < G::NS; ++i) {
+            const int idx = tid + 256 * i, r = idx / G::P, c = G::swz(idx - r * G::P, r);
+            off[i] = (c * G::EP < d) ? (int)((long)r * ld * G::ES + c * 16) : SEQ_OOB;
+        }
+    }
+    // dst: the tile's image + this wave's 1 KiB piece of a slot
+    __device__ __forceinline__ void dma(const T* rows, char* dst, unsigned long long live, int tid) const {
+        const __amdgpu_buffer_rsrc_t srd = seq_srd(rows);
+        if (live == (G::TK == 64 ? ~0ull : 0xFFFFFFFFull)) {
+#pragma unroll
+            for (int i = 0; i < G::NS; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_vp)(dst + i * 4096), 16, off[i], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < G::NS; ++i) {
+                const int r = (tid + 256 * i) / G::P;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_vp)(dst + i * 4096), 16, ((live >> r) & 1ull) ? off[i] : SEQ_OOB, 0, 0, 0);
+            }
+        }
+    }
+};
+
+// fragment of rows 16 blk + l15, 32-wide group s of the head dim
+template <typename T, int DT>
+__device__ __forceinline__ SeqFrag<T> seq_frag_lds(const char* img, int blk, int s, int l15, int g) {
+    using G = SeqGeo<T, DT>;
+    const int r = blk * 16 + l15;
+    SeqFrag<T> f;
+    if constexpr (G::ES == 2) {
+        f.v = *reinterpret_cast<const bf16x8_t*>(img + (r * G::P + G::swz(4 * s + g, l15)) * 16);
+    } else {
+        f.v[0] = *reinterpret_cast<const f32x4*>(img + (r * G::P + G::swz(8 * s + 2 * g, l15)) * 16);
+        f.v[1] = *reinterpret_cast<const f32x4*>(img + (r * G::P + G::swz(8 * s + 2 * g + 1, l15)) * 16);
+    }
+    return f;
+}
+// the same of a row in global memory, zeros where the row is not valid
+template <typename T>
+__device__ __forceinline__ SeqFrag<T> seq_frag_row(const T* row, bool valid, int s, int g, int d) {
+    SeqFrag<T> f;
+    const int c = 32 * s + 8 * g;
+    const bool ok = valid && c < d;
+    if constexpr (sizeof(T) == 2) {
+        u32x4s v = {0u, 0u, 0u, 0u};
+        if (ok) v = *reinterpret_cast<const u32x4s*>(row + c);
+        f.v = __builtin_bit_cast(bf16x8_t, v);
+    } else {
+        f.v[0] = (f32x4){0.f, 0.f, 0.f, 0.f}; f.v[1] = f.v[0];
+        if (ok) { f.v[0] = *reinterpret_cast<const f32x4*>(row + c); f.v[1] = *reinterpret_cast<const f32x4*>(row + c + 4); }
+    }
+    return f;
+}
+
+// acc[QB][DA] += (tile rows)^T . w: the transposed product of the second half of attention. w[qb][kt] is the accumulator of a product of the
+// same tile (lane: tile rows 16 kt + 4g + r, column l15).
+//   bf16: the A operand (head-dim index l15, k slot 8g + j <-> row 32G + 4g + j, or 32G + 16 + 4g + j - 4) comes from two transposing LDS reads
+//         (a 16-lane group reads four rows of 16 elements and gets their columns).
+//   fp32: one 8-byte read of row 16 kt + 4g + r at columns 32 tt + 2 l15, + 1 feeds two calls; accumulator (tt, e) then holds column
+//         32 tt + 2 (4g + r) + e, so that a lane owns the 8 consecutive columns 32 tt + 8g .. + 7.
+template <typename T, int DT, int QB> using SeqAcc = f32x4[QB][SeqGeo<T, DT>::DA];
+template <typename T, int DT, int QB> using SeqScores = f32x4[QB][SeqGeo<T, DT>::KT];
+template <typename T, int DT> using SeqRow = f32x4[SeqGeo<T, DT>::DA];
+template <typename T, int DT, int QB>
+__device__ __forceinline__ void seq_tmul(SeqAcc<T, DT, QB>& acc, const char* img, const SeqScores<T, DT, QB>& w, int l15, int g) {
+    using G = SeqGeo<T, DT>;
+    if constexpr (G::ES == 2) {
+#pragma unroll
+        for (int kg = 0; kg < G::KT / 2; ++kg) {
+            SeqFrag<bf16_t> b[QB];
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
+                const f32x4 x = w[qb][2 * kg], y = w[qb][2 * kg + 1];
+                b[qb].v = (bf16x8_t){(bf16_t)x[0], (bf16_t)x[1], (bf16_t)x[2], (bf16_t)x[3], (bf16_t)y[0], (bf16_t)y[1], (bf16_t)y[2], (bf16_t)y[3]};
+            }
+            const int r0 = 4 * g + (l15 >> 2), r1 = r0 + 16;             // row inside the 32-row group
+            const int half = (l15 & 3) >> 1, sub = (l15 & 1) * 8;
+#pragma unroll
+            for (int t = 0; t < G::DA; ++t) {
+                const char* p0 = img + ((kg * 32 + r0) * G::P + G::swz(2 * t + half, r0)) * 16 + sub;
+                const char* p1 = img + ((kg * 32 + r1) * G::P + G::swz(2 * t + half, r1)) * 16 + sub;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p0), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p1);
+                SeqFrag<bf16_t> a;
+                typedef short s16x8 __attribute__((ext_vector_type(8)));
+                a.v = __builtin_bit_cast(bf16x8_t, (s16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) acc[qb][t] = seq_mma(a, b[qb], acc[qb][t]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int kt = 0; kt < G::KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = kt * 16 + 4 * g + r;
+#pragma unroll
+                for (int tt = 0; tt < G::KS; ++tt) {
+                    const int c = 8 * tt + (l15 >> 1);
+                    const f32x2 v = *reinterpret_cast<const f32x2*>(img + (row * G::P + G::swz(c, row)) * 16 + (l15 & 1) * 8);
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb) {
+                        acc[qb][2 * tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[0], w[qb][kt][r], acc[qb][2 * tt], 0, 0, 0);
+                        acc[qb][2 * tt + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[1], w[qb][kt][r], acc[qb][2 * tt + 1], 0, 0, 0);
+                    }
+                }
+            }
+    }
+}
+// one row of such an accumulator (this lane's share) through f(column, value); columns at or beyond d are left out
+template <typename T, int DT, typename F>
+__device__ __forceinline__ void seq_row4(const SeqRow<T, DT>& acc, int d, int g, F f) {
+    using G = SeqGeo<T, DT>;
+    if constexpr (G::ES == 2) {
+#pragma unroll
+        for (int t = 0; t < G::DA; ++t) {
+            const int c = 16 * t + 4 * g;
+            if (c < d) f(c, make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]));
+        }
+    } else {
+#pragma unroll
+        for (int tt = 0; tt < G::KS; ++tt) {
+            const int c = 32 * tt + 8 * g;
+            const f32x4 e = acc[2 * tt], o = acc[2 * tt + 1];
+            if (c < d) { f(c, make_float4(e[0], o[0], e[1], o[1])); f(c + 4, make_float4(e[2], o[2], e[3], o[3])); }
+        }
+    }
+}
+
+// the bias of one head by distance, times log2(e), in LDS: bw[rel + D + pad]. Distances past D share the outermost bucket. The entries stay
+// finite in the log2 domain (a table may hold its type's lowest value): held to +-1e37; minus infinity and
+// NaN are kept.
+__device__ __forceinline__ void seq_bias_fill(float* bw, const SeqArgs& a, int h, int pad, int tid) {
+    const int n = 2 * (a.D + pad) + 1;
+    for (int i = tid; i < n; i += 256) {
+        const int rel = min(max(i - (a.D + pad), -a.D), a.D);
+        const float b = a.table[(long)a.bmap[rel + a.D] * a.H + h];
+        bw[i] = ((b == -INFINITY || b != b) ? b : fminf(fmaxf(b, -1e37f), 1e37f)) * SEQ_L2E;
+    }
+}
+// visible rows of a tile as a bit mask (wave-uniform): rows at or beyond `len` and rows that the key mask hides are clear
+template <int TK>
+__device__ __forceinline__ unsigned long long seq_live(const unsigned char* mask, int r0, int len, int lane) {
+    if (mask) {
+        const int r = r0 + lane;
+        return __ballot(lane < TK && r < len && mask[min(r, len - 1)] != 0);
+    }
+    const int n = len - r0;
+    return n >= 64 ? (TK == 64 ? ~0ull : 0xFFFFFFFFull) : (n <= 0 ? 0ull : (((1ull << n) - 1) & (TK == 64 ? ~0ull : 0xFFFFFFFFull)));
+}
+__device__ __forceinline__ int seq_clamp_len(const int* p, int b, int n) { return p ? min(max(p[b], 0), n) : n; }
+__device__ __forceinline__ int seq_pos(const int* p, int b) { return p ? min(max(p[b], -SEQ_POS_LIM), SEQ_POS_LIM) : 0; }
+// block index -> work item such that a contiguous run of items lands on one XCD (blocks are dealt to the 8 XCDs in turn)
+__device__ __forceinline__ int seq_xcd(int id, int n) {
+    const int per = n >> 3, rem = n & 7, x = id & 7, y = id >> 3;
+    return x * per + min(x, rem) + y;
+}
+#endif  // __HIPCC__
+
+#define SEQ_DT_SWITCH(d, DTC, ...)                                   \
+    do {                                                             \
+        if ((d) <= 32) { constexpr int DTC = 2; __VA_ARGS__; }       \
+        else if ((d) <= 48) { constexpr int DTC = 3; __VA_ARGS__; }  \
+        else if ((d) <= 64) { constexpr int DTC = 4; __VA_ARGS__; }  \
+        else if ((d) <= 80) { constexpr int DTC = 5; __VA_ARGS__; }  \
+        else if ((d) <= 128) { constexpr int DTC = 8; __VA_ARGS__; } \
+        else { constexpr int DTC = 10; __VA_ARGS__; }                \
+    } while (0)
+
+}  // namespace cb

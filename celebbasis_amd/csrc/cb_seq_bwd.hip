@@ -1,0 +1,511 @@
+// cb_seq_bwd.hip — backward of the attention of cb_seq.h. With p = exp(s - lse) recomputed tile by tile:
+//   dP = dO V^T,  D = rowsum(dO * O),  dS = p (dP - D);   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,  dtable[c] = sum of dS over the
+//   pairs whose distance j - i lies in bucket c.
+// Two kernels, so that no sum depends on the order of arrival: one block of queries over the keys (dQ, D, dtable), one block of keys over the
+// queries of all heads that share them (dK, dV). Both hold the streamed side in LDS row-major and their own side in registers.
+//
+// dtable: the distance is constant along the diagonals of a dS tile. Tiles past the table's range add to one number a lane. The others are
+// summed over equal kt - qb in registers, written to LDS with row i shifted by i, and summed by column: each lane owns whole distances, in a
+// fixed order. A wave's sums by distance are folded by bucket at its end.
+#include "cb_seq.h"
+
+namespace cb {
+
+template <typename T, int DT, int QB, bool BIAS, bool TAB> struct SeqDq {
+    using G = SeqGeo<T, DT>;
+    static constexpr int PAD = G::TK + 16 * QB, NE = QB + G::KT - 1, NCOL = 16 * NE + 15, SP = NCOL + 2;
+    static constexpr int SKEW = TAB ? 4 * 16 * SP * 4 : 0;
+    static int lds(int D) {
+        const int w = 2 * (D + PAD) + 1;
+        return 4 * G::TILE + (BIAS ? (int)rup(w * 4, 16) : 0) + SKEW + (TAB ? 4 * w * 4 : 0);
+    }
+};
+
+template <typename T, int DT, int QB, bool BIAS, bool TAB>
+__global__ __launch_bounds__(256) void seq_dq_kernel(const SeqArgs a, const int nqb) {
+#ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
+    using G = SeqGeo<T, DT>;
+    using S = SeqDq<T, DT, QB, BIAS, TAB>;
+    constexpr int TK = G::TK, KT = G::KT, KS = G::KS, STAGE = 2 * G::TILE, PAD = S::PAD, NE = S::NE, SP = S::SP;
+    extern __shared__ __attribute__((aligned(16))) char lds_seq[];
+    const int W = 2 * (a.D + PAD) + 1;
+    float* bw = reinterpret_cast<float*>(lds_seq + 2 * STAGE);
+    float* skew = bw + ((W + 3) & ~3);
+    float* hist = skew + 4 * 16 * SP;
+    const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int item = seq_xcd(blockIdx.x, gridDim.x);
+    const int bh = item / nqb, qblk = nqb - 1 - (item - bh * nqb), b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
+    const int qlen = seq_clamp_len(a.q_len, b, a.Nq), klen = seq_clamp_len(a.kv_len, b, a.Nk), pos0 = seq_pos(a.q_pos, b);
+    const int qb0 = qblk * (64 * QB), q0 = qb0 + wave * (16 * QB);
+    const T* Q = static_cast<const T*>(a.q.p) + b * a.q.batch + h * a.q.head;
+    const T* K = static_cast<const T*>(a.k.p) + b * a.k.batch + hk * a.k.head;
+    const T* V = static_cast<const T*>(a.v.p) + b * a.v.batch + hk * a.v.head;
+    const T* dO = static_cast<const T*>(a.dout.p) + b * a.dout.batch + h * a.dout.head;
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+    int kend = klen;
+    if (a.causal) kend = max(0, min(kend, pos0 + min(qb0 + 64 * QB, qlen)));
+    if (qb0 >= qlen) kend = 0;
+    const int t1 = (kend + TK - 1) / TK;
+
+    SeqFrag<T> qf[QB][KS], df[QB][KS];
+    float lse2[QB], dsum[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const int row = q0 + 16 * qb + l15;
+        const bool valid = row < qlen;
+        const long ri = (long)bh * a.Nq + row;
+        // a row without a visible key has lse = -inf: with +inf in its place its probabilities are zero
+        float ls = valid ? a.lse[ri] : -INFINITY;
+        lse2[qb] = ls == -INFINITY ? INFINITY : ls * SEQ_L2E;
+        const T* O = static_cast<const T*>(a.o.p) + b * a.o.batch + h * a.o.head + (long)row * a.o.row;
+        const float* O32 = a.o32 ? a.o32 + (((long)b * a.Nq + row) * a.H + h) * a.d : nullptr;
+        float ds = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            qf[qb][s] = seq_frag_row<T>(Q + (long)row * a.q.row, valid, s, g, a.d);
+            df[qb][s] = seq_frag_row<T>(dO + (long)row * a.dout.row, valid, s, g, a.d);
+            float x[8], y[8];
+            if constexpr (G::ES == 2) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = (float)df[qb][s].v[e];
+                if (O32) {
+                    const SeqFrag<float> f = seq_frag_row<float>(O32, valid, s, g, a.d);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = f.v[e >> 2][e & 3];
+                } else {
+                    const SeqFrag<T> f = seq_frag_row<T>(O, valid, s, g, a.d);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = (float)f.v[e];
+                }
+            } else {
+                const SeqFrag<T> f = seq_frag_row<T>(O, valid, s, g, a.d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { x[e] = df[qb][s].v[e >> 2][e & 3]; y[e] = f.v[e >> 2][e & 3]; }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ds = __builtin_fmaf(x[e], y[e], ds);
+        }
+        dsum[qb] = seq_group_sum(ds);
+        if (g == 0 && row < a.Nq) a.dvec[ri] = dsum[qb];
+    }
+    const float scale2 = a.scale * SEQ_L2E;
+    f32x4 acc[QB][G::DA];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int t = 0; t < G::DA; ++t) acc[qb][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float far_l = 0.f, far_r = 0.f;
+    SeqSlots<T, DT> sk, sv;
+    sk.init(a.k.row, a.d, tid);
+    sv.init(a.v.row, a.d, tid);
+    if constexpr (BIAS) seq_bias_fill(bw, a, h, PAD, tid);
+    float* sw = skew + wave * 16 * SP;
+    float* hw = hist + wave * W;
+    if constexpr (TAB) {
+        for (int i = lane; i < 16 * SP; i += 64) sw[i] = 0.f;
+        for (int i = lane; i < W; i += 64) hw[i] = 0.f;
+    }
+    const int wbase = wave * 1024;
+    auto stage = [&](int t, unsigned long long live) {
+        char* dst = lds_seq + (t & 1) * STAGE + wbase;
+        sk.dma(K + (long)t * TK * a.k.row, dst, live, tid);
+        sv.dma(V + (long)t * TK * a.v.row, dst + G::TILE, live, tid);
+    };
+    unsigned long long live = 0, next = 0;
+    if (0 < t1) { next = seq_live<TK>(mask, 0, klen, lane); stage(0, next); }
+    for (int t = 0; t < t1; ++t) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        live = next;
+        if (t + 1 < t1) { next = seq_live<TK>(mask, (t + 1) * TK, klen, lane); stage(t + 1, next); }
+        if (live == 0) continue;
+        const char* Ks = lds_seq + (t & 1) * STAGE;
+        const char* Vs = Ks + G::TILE;
+        const int k0 = t * TK, p0 = pos0 + q0;
+        f32x4 s[QB][KT], dp[QB][KT];
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) { s[qb][kt] = (f32x4){0.f, 0.f, 0.f, 0.f}; dp[qb][kt] = s[qb][kt]; }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const SeqFrag<T> kf = seq_frag_lds<T, DT>(Ks, kt, ks, l15, g);
+                const SeqFrag<T> vf = seq_frag_lds<T, DT>(Vs, kt, ks, l15, g);
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) {
+                    s[qb][kt] = seq_mma(kf, qf[qb][ks], s[qb][kt]);
+                    dp[qb][kt] = seq_mma(vf, df[qb][ks], dp[qb][kt]);
+                }
+            }
+        float cb = 0.f, sc = scale2;
+        int side = 0;                                             // -1 / 1: past the table's range on the left / right, 0: by distance
+        if constexpr (BIAS) {
+            const int hi = k0 + TK - 1 - p0, lo = k0 - p0 - (16 * QB - 1);
+            if (hi <= -a.D) { cb = bw[PAD]; side = -1; }
+            else if (lo >= a.D) { cb = bw[2 * a.D + PAD]; side = 1; }
+            else {
+                const float* w = bw + (k0 + 4 * g - p0 - l15 + a.D + PAD);
+                sc = 1.f;
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[qb][kt][r] = __builtin_fmaf(s[qb][kt][r], scale2, w[16 * kt + r - 16 * qb]);
+            }
+        }
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            const float off = cb - lse2[qb];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][kt][r], sc, off));
+                    s[qb][kt][r] = p * (dp[qb][kt][r] - dsum[qb]);
+                }
+        }
+        const bool full = live == (TK == 64 ? ~0ull : 0xFFFFFFFFull) && (!a.causal || k0 + TK - 1 <= p0);
+        if (!full) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const unsigned nib = (unsigned)(live >> (16 * kt + 4 * g)) & 15u;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool ok = ((nib >> r) & 1u) && (!a.causal || k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15);
+                        s[qb][kt][r] = ok ? s[qb][kt][r] : 0.f;
+                    }
+                }
+        }
+        if constexpr (TAB) {
+            if (side != 0) {
+                float sum = 0.f;
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) sum += (s[qb][kt][0] + s[qb][kt][1]) + (s[qb][kt][2] + s[qb][kt][3]);
+                if (side < 0) far_l += sum; else far_r += sum;
+            } else {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    f32x4 x = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb) {
+                        const int kt = e - (QB - 1) + qb;
+                        if (kt >= 0 && kt < KT) x += s[qb][kt];
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sw[l15 * SP + 16 * e + 4 * g + r + 15 - l15] = x[r];
+                }
+                asm volatile("" ::: "memory");                    // one wave's LDS accesses execute in order
+                float* hb = hw + (k0 - p0 - 16 * (QB - 1) - 15 + a.D + PAD);
+                for (int c = lane; c < S::NCOL; c += 64) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x += sw[i * SP + c];
+                    hb[c] += x;
+                }
+                asm volatile("" ::: "memory");
+            }
+        }
+        seq_tmul<T, DT, QB>(acc, Ks, s, l15, g);
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const int row = q0 + 16 * qb + l15;
+        if (row >= a.Nq) continue;
+        T* dQ = static_cast<T*>(a.dq.p) + b * a.dq.batch + h * a.dq.head + (long)row * a.dq.row;
+        seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(dQ + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
+    }
+    if constexpr (TAB) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { far_l += __shfl_xor(far_l, o, 64); far_r += __shfl_xor(far_r, o, 64); }
+        asm volatile("" ::: "memory");
+        if (lane == 0) { hw[0] += far_l; hw[W - 1] += far_r; }
+        __syncthreads();
+        for (int i = tid; i < W; i += 256) hist[i] = (hist[i] + hist[W + i]) + (hist[2 * W + i] + hist[3 * W + i]);
+        __syncthreads();
+        float* out = a.tpart + ((long)bh * nqb + qblk) * a.nb;
+        for (int c = wave; c < a.nb; c += 4) {
+            const int lo = a.brange[2 * c], hi = a.brange[2 * c + 1];           // distances + D of the bucket, [lo, hi)
+            float x = 0.f;
+            if (lo < hi) {
+                const int i0 = lo == 0 ? 0 : lo + PAD, i1 = hi == 2 * a.D + 1 ? W : hi + PAD;
+                for (int i = i0 + lane; i < i1; i += 64) x += hist[i];
+            }
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+            if (lane == 0) out[c] = x;
+        }
+    }
+#endif
+}
+
+// dtable[c][h] = sum over samples and query blocks of their parts; one wave a (bucket, head), 64-bit sums
+__global__ __launch_bounds__(64) void seq_dtable_kernel(const SeqArgs a, const int nqb) {
+    const int c = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
+    double x = 0.0;
+    for (int i = lane; i < a.B * nqb; i += 64) {
+        const int b = i / nqb, y = i - b * nqb;
+        x += (double)a.tpart[(((long)b * a.H + h) * nqb + y) * a.nb + c];
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+    if (lane == 0) a.dtable[(long)c * a.H + h] = (float)x;
+}
+
+template <typename T, int DT, int KB, bool BIAS> struct SeqDkv {
+    using G = SeqGeo<T, DT>;
+    static constexpr int PAD = G::TK + 16 * KB;
+    static int lds(int D) { return 4 * G::TILE + 4 * G::TK * 4 + (BIAS ? (int)rup((2 * (D + PAD) + 1) * 4, 16) : 0); }
+};
+
+template <typename T, int DT, int KB, bool BIAS>
+__global__ __launch_bounds__(256) void seq_dkv_kernel(const SeqArgs a, const int nkb) {
+#ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
+    using G = SeqGeo<T, DT>;
+    constexpr int TQ = G::TK, QT = G::KT, KS = G::KS, STAGE = 2 * G::TILE, PAD = SeqDkv<T, DT, KB, BIAS>::PAD;
+    extern __shared__ __attribute__((aligned(16))) char lds_seq[];
+    float* rows = reinterpret_cast<float*>(lds_seq + 2 * STAGE);      // [2 stages][lse, D][TQ]
+    float* bw = rows + 4 * TQ;
+    const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int item = seq_xcd(blockIdx.x, gridDim.x);
+    const int bk = item / nkb, kblk = item - bk * nkb, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+    const int split = blockIdx.y;
+    const int qlen = seq_clamp_len(a.q_len, b, a.Nq), klen = seq_clamp_len(a.kv_len, b, a.Nk), pos0 = seq_pos(a.q_pos, b);
+    const int kb0 = kblk * (64 * KB), k0 = kb0 + wave * (16 * KB);
+    const T* K = static_cast<const T*>(a.k.p) + b * a.k.batch + hk * a.k.head;
+    const T* V = static_cast<const T*>(a.v.p) + b * a.v.batch + hk * a.v.head;
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+
+    SeqFrag<T> kf[KB][KS], vf[KB][KS];
+    bool seen[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+        const int key = k0 + 16 * kb + l15;
+        seen[kb] = key < klen && (!mask || mask[key] != 0);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            kf[kb][s] = seq_frag_row<T>(K + (long)key * a.k.row, seen[kb], s, g, a.d);
+            vf[kb][s] = seq_frag_row<T>(V + (long)key * a.v.row, seen[kb], s, g, a.d);
+        }
+    }
+    // steps: the query tiles that can see this block's keys, head after head of those that share them
+    const int tq0 = a.causal ? max(0, kb0 - pos0) / TQ : 0;
+    const int n1 = kb0 < klen ? max(0, (qlen + TQ - 1) / TQ - tq0) : 0;
+    int u0 = 0, u1 = n1 * a.G;
+    if (a.nsplit > 1) {
+        const int per = (u1 + a.nsplit - 1) / a.nsplit;
+        u0 = min(split * per, u1); u1 = min(u0 + per, u1);
+    }
+    f32x4 dk[KB][G::DA], dv[KB][G::DA];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int t = 0; t < G::DA; ++t) { dk[kb][t] = (f32x4){0.f, 0.f, 0.f, 0.f}; dv[kb][t] = dk[kb][t]; }
+    SeqSlots<T, DT> sq, sd;
+    sq.init(a.q.row, a.d, tid);
+    sd.init(a.dout.row, a.d, tid);
+    const float scale2 = a.scale * SEQ_L2E;
+    const int wbase = wave * 1024;
+    float ls = 0.f, dd = 0.f;
+    // per-row numbers of a tile: fetched ahead of its DMA, written to LDS at the end of the step that fetched them
+    auto fetch = [&](int u) {
+        const int h = hk * a.G + u / n1, row = (tq0 + u % n1) * TQ + tid;
+        if (tid < TQ) {
+            ls = INFINITY; dd = 0.f;
+            if (row < qlen) {
+                const long ri = ((long)b * a.H + h) * a.Nq + row;
+                const float x = a.lse[ri];
+                ls = x == -INFINITY ? INFINITY : x * SEQ_L2E;
+                dd = a.dvec[ri];
+            }
+        }
+    };
+    auto stage = [&](int u) {
+        const int h = hk * a.G + u / n1, r0 = (tq0 + u % n1) * TQ;
+        char* dst = lds_seq + (u & 1) * STAGE + wbase;
+        const unsigned long long live = seq_live<TQ>(nullptr, r0, qlen, lane);
+        sq.dma(static_cast<const T*>(a.q.p) + b * a.q.batch + h * a.q.head + (long)r0 * a.q.row, dst, live, tid);
+        sd.dma(static_cast<const T*>(a.dout.p) + b * a.dout.batch + h * a.dout.head + (long)r0 * a.dout.row, dst + G::TILE, live, tid);
+    };
+    auto put = [&](int u) {
+        if (tid < TQ) { float* w = rows + (u & 1) * 2 * TQ; w[tid] = ls; w[TQ + tid] = dd; }
+    };
+    if (u0 < u1) { fetch(u0); stage(u0); put(u0); }
+    int hcur = -1;
+    for (int u = u0; u < u1; ++u) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int h = hk * a.G + u / n1;
+        if (BIAS && h != hcur) { seq_bias_fill(bw, a, h, PAD, tid); hcur = h; __syncthreads(); }
+        if (u + 1 < u1) { fetch(u + 1); stage(u + 1); }
+        const char* Qs = lds_seq + (u & 1) * STAGE;
+        const char* Ds = Qs + G::TILE;
+        const float* rw = rows + (u & 1) * 2 * TQ;
+        const int q0 = (tq0 + u % n1) * TQ, p0 = pos0 + q0;
+        f32x4 s[KB][QT], dp[KB][QT];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) { s[kb][qt] = (f32x4){0.f, 0.f, 0.f, 0.f}; dp[kb][qt] = s[kb][qt]; }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+                const SeqFrag<T> qf = seq_frag_lds<T, DT>(Qs, qt, ks, l15, g);
+                const SeqFrag<T> df = seq_frag_lds<T, DT>(Ds, qt, ks, l15, g);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    s[kb][qt] = seq_mma(qf, kf[kb][ks], s[kb][qt]);
+                    dp[kb][qt] = seq_mma(df, vf[kb][ks], dp[kb][qt]);
+                }
+            }
+        float cb = 0.f, sc = scale2;
+        if constexpr (BIAS) {
+            const int hi = k0 + 16 * KB - 1 - p0, lo = k0 - p0 - (TQ - 1);
+            if (hi <= -a.D) cb = bw[PAD];
+            else if (lo >= a.D) cb = bw[2 * a.D + PAD];
+            else {
+                const float* w = bw + (k0 + l15 - p0 - 4 * g + a.D + PAD);
+                sc = 1.f;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[kb][qt][r] = __builtin_fmaf(s[kb][qt][r], scale2, w[16 * kb - 16 * qt - r]);
+            }
+        }
+        const bool full = !a.causal || k0 + 16 * KB - 1 <= p0;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+            const f32x4 lq = *reinterpret_cast<const f32x4*>(rw + 16 * qt + 4 * g), dq = *reinterpret_cast<const f32x4*>(rw + TQ + 16 * qt + 4 * g);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][qt][r], sc, cb - lq[r]));
+                    if (!full) p = (k0 + 16 * kb + l15 <= p0 + 16 * qt + 4 * g + r) ? p : 0.f;
+                    s[kb][qt][r] = p;
+                    dp[kb][qt][r] = p * (dp[kb][qt][r] - dq[r]);
+                }
+        }
+        seq_tmul<T, DT, KB>(dv, Ds, s, l15, g);
+        seq_tmul<T, DT, KB>(dk, Qs, dp, l15, g);
+        if (u + 1 < u1) put(u + 1);
+    }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+        const int key = k0 + 16 * kb + l15;
+        if (key >= a.Nk) continue;
+        const float f = seen[kb] ? 1.f : 0.f, fs = seen[kb] ? a.scale : 0.f;
+        const bool hid = !seen[kb];
+        if (a.nsplit > 1) {
+            const long n = (long)a.B * a.Hkv * a.Nk, ri = (long)bk * a.Nk + key;
+            float* P = a.part + ((long)split * 2 * n + ri) * a.d;
+            seq_row4<T, DT>(dk[kb], a.d, g, [&](int c, float4 v) { st4(P + c, hid ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * fs, v.y * fs, v.z * fs, v.w * fs)); });
+            P += n * a.d;
+            seq_row4<T, DT>(dv[kb], a.d, g, [&](int c, float4 v) { st4(P + c, hid ? make_float4(0.f, 0.f, 0.f, 0.f) : v); });
+            continue;
+        }
+        T* dK = static_cast<T*>(a.dk.p) + b * a.dk.batch + hk * a.dk.head + (long)key * a.dk.row;
+        T* dV = static_cast<T*>(a.dv.p) + b * a.dv.batch + hk * a.dv.head + (long)key * a.dv.row;
+        seq_row4<T, DT>(dk[kb], a.d, g, [&](int c, float4 v) { st4(dK + c, hid ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * fs, v.y * fs, v.z * fs, v.w * fs)); });
+        seq_row4<T, DT>(dv[kb], a.d, g, [&](int c, float4 v) { st4(dV + c, hid ? make_float4(0.f, 0.f, 0.f, 0.f) : v); });
+    }
+#endif
+}
+
+// dk, dv = sum of the parts of a split query axis, in order; one thread per 4 columns
+template <typename T>
+__global__ __launch_bounds__(256) void seq_dkv_sum_kernel(const SeqArgs a) {
+    const int d4 = a.d >> 2;
+    const long n = (long)a.B * a.Hkv * a.Nk, i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= 2 * n * d4) return;
+    const long rr = i / d4;
+    const int c = (int)(i - rr * d4) * 4;
+    const bool isv = rr >= n;
+    const long ri = isv ? rr - n : rr;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float4 v = ld4(a.part + ((long)s * 2 * n + rr) * a.d + c);
+        x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
+    }
+    const long bk = ri / a.Nk, key = ri - bk * a.Nk, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+    const SeqT& t = isv ? a.dv : a.dk;
+    st4(static_cast<T*>(t.p) + b * t.batch + hk * t.head + key * t.row + c, x);
+}
+
+// ---------------------------------------------------------------- host side
+SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable) {
+    SeqBwdPlan p;
+    p.qb = 1; p.kb = 1; p.qsplit = 1;
+    p.nqb = (int)cdiv(a.Nq, 64 * p.qb);
+    p.dvec = (size_t)rup((long)a.B * a.H * a.Nq * 4, 256);
+    p.tpart = want_dtable ? (size_t)rup((long)a.B * a.H * p.nqb * a.nb * 4, 256) : 0;
+    p.part = p.qsplit > 1 ? (size_t)p.qsplit * 2 * a.B * a.Hkv * a.Nk * a.d * 4 : 0;
+    p.total = p.dvec + p.tpart + p.part;
+    return p;
+}
+template <typename T, int DT, int QB, bool BIAS, bool TAB>
+static void dq_go(const Launch& L, const SeqArgs& a, int nqb) {
+    if (!((long)nqb * a.B)) return;
+    L.count();
+    if (L.dry) return;
+    const int lds = SeqDq<T, DT, QB, BIAS, TAB>::lds(a.D);
+    set_dyn_lds(reinterpret_cast<const void*>(&seq_dq_kernel<T, DT, QB, BIAS, TAB>), 160 * 1024);
+    hipLaunchKernelGGL((seq_dq_kernel<T, DT, QB, BIAS, TAB>), dim3((unsigned)nqb * a.B * a.H), dim3(256), lds, L.stream, a, nqb);
+    CB_HIP(hipGetLastError());
+}
+template <typename T, int DT, int KB, bool BIAS>
+static void dkv_go(const Launch& L, const SeqArgs& a) {
+    const int nkb = (int)cdiv(a.Nk, 64 * KB);
+    if (!((long)nkb * a.B)) return;
+    L.count();
+    if (L.dry) return;
+    const int lds = SeqDkv<T, DT, KB, BIAS>::lds(a.D);
+    set_dyn_lds(reinterpret_cast<const void*>(&seq_dkv_kernel<T, DT, KB, BIAS>), 160 * 1024);
+    hipLaunchKernelGGL((seq_dkv_kernel<T, DT, KB, BIAS>), dim3((unsigned)nkb * a.B * a.Hkv, a.nsplit), dim3(256), lds, L.stream, a, nkb);
+    CB_HIP(hipGetLastError());
+}
+template <typename T, int DT>
+static void bwd_pick(const Launch& L, const SeqArgs& a, const SeqBwdPlan& p) {
+    if (a.table && a.dtable) dq_go<T, DT, 1, true, true>(L, a, p.nqb);
+    else if (a.table) dq_go<T, DT, 1, true, false>(L, a, p.nqb);
+    else dq_go<T, DT, 1, false, false>(L, a, p.nqb);
+    if (a.table) dkv_go<T, DT, 1, true>(L, a);
+    else dkv_go<T, DT, 1, false>(L, a);
+}
+void seq_backward(const Launch& L, SeqArgs a, void* ws) {
+    const SeqBwdPlan p = seq_bwd_plan(a, a.dtable != nullptr);
+    char* w = static_cast<char*>(ws);
+    a.dvec = reinterpret_cast<float*>(w); w += p.dvec;
+    a.tpart = reinterpret_cast<float*>(w); w += p.tpart;
+    a.part = reinterpret_cast<float*>(w);
+    a.nsplit = p.qsplit;
+    CB_DT_SWITCH(a.dt, T, SEQ_DT_SWITCH(a.d, DT, bwd_pick<T, DT>(L, a, p)));
+    if (a.dtable) {
+        L.count();
+        if (!L.dry) {
+            hipLaunchKernelGGL(seq_dtable_kernel, dim3(a.nb, a.H), dim3(64), 0, L.stream, a, p.nqb);
+            CB_HIP(hipGetLastError());
+        }
+    }
+    if (a.nsplit > 1 && (long)a.B * a.Nk) {
+        L.count();
+        if (L.dry) return;
+        CB_DT_SWITCH(a.dt, T, hipLaunchKernelGGL((seq_dkv_sum_kernel<T>), dim3(cdiv(2L * a.B * a.Hkv * a.Nk * (a.d / 4), 256)), dim3(256), 0, L.stream, a));
+        CB_HIP(hipGetLastError());
+    }
+}
+
+}  // namespace cb

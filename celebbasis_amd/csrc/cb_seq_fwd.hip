@@ -1,0 +1,252 @@
+// cb_seq_fwd.hip — forward of the attention of cb_seq.h (lengths, key masks, shared heads, relative position bias).
+//
+// One pass over the keys with the running maximum and sum of the softmax: S^T = K Q^T, p = exp2(s - m), O^T += V^T P^T, the probabilities
+// going from the first product's accumulators into the second's operand inside the lane. A block has 4 waves of 16 QB queries of one (sample,
+// head); K and V tiles come by LDS-DMA into a ring of two stages (one wait and one barrier a tile).
+#include "cb_seq.h"
+
+namespace cb {
+
+template <typename T, int DT, int QB, bool BIAS>
+__global__ __launch_bounds__(256) void seq_fwd_kernel(const SeqArgs a, const int nqb) {
+#ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
+    using G = SeqGeo<T, DT>;
+    constexpr int TK = G::TK, KT = G::KT, KS = G::KS, STAGE = 2 * G::TILE, PAD = TK + 16 * QB;
+    extern __shared__ __attribute__((aligned(16))) char lds_seq[];
+    float* bw = reinterpret_cast<float*>(lds_seq + 2 * STAGE);
+    const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int item = seq_xcd(blockIdx.x, gridDim.x);
+    const int bh = item / nqb, qblk = nqb - 1 - (item - bh * nqb), b = bh / a.H, h = bh - b * a.H, hk = h / a.G;     // causal: the long rows first
+    const int split = blockIdx.y;
+    const int qlen = seq_clamp_len(a.q_len, b, a.Nq), klen = seq_clamp_len(a.kv_len, b, a.Nk), pos0 = seq_pos(a.q_pos, b);
+    const int qb0 = qblk * (64 * QB), q0 = qb0 + wave * (16 * QB);
+    const T* Q = static_cast<const T*>(a.q.p) + b * a.q.batch + h * a.q.head;
+    const T* K = static_cast<const T*>(a.k.p) + b * a.k.batch + hk * a.k.head;
+    const T* V = static_cast<const T*>(a.v.p) + b * a.v.batch + hk * a.v.head;
+    const unsigned char* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+
+    // keys this block has to look at: up to the sample's length and, causal, the block's last position
+    int kend = klen;
+    if (a.causal) kend = max(0, min(kend, pos0 + min(qb0 + 64 * QB, qlen)));
+    if (qb0 >= qlen) kend = 0;
+    int t0 = 0, t1 = (kend + TK - 1) / TK;
+    if (a.nsplit > 1) {
+        const int per = (t1 + a.nsplit - 1) / a.nsplit;
+        t0 = min(split * per, t1); t1 = min(t0 + per, t1);
+    }
+
+    SeqFrag<T> qf[QB][KS];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int row = q0 + 16 * qb + l15;
+            qf[qb][s] = seq_frag_row<T>(Q + (long)row * a.q.row, row < qlen, s, g, a.d);
+        }
+    const float scale2 = a.scale * SEQ_L2E;
+    f32x4 o[QB][G::DA];
+    float m[QB], l[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        m[qb] = -INFINITY; l[qb] = 0.f;
+#pragma unroll
+        for (int t = 0; t < G::DA; ++t) o[qb][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    SeqSlots<T, DT> sk, sv;
+    sk.init(a.k.row, a.d, tid);
+    sv.init(a.v.row, a.d, tid);
+    if constexpr (BIAS) seq_bias_fill(bw, a, h, PAD, tid);
+    const int wbase = wave * 1024;
+    auto stage = [&](int t, unsigned long long live) {
+        char* dst = lds_seq + (t & 1) * STAGE + wbase;
+        sk.dma(K + (long)t * TK * a.k.row, dst, live, tid);
+        sv.dma(V + (long)t * TK * a.v.row, dst + G::TILE, live, tid);
+    };
+    unsigned long long live = 0, next = 0;
+    if (t0 < t1) { next = seq_live<TK>(mask, t0 * TK, klen, lane); stage(t0, next); }
+    for (int t = t0; t < t1; ++t) {
+        // tile t has landed for this wave and, behind the barrier, for all; everybody has read the other stage, which is filled next
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        live = next;
+        if (t + 1 < t1) { next = seq_live<TK>(mask, (t + 1) * TK, klen, lane); stage(t + 1, next); }
+        if (live == 0) continue;
+        const char* Ks = lds_seq + (t & 1) * STAGE;
+        const char* Vs = Ks + G::TILE;
+        const int k0 = t * TK;
+        f32x4 s[QB][KT];
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) s[qb][kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const SeqFrag<T> kf = seq_frag_lds<T, DT>(Ks, kt, ks, l15, g);
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) s[qb][kt] = seq_mma(kf, qf[qb][ks], s[qb][kt]);
+            }
+        // the bias: one number for the whole tile where every distance is past the table's range, else by distance from LDS; s is then in the
+        // log2 domain already (sc = 1)
+        const int p0 = pos0 + q0;
+        float cb = 0.f, sc = scale2;
+        if constexpr (BIAS) {
+            const int hi = k0 + TK - 1 - p0, lo = k0 - p0 - (16 * QB - 1);
+            if (hi <= -a.D) cb = bw[PAD];
+            else if (lo >= a.D) cb = bw[2 * a.D + PAD];
+            else {
+                const float* w = bw + (k0 + 4 * g - p0 - l15 + a.D + PAD);
+                sc = 1.f;
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[qb][kt][r] = __builtin_fmaf(s[qb][kt][r], scale2, w[16 * kt + r - 16 * qb]);
+            }
+        }
+        const bool full = live == (TK == 64 ? ~0ull : 0xFFFFFFFFull) && (!a.causal || k0 + TK - 1 <= p0);
+        if (!full) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    const unsigned nib = (unsigned)(live >> (16 * kt + 4 * g)) & 15u;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool ok = ((nib >> r) & 1u) && (!a.causal || k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15);
+                        s[qb][kt][r] = ok ? s[qb][kt][r] : -INFINITY;
+                    }
+                }
+        }
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[qb][kt][r]);
+            mx = __builtin_fmaf(seq_group_max(mx), sc, cb);
+            const float mnew = fmaxf(m[qb], mx);
+            const float off = (mnew == -INFINITY) ? 0.f : cb - mnew;
+            float ps = 0.f;
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][kt][r], sc, off));
+                    s[qb][kt][r] = p;
+                    ps += p;
+                }
+            if (!__all(mnew == m[qb])) {
+                const float alpha = __builtin_amdgcn_exp2f(m[qb] - (mnew == -INFINITY ? 0.f : mnew));
+#pragma unroll
+                for (int t2 = 0; t2 < G::DA; ++t2) o[qb][t2] *= alpha;
+                l[qb] *= alpha;
+                m[qb] = mnew;
+            }
+            l[qb] += seq_group_sum(ps);
+        }
+        seq_tmul<T, DT, QB>(o, Vs, s, l15, g);
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const int row = q0 + 16 * qb + l15;
+        if (row >= a.Nq) continue;
+        const long ri = (long)bh * a.Nq + row;
+        if (row >= qlen) l[qb] = 0.f;            // a row behind the sample's last query sees nothing
+        if (a.nsplit > 1) {                      // unnormalised; seq_combine_kernel joins the parts
+            float* P = a.part + ((long)split * a.B * a.H * a.Nq + ri) * a.d;
+            seq_row4<T, DT>(o[qb], a.d, g, [&](int c, float4 v) { st4(P + c, v); });
+            if (g == 0) { float* w = a.ml + ((long)split * a.B * a.H * a.Nq + ri) * 2; w[0] = m[qb]; w[1] = l[qb]; }
+            continue;
+        }
+        const bool none = l[qb] == 0.f;          // nothing visible: zeros
+        const float inv = none ? 0.f : 1.f / l[qb];
+        T* O = static_cast<T*>(a.o.p) + b * a.o.batch + h * a.o.head + (long)row * a.o.row;
+        float* O32 = a.o32 ? a.o32 + (((long)b * a.Nq + row) * a.H + h) * a.d : nullptr;
+        seq_row4<T, DT>(o[qb], a.d, g, [&](int c, float4 v) {
+            v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            st4(O + c, v);
+            if (O32) st4(O32 + c, v);
+        });
+        if (g == 0 && a.lse) a.lse[ri] = none ? -INFINITY : (m[qb] + __builtin_amdgcn_logf(l[qb])) * SEQ_LN2;
+    }
+#endif
+}
+
+// joins the parts of a split key axis: o = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), s in order. One thread per 4 columns.
+template <typename T>
+__global__ __launch_bounds__(256) void seq_combine_kernel(const SeqArgs a) {
+    const int d4 = a.d >> 2;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, rows = (long)a.B * a.H * a.Nq;
+    if (i >= rows * d4) return;
+    const long ri = i / d4;
+    const int c = (int)(i - ri * d4) * 4;
+    float m = -INFINITY;
+    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, a.ml[(s * rows + ri) * 2]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.nsplit; ++s) {
+        const float2 w = *reinterpret_cast<const float2*>(a.ml + (s * rows + ri) * 2);
+        if (w.y == 0.f) continue;                // a part without visible keys
+        const float f = __builtin_amdgcn_exp2f(w.x - (m == -INFINITY ? 0.f : m));
+        const float4 v = ld4(a.part + (s * rows + ri) * a.d + c);
+        l = __builtin_fmaf(w.y, f, l);
+        o.x = __builtin_fmaf(v.x, f, o.x); o.y = __builtin_fmaf(v.y, f, o.y); o.z = __builtin_fmaf(v.z, f, o.z); o.w = __builtin_fmaf(v.w, f, o.w);
+    }
+    const bool none = l == 0.f;
+    const float inv = none ? 0.f : 1.f / l;
+    const long bh = ri / a.Nq, row = ri - bh * a.Nq, b = bh / a.H, h = bh - b * a.H;
+    const float4 v = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    st4(static_cast<T*>(a.o.p) + b * a.o.batch + h * a.o.head + row * a.o.row + c, v);
+    if (a.o32) st4(a.o32 + ((b * a.Nq + row) * a.H + h) * a.d + c, v);
+    if (c == 0 && a.lse) a.lse[ri] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * SEQ_LN2;
+}
+
+// ---------------------------------------------------------------- host side
+SeqPlan seq_fwd_plan(const SeqArgs& a) {
+    SeqPlan p;
+    p.qb = 1;
+    p.nsplit = 1;
+    if (p.nsplit > 1) {
+        p.part = (size_t)p.nsplit * a.B * a.H * a.Nq * a.d * 4;
+        p.ml = (size_t)p.nsplit * a.B * a.H * a.Nq * 2 * 4;
+    }
+    p.total = p.part + p.ml;
+    return p;
+}
+template <typename T, int DT, int QB, bool BIAS>
+static void fwd_go(const Launch& L, const SeqArgs& a) {
+    using G = SeqGeo<T, DT>;
+    const int nqb = (int)cdiv(a.Nq, 64 * QB);
+    const int lds = 4 * G::TILE + (BIAS ? (int)rup((2 * (a.D + G::TK + 16 * QB) + 1) * 4, 16) : 0);
+    L.count();
+    if (L.dry) return;
+    set_dyn_lds(reinterpret_cast<const void*>(&seq_fwd_kernel<T, DT, QB, BIAS>), 160 * 1024);
+    hipLaunchKernelGGL((seq_fwd_kernel<T, DT, QB, BIAS>), dim3((unsigned)nqb * a.B * a.H, a.nsplit), dim3(256), lds, L.stream, a, nqb);
+    CB_HIP(hipGetLastError());
+}
+template <typename T, int DT>
+static void fwd_pick(const Launch& L, const SeqArgs& a, int qb) {
+    if (a.table) fwd_go<T, DT, 1, true>(L, a);
+    else fwd_go<T, DT, 1, false>(L, a);
+}
+void seq_forward(const Launch& L, SeqArgs a, void* ws) {
+    const SeqPlan p = seq_fwd_plan(a);
+    a.nsplit = p.nsplit;
+    a.part = static_cast<float*>(ws);
+    a.ml = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part);
+    CB_DT_SWITCH(a.dt, T, SEQ_DT_SWITCH(a.d, DT, fwd_pick<T, DT>(L, a, p.qb)));
+    if (a.nsplit > 1) {
+        L.count();
+        if (L.dry) return;
+        CB_DT_SWITCH(a.dt, T, hipLaunchKernelGGL((seq_combine_kernel<T>), dim3(cdiv((long)a.B * a.H * a.Nq * (a.d / 4), 256)), dim3(256), 0, L.stream, a));
+        CB_HIP(hipGetLastError());
+    }
+}
+
+}  // namespace cb

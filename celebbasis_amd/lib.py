@@ -72,6 +72,21 @@ class AttentionDesc(_Sized):
                 ("out", C.c_void_p), ("dout", C.c_void_p), ("dqbuf", C.c_void_p), ("dkvbuf", C.c_void_p), ("dtype", C.c_int)]
 
 
+class SeqTensor(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("row", C.c_int64), ("head", C.c_int64), ("batch", C.c_int64)]
+
+
+class SeqAttentionDesc(_Sized):
+    _fields_ = [("struct_size", C.c_int), ("dtype", C.c_int),
+                ("B", C.c_int), ("Nq", C.c_int), ("Nk", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("d", C.c_int),
+                ("scale", C.c_float), ("causal", C.c_int),
+                ("q", SeqTensor), ("k", SeqTensor), ("v", SeqTensor), ("out", SeqTensor),
+                ("q_pos", C.c_void_p), ("q_len", C.c_void_p), ("kv_len", C.c_void_p), ("kv_mask", C.c_void_p), ("mask_stride", C.c_int64),
+                ("relpos", C.c_void_p), ("table", C.c_void_p), ("lse", C.c_void_p), ("out32", C.c_void_p),
+                ("dout", SeqTensor), ("dq", SeqTensor), ("dk", SeqTensor), ("dv", SeqTensor), ("dtable", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 class UNetCfg(C.Structure):
     _fields_ = [("in_channels", C.c_int), ("out_channels", C.c_int), ("model_channels", C.c_int), ("num_res_blocks", C.c_int),
                 ("channel_mult", C.c_int * 8), ("n_mult", C.c_int),
@@ -116,6 +131,7 @@ ABI_SYMBOLS = [
     "cb_clip_backward_embeds", "cb_frnet_create", "cb_frnet_destroy", "cb_frnet_forward", "cb_trainer_cfg_default",
     "cb_trainer_create", "cb_trainer_destroy", "cb_trainer_step", "cb_trainer_get_state", "cb_trainer_set_state",
     "cb_debug_force_plan", "cb_trainer_prefetch", "cb_trainer_set_graph_replay", "cb_trainer_graph_stats", "cb_trainer_prefetch_stream", "cb_trainer_set_prefetch_stream", "cb_trainer_loss_to", "cb_celeb_head_forward", "cb_face_augment", "cb_paste_on_canvas", "cb_row_surgery_multi", "cb_trainer_share_unet", "cb_trainer_share_clip", "cb_unet_ddim_sample", "cb_ddim_update", "cb_vae_decoder_create", "cb_vae_decoder_destroy", "cb_vae_decode",
+    "cb_relpos_create", "cb_relpos_destroy", "cb_relpos_bucket", "cb_seq_attention_workspace", "cb_seq_attention_fwd", "cb_seq_attention_bwd",
 ]
 
 
@@ -161,6 +177,8 @@ _ARGTYPES = {
     "cb_ddim_update": [_P, _P, _P, _P, _I, _I, _I, _I, _F, _F, _F, _F, _F, _P],
     "cb_vae_decoder_create": [_P, _P, C.c_char_p, _P, _P], "cb_vae_decoder_destroy": [_P],
     "cb_vae_decode": [_P, _P, _I, _I, _I, _F, _I, _P],
+    "cb_relpos_create": [_P, _I, _I, _I, _P], "cb_relpos_destroy": [_P], "cb_relpos_bucket": [_P, _L, _P],
+    "cb_seq_attention_workspace": [_P, _P, _I, _P], "cb_seq_attention_fwd": [_P, _P], "cb_seq_attention_bwd": [_P, _P],
 }
 
 
@@ -228,6 +246,7 @@ class Context:
             dev = torch.cuda.current_device() if device is None else device
             stream = C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
         self.device = dev
+        self.stream_ptr = stream.value or 0 if stream is not None else 0
         self.h = C.c_void_p()
         check(lib.cb_ctx_create_dtype(C.c_int(dev), stream, C.c_int(self.dtype), C.byref(self.h)))
 
@@ -651,3 +670,170 @@ class Trainer(_Handle):
     def set_state(self, name, value):
         v = value.detach().to(torch.float32).contiguous().cpu().reshape(-1)
         check(load().cb_trainer_set_state(self.h, name.encode(), C.c_void_p(v.data_ptr()), C.c_int64(v.numel())))
+
+
+# ---------------------------------------------------------------- sequence attention, residual RMS norm, 8-bit products
+# Outputs and workspaces of these calls come from torch's allocator on the context's stream, so the calls run on that stream and no other:
+# a caller whose current stream is another one is refused rather than raced (make the context under the stream that will capture).
+def _place(ctx, **tensors):
+    """every given tensor is on the context's device, and the current stream is the context's"""
+    if ctx.dry:
+        return
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.device.index != ctx.device):
+            raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+    if torch.cuda.current_stream(ctx.device).cuda_stream != ctx.stream_ptr:
+        raise ValueError("the current stream is not the stream the context was created on")
+
+
+def _device_of(ctx):
+    return torch.device("cpu") if ctx.dry else torch.device("cuda", ctx.device)
+
+
+def _workspace(ctx, n):
+    return torch.empty(n, dtype=torch.uint8, device=_device_of(ctx)) if n else None
+
+
+class RelPos(_Handle):
+    """buckets of a learned relative position bias (cb_relpos): a table [num_buckets, heads] is looked up by the distance key - query.
+    Keep the handle for as long as graphs captured with it are replayed."""
+    _destroy = "cb_relpos_destroy"
+
+    def __init__(self, ctx, num_buckets=32, max_distance=128, bidirectional=True):
+        self.ctx, self.num_buckets, self.max_distance, self.bidirectional = ctx, num_buckets, max_distance, bool(bidirectional)
+        self.h = C.c_void_p()
+        check(load().cb_relpos_create(ctx.h, int(num_buckets), int(max_distance), 1 if bidirectional else 0, C.byref(self.h)))
+
+    def bucket(self, relative):
+        """bucket of the distance `key position - query position`"""
+        out = C.c_int()
+        check(load().cb_relpos_bucket(self.h, int(relative), C.byref(out)))
+        return out.value
+
+
+def _seq_tensor(t, name, shape, dtype):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape} ([batch, tokens, heads, d])")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected dtype {dtype}, got {t.dtype}")
+    s = t.stride()
+    if s[3] != 1:
+        raise ValueError(f"{name}: the head dim must be contiguous")
+    # the stride of a dimension of one element says nothing: 0 passes every check
+    return SeqTensor(t.data_ptr() or None, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0, s[0] if shape[0] > 1 else 0)
+
+
+def _per_sample(t, name, B):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 tensor of shape ({B},), got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+class SeqTape:
+    """what the forward call leaves for its backward: the inputs (by reference), the output and its row statistics"""
+    __slots__ = ("q", "k", "v", "out", "lse", "out32", "kw")
+
+
+class SeqGrads:
+    __slots__ = ("dq", "dk", "dv", "dtable")
+
+
+def _seq_desc(ctx, q, k, v, scale, causal, q_pos, q_len, kv_len, kv_mask, relpos, table):
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q, k and v are [batch, tokens, heads, d]")
+    B, Nq, H, d = q.shape
+    Nk, Hkv = k.shape[1], k.shape[2]
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"q: expected float32 or bfloat16, got {q.dtype}")
+    _place(ctx, q=q, k=k, v=v, q_pos=q_pos, q_len=q_len, kv_len=kv_len, kv_mask=kv_mask, table=table)
+    D = SeqAttentionDesc()
+    D.dtype = DTYPE_BF16 if q.dtype == torch.bfloat16 else DTYPE_F32
+    D.B, D.Nq, D.Nk, D.heads, D.kv_heads, D.d = B, Nq, Nk, H, Hkv, d
+    D.scale, D.causal = d ** -0.5 if scale is None else float(scale), 1 if causal else 0
+    D.q = _seq_tensor(q, "q", (B, Nq, H, d), q.dtype)
+    D.k = _seq_tensor(k, "k", (B, Nk, Hkv, d), q.dtype)
+    D.v = _seq_tensor(v, "v", (B, Nk, Hkv, d), q.dtype)
+    D.q_pos, D.q_len, D.kv_len = _per_sample(q_pos, "q_pos", B), _per_sample(q_len, "q_len", B), _per_sample(kv_len, "kv_len", B)
+    if kv_mask is not None:
+        if kv_mask.dtype not in (torch.bool, torch.uint8) or tuple(kv_mask.shape) != (B, Nk) or (Nk > 1 and kv_mask.stride(1) != 1):
+            raise ValueError(f"kv_mask: expected bool or uint8 of shape ({B}, {Nk}) with contiguous rows, got {kv_mask.dtype} {tuple(kv_mask.shape)}")
+        D.kv_mask, D.mask_stride = kv_mask.data_ptr() or None, kv_mask.stride(0)
+    if (relpos is None) != (table is None):
+        raise ValueError("relpos and table go together")
+    if relpos is not None:
+        if table.dtype != torch.float32 or tuple(table.shape) != (relpos.num_buckets, H) or not table.is_contiguous():
+            raise ValueError(f"table: expected contiguous float32 of shape ({relpos.num_buckets}, {H}), got {table.dtype} {tuple(table.shape)}")
+        D.relpos, D.table = relpos.h, table.data_ptr()
+    return D
+
+
+def _seq_workspace(ctx, D, backward):
+    n = C.c_int64()
+    check(load().cb_seq_attention_workspace(ctx.h, C.byref(D), 1 if backward else 0, C.byref(n)))
+    ws = _workspace(ctx, n.value)
+    D.workspace, D.workspace_bytes = None if ws is None else ws.data_ptr(), n.value
+    return ws
+
+
+def seq_attention(ctx, q, k, v, scale=None, causal=False, q_pos=None, q_len=None, kv_len=None, kv_mask=None, relpos=None, table=None, out=None,
+                  need_grad=False):
+    """Attention over sequences (cb_seq_attention_fwd). q [B, Nq, heads, d], k / v [B, Nk, kv_heads, d], fp32 or bf16, views with a contiguous
+    head dim (slices of a fused projection, transposed caches); scale defaults to d ** -0.5.
+    causal: key j is visible to query i where j <= q_pos[b] + i. q_pos, q_len, kv_len: int32 [B] on the device (0, Nq, Nk by default).
+    kv_mask: bool or uint8 [B, Nk], non-zero = visible. relpos + table [num_buckets, heads]: learned bias by the distance key - query.
+    Rows at or beyond q_len and rows that see no key are 0.
+    Returns out [B, Nq, heads, d] (or `out`, written), with need_grad (out, tape) for seq_attention_backward."""
+    D = _seq_desc(ctx, q, k, v, scale, causal, q_pos, q_len, kv_len, kv_mask, relpos, table)
+    dev = q.device
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _place(ctx, out=out)
+    D.out = _seq_tensor(out, "out", tuple(q.shape), q.dtype)
+    lse = out32 = None
+    if need_grad:
+        lse = torch.empty((D.B, D.heads, D.Nq), dtype=torch.float32, device=dev)
+        D.lse = lse.data_ptr() or None
+        if q.dtype == torch.bfloat16:
+            out32 = torch.empty(q.shape, dtype=torch.float32, device=dev)
+            D.out32 = out32.data_ptr() or None
+    ws = _seq_workspace(ctx, D, False)
+    check(load().cb_seq_attention_fwd(ctx.h, C.byref(D)))
+    if not need_grad:
+        return out
+    t = SeqTape()
+    t.q, t.k, t.v, t.out, t.lse, t.out32 = q, k, v, out, lse, out32
+    t.kw = dict(scale=scale, causal=causal, q_pos=q_pos, q_len=q_len, kv_len=kv_len, kv_mask=kv_mask, relpos=relpos, table=table)
+    return out, t
+
+
+def seq_attention_backward(ctx, tape, dout, dq=None, dk=None, dv=None, want_dtable=True):
+    """Gradients of seq_attention (cb_seq_attention_bwd) -> SeqGrads(dq, dk, dv, dtable). dq / dk / dv may be given as views to write into (slices
+    of a fused projection's gradient); dk and dv are summed over the query heads that share a key / value head, dtable [num_buckets, heads]
+    is float32. The call neither changes the tape nor adds to earlier results."""
+    q, k, v = tape.q, tape.k, tape.v
+    D = _seq_desc(ctx, q, k, v, **tape.kw)
+    _place(ctx, dout=dout, dq=dq, dk=dk, dv=dv)
+    g = SeqGrads()
+    g.dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq is None else dq
+    g.dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if dk is None else dk
+    g.dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dv is None else dv
+    D.out = _seq_tensor(tape.out, "out", tuple(q.shape), q.dtype)
+    D.dout = _seq_tensor(dout, "dout", tuple(q.shape), q.dtype)
+    D.dq = _seq_tensor(g.dq, "dq", tuple(q.shape), q.dtype)
+    D.dk = _seq_tensor(g.dk, "dk", tuple(k.shape), q.dtype)
+    D.dv = _seq_tensor(g.dv, "dv", tuple(v.shape), q.dtype)
+    D.lse = tape.lse.data_ptr() or None
+    D.out32 = (tape.out32.data_ptr() or None) if tape.out32 is not None else None
+    table = tape.kw["table"]
+    g.dtable = None
+    if table is not None and want_dtable:
+        g.dtable = torch.empty(table.shape, dtype=torch.float32, device=table.device)
+        D.dtable = g.dtable.data_ptr()
+    ws = _seq_workspace(ctx, D, True)
+    check(load().cb_seq_attention_bwd(ctx.h, C.byref(D)))
+    return g

@@ -51,6 +51,7 @@ typedef struct cb_vae_dec cb_vae_dec;
 typedef struct cb_clip cb_clip;
 typedef struct cb_frnet cb_frnet;
 typedef struct cb_trainer cb_trainer;
+typedef struct cb_relpos cb_relpos;
 
 const char* cb_last_error(void);
 /* ABI version of this header. It changes whenever a struct layout or the meaning of an argument changes: 100 = round 1 (float-only
@@ -177,6 +178,48 @@ typedef struct {
     int dtype;                                   /* cb_dtype of every tensor above (descriptor-level) */
 } cb_attention_desc;
 int cb_attention(cb_ctx* ctx, const cb_attention_desc* d);
+
+/* ---- sequence attention, residual RMS norm, products in 8-bit integers: the block of text towers other than CLIP's, and cross attention
+ * to padded prompts. Element types travel in the descriptors (cb_dtype), independent of the context's. None of these calls uses the
+ * context's step arena: outputs and workspaces are the caller's, so two captured graphs share memory only if the caller lets them.
+ * Lengths, positions and masks are DEVICE data; they are read by the kernels and held to their legal range there. */
+
+/* Relative position buckets of a learned bias (one table row per bucket, one column per head). Of `num_buckets` a two-sided
+ * (bidirectional) map uses one half for keys at or before the query and the other half for keys behind it; a one-sided map puts all keys
+ * behind the query into bucket 0. With nb buckets a side and E = nb / 2: distance n < E has a bucket of its own, n >= E has
+ * E + #{k in 1 .. nb-E-1 : n >= E (max_distance / E)^(k / (nb-E))}: the usual logarithm, with its borders in exact arithmetic.
+ * 2 <= num_buckets <= 256 (two-sided: a multiple of 4, else of 2), E < max_distance <= 1024. */
+int cb_relpos_create(cb_ctx* ctx, int num_buckets, int max_distance, int bidirectional, cb_relpos** out);
+int cb_relpos_destroy(cb_relpos* rp);                                /* the handle must outlive the graphs that captured calls with it */
+int cb_relpos_bucket(const cb_relpos* rp, int64_t relative, int* bucket);       /* relative = key position - query position; host only */
+
+typedef struct { void* p; int64_t row, head, batch; } cb_seq_tensor; /* [batch][token][head][d]; element strides, d contiguous */
+/* o_i = sum_j softmax_j(scale q_i.k_j + table[bucket(j - q_pos[b] - i)][h]) v_j over the keys visible to query i of sample b:
+ *   j < kv_len[b], kv_mask[b][j] != 0, causal: j <= q_pos[b] + i; i < q_len[b].
+ * Query rows without a visible key, and rows at or beyond q_len[b], give o = 0, lse = -inf and take part in no gradient; gradients of keys
+ * that are not visible are 0. What K, V hold in places hidden by kv_len or kv_mask, and Q, dout in rows beyond q_len, is never used (it may be
+ * NaN). A table entry of -inf hides its bucket. A one-token call over a cache: Nq = 1, q_pos[b] = kv_len[b] - 1.
+ * kv_heads divides heads; head h reads key / value head h / (heads / kv_heads). d % 8 == 0, d <= 160. Pointers 16-byte aligned, strides
+ * multiples of 16 bytes, row strides below 2^22 elements; out, dq, dk, dv must not overlap themselves. Inputs may have stride 0. */
+typedef struct {
+    int struct_size;                             /* = sizeof(cb_seq_attention_desc) */
+    int dtype;                                   /* cb_dtype of q, k, v, out, dout, dq, dk, dv */
+    int B, Nq, Nk, heads, kv_heads, d;
+    float scale; int causal;
+    cb_seq_tensor q, k, v, out;
+    const int32_t* q_pos; const int32_t* q_len; const int32_t* kv_len;       /* [B] each or NULL: 0, Nq, Nk */
+    const uint8_t* kv_mask; int64_t mask_stride;                             /* [B][Nk], stride of a sample, or NULL */
+    const cb_relpos* relpos; const float* table;                             /* [num_buckets][heads] float32; both or neither */
+    float* lse;                                  /* [B][heads][Nq] natural log; out of fwd (or NULL), into bwd */
+    float* out32;                                /* [B][Nq][heads][d] float32 or NULL: the unrounded output of a bf16 forward, kept for bwd, whose
+                                                    row sums dout.out (and with them dtable) then carry fp32 instead of bf16 rounding */
+    cb_seq_tensor dout, dq, dk, dv;              /* backward: gradients are written, not accumulated */
+    float* dtable;                               /* [num_buckets][heads] or NULL */
+    void* workspace; int64_t workspace_bytes;    /* 16-byte aligned, at least cb_seq_attention_workspace() */
+} cb_seq_attention_desc;
+int cb_seq_attention_workspace(cb_ctx* ctx, const cb_seq_attention_desc* d, int backward, int64_t* bytes);
+int cb_seq_attention_fwd(cb_ctx* ctx, const cb_seq_attention_desc* d);
+int cb_seq_attention_bwd(cb_ctx* ctx, const cb_seq_attention_desc* d);
 
 /* small ops of the step, exported for parity tests */
 int cb_timestep_embedding(cb_ctx* ctx, const int64_t* t, void* out, int B, int dim);                   /* util.py:151-171 */

@@ -1,0 +1,144 @@
+"""CPU tests of the sequence operators' host side: bucket borders in exact arithmetic, refusals through a dry context, descriptor layout."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def dry(built_lib):
+    from celebbasis_amd import lib
+    return lib, lib.Context(device=-1)
+
+
+def exact_bucket(rel, num_buckets, D, two):
+    """the definition, in whole numbers"""
+    nb = num_buckets // 2 if two else num_buckets
+    E, base = nb // 2, nb if two and rel > 0 else 0
+    n = abs(rel) if two else max(-rel, 0)
+    if n < E:
+        return base + n
+    m = nb - E
+    return base + E + sum(n ** m * E ** k >= E ** m * D ** k for k in range(1, m))
+
+
+@pytest.mark.parametrize("nb,D,two", [(32, 128, True), (32, 128, False), (64, 256, True), (16, 64, True), (16, 64, False), (4, 2, True), (2, 2, False),
+                                      (256, 1024, False), (8, 1024, True), (64, 33, False)])
+def test_relpos_buckets_are_exact(dry, nb, D, two):
+    lib, ctx = dry
+    rp = lib.RelPos(ctx, nb, D, two)
+    for rel in list(range(-min(D, 300) - 3, min(D, 300) + 4)) + [-D - 1, -D, D, D + 1, -10 ** 12, 10 ** 12]:
+        assert rp.bucket(rel) == exact_bucket(max(-D, min(D, rel)), nb, D, two), rel
+    # past the range everything shares the outermost bucket
+    assert rp.bucket(-D) == rp.bucket(-10 ** 9) and rp.bucket(D) == rp.bucket(10 ** 9)
+
+
+@pytest.mark.parametrize("nb,D,two", [(30, 128, True), (258, 128, False), (0, 128, True), (32, 8, True), (32, 1025, True), (3, 128, False)])
+def test_relpos_refusals(dry, nb, D, two):
+    lib, ctx = dry
+    with pytest.raises(lib.CBError) as e:
+        lib.RelPos(ctx, nb, D, two)
+    assert e.value.code == -1
+
+
+def test_sequence_descriptors_match_the_header(built_lib, tmp_path):
+    from celebbasis_amd import lib
+    if shutil.which("gcc") is None:
+        pytest.skip("no gcc")
+    pairs = [("cb_seq_tensor", lib.SeqTensor), ("cb_seq_attention_desc", lib.SeqAttentionDesc)]
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "celebbasis_hip.h"', "int main(void) {"]
+    for cname, cls in pairs:
+        lines.append(f'  printf("%zu\\n", sizeof({cname}));')
+        lines += [f'  printf("%zu\\n", offsetof({cname}, {f}));' for f, _ in cls._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    want = []
+    for _, cls in pairs:
+        want += [C.sizeof(cls)] + [getattr(cls, f).offset for f, _ in cls._fields_]
+    assert got == want
+
+
+def qkv(B=2, Nq=5, Nk=7, H=4, Hkv=2, d=16, dtype=torch.float32):
+    return torch.zeros(B, Nq, H, d, dtype=dtype), torch.zeros(B, Nk, Hkv, d, dtype=dtype), torch.zeros(B, Nk, Hkv, d, dtype=dtype)
+
+
+def test_seq_attention_accepts_what_it_documents(dry):
+    lib, ctx = dry
+    for dtype in (torch.float32, torch.bfloat16):
+        q, k, v = qkv(dtype=dtype)
+        rp = lib.RelPos(ctx)
+        out, tape = lib.seq_attention(ctx, q, k, v, relpos=rp, table=torch.zeros(32, 4), causal=True, kv_len=torch.zeros(2, dtype=torch.int32),
+                                      kv_mask=torch.ones(2, 7, dtype=torch.bool), need_grad=True)
+        g = lib.seq_attention_backward(ctx, tape, torch.zeros_like(out))
+        assert out.shape == q.shape and g.dk.shape == k.shape and g.dtable.shape == (32, 4)
+    for kw in (dict(B=0), dict(Nq=0), dict(Nk=0), dict(Nq=1, Nk=1, H=1, Hkv=1, d=8)):
+        q, k, v = qkv(**kw)
+        out, tape = lib.seq_attention(ctx, q, k, v, need_grad=True)
+        lib.seq_attention_backward(ctx, tape, torch.zeros_like(out))
+    x = torch.zeros(2, 5, 8, 16)                                     # slices of one fused projection, and a transposed cache
+    lib.seq_attention(ctx, x[:, :, :4], x[:, :, 4:6], x[:, :, 6:])
+    cache = torch.zeros(2, 2, 7, 16).transpose(1, 2)
+    lib.seq_attention(ctx, qkv()[0], cache, cache)
+    lib.seq_attention(ctx, qkv()[0], cache[:1].expand(2, -1, -1, -1), cache)
+
+
+@pytest.mark.parametrize("change,exc", [
+    (dict(d=12), "head dim"), (dict(d=168), "head dim"), (dict(H=3), "kv_heads"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(kv_len=torch.zeros(3, dtype=torch.int32)), "kv_len"),
+    (dict(kv_len=torch.zeros(2, dtype=torch.int64)), "kv_len"), (dict(kv_mask=torch.zeros(2, 6, dtype=torch.bool)), "kv_mask"),
+    (dict(kv_mask=torch.zeros(2, 7)), "kv_mask"), (dict(table=torch.zeros(32, 4)), "together"), (dict(dtype=torch.float16), "float"),
+    (dict(v_shape=(2, 6, 2, 16)), "v has shape"), (dict(v_dtype=torch.bfloat16), "v: expected dtype"), (dict(stride=True), "contiguous"),
+    (dict(odd=True), "16 bytes"), (dict(shift=True), "aligned"), (dict(overlap=True), "overlaps"),
+])
+def test_seq_attention_refusals(dry, change, exc):
+    lib, ctx = dry
+    q, k, v = qkv(**{x: y for x, y in change.items() if x in ("d", "H", "dtype")})
+    kw = {x: y for x, y in change.items() if x in ("scale", "kv_len", "kv_mask", "table")}
+    if "v_shape" in change:
+        v = torch.zeros(change["v_shape"])
+    if "v_dtype" in change:
+        v = v.to(change["v_dtype"])
+    if "stride" in change:
+        k = torch.zeros(2, 7, 16, 2).transpose(2, 3)
+    if "odd" in change:
+        k = torch.zeros(2, 7, 2, 18)[..., :16]
+    if "shift" in change:
+        k = torch.zeros(2 * 7 * 2 * 16 + 1)[1:].view(2, 7, 2, 16)
+    if "overlap" in change:
+        kw["out"] = torch.zeros(1, 5, 4, 16).expand(2, 5, 4, 16)
+    with pytest.raises((ValueError, TypeError, lib.CBError), match=exc):
+        lib.seq_attention(ctx, q, k, v, **kw)
+
+
+def test_seq_attention_descriptor_refusals(dry):
+    """what the Python wrapper cannot express: a foreign struct size, a short or misaligned workspace, gradients of a table that is not there"""
+    lib, ctx = dry
+    q, k, v = qkv()
+    out, tape = lib.seq_attention(ctx, q, k, v, need_grad=True)
+    D = lib._seq_desc(ctx, q, k, v, **tape.kw)
+    D.out = lib._seq_tensor(out, "out", tuple(q.shape), q.dtype)
+    so = lib.load()
+    D.struct_size -= 8
+    assert so.cb_seq_attention_fwd(ctx.h, C.byref(D)) == -1 and b"struct_size" in so.cb_last_error()
+    D.struct_size += 8
+    assert so.cb_seq_attention_fwd(ctx.h, None) == -1 and so.cb_seq_attention_fwd(None, C.byref(D)) == -1
+    for x, t in (("dout", out), ("dq", q), ("dk", k), ("dv", v)):
+        setattr(D, x, lib._seq_tensor(t, x, tuple(t.shape), t.dtype))
+    need = C.c_int64()
+    assert so.cb_seq_attention_workspace(ctx.h, C.byref(D), 1, C.byref(need)) == 0 and need.value > 0
+    D.workspace_bytes = need.value - 1
+    assert so.cb_seq_attention_bwd(ctx.h, C.byref(D)) == -1 and b"workspace" in so.cb_last_error()
+    D.workspace_bytes, D.workspace = need.value, 0x1008
+    assert so.cb_seq_attention_bwd(ctx.h, C.byref(D)) == -1 and b"aligned" in so.cb_last_error()
+    D.workspace, D.dtable = 0x1000, 0x1000
+    assert so.cb_seq_attention_bwd(ctx.h, C.byref(D)) == -1 and b"dtable" in so.cb_last_error()
+    D.dtable, D.dtype = None, 7
+    assert so.cb_seq_attention_bwd(ctx.h, C.byref(D)) == -1
