@@ -3,6 +3,7 @@
 #include "cb_models.h"
 #include "cb_gemm_tiles.h"
 #include "cb_seq.h"
+#include "cb_i8.h"
 #include <algorithm>
 #include <cmath>
 
@@ -1126,7 +1127,7 @@ static SeqArgs seq_args(const cb_ctx* ctx, const cb_seq_attention_desc* d, bool 
         CB_CHECK(!d->dtable || d->relpos, CB_ERR_ARG, "seq attention: dtable without a table");
         a.dtable = d->dtable;
     }
-    a.lse = d->lse; a.o32 = a.dt == DT_BF16 ? d->out32 : nullptr;
+    a.lse = d->lse; a.o32 = a.dt == DT_BF16 && d->table ? d->out32 : nullptr;
     if (!pointers) return a;
     a.q = seq_tensor(d->q, "q", a.dt, d->B, d->Nq, d->heads, d->d, false, c.dry);
     a.k = seq_tensor(d->k, "k", a.dt, d->B, d->Nk, d->kv_heads, d->d, false, c.dry);
@@ -1171,6 +1172,140 @@ int cb_seq_attention_bwd(cb_ctx* ctx, const cb_seq_attention_desc* d) {
     seq_ws_check(d, seq_ws(a, true), ctx->c.dry);
     OnDevice on(ctx->c);
     seq_backward(ctx->c.launch(), a, d->workspace);
+    CB_END
+}
+
+// ------------------------------------------------------------------ residual RMS norm, rows in 8 bits, 8-bit product
+static DType dtype_of(int dt, const char* what) {
+    CB_CHECK(dt == CB_DTYPE_F32 || dt == CB_DTYPE_BF16, CB_ERR_ARG, "%s: unknown dtype %d", what, dt);
+    return (DType)dt;
+}
+// a [rows][ld] operand: there, aligned to its elements, rows not shorter than C
+static void rows_check(const void* p, int64_t ld, int64_t rows, int C, size_t es, const char* what, bool dry) {
+    if (!dry && rows > 0) require(p, what);
+    CB_CHECK(reinterpret_cast<uintptr_t>(p) % es == 0, CB_ERR_ARG, "%s is not aligned to its elements", what);
+    CB_CHECK(ld >= C || (rows <= 1 && ld >= 0), CB_ERR_SHAPE, "%s: row stride %ld is shorter than a row of %d", what, (long)ld, C);
+}
+static void i8_rows_check(const void* p, int64_t ld, int64_t rows, int C, const char* what, bool dry) {
+    rows_check(p, ld, rows, C, 1, what, dry);
+    CB_CHECK((reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 16 == 0, CB_ERR_SHAPE, "%s: rows of 8-bit values are 16-byte aligned (row stride %ld)", what, (long)ld);
+}
+static RmsArgs rms_args(const cb_ctx* ctx, const cb_rmsnorm_desc* d) {
+    CB_CHECK(d->struct_size == (int)sizeof(cb_rmsnorm_desc), CB_ERR_ARG, "rmsnorm: desc.struct_size %d != %d — caller built against "
+             "another header (ABI %d)", d->struct_size, (int)sizeof(cb_rmsnorm_desc), CB_ABI_VERSION);
+    RmsArgs a;
+    a.dt = dtype_of(d->dtype, "rmsnorm");
+    CB_CHECK(d->rows >= 0 && d->rows < (1ll << 31) && d->C >= 1 && d->C <= RMS_MAX_C, CB_ERR_SHAPE, "rmsnorm: rows = %ld, C = %d (at most %d)", (long)d->rows, d->C, RMS_MAX_C);
+    CB_CHECK(d->eps >= 0.f && std::isfinite(d->eps), CB_ERR_ARG, "rmsnorm: eps = %g", (double)d->eps);
+    a.rows = d->rows; a.C = d->C; a.eps = d->eps;
+    rows_check(d->gamma, d->C, 1, d->C, 4, "rmsnorm: gamma", ctx->c.dry);
+    a.gamma = d->gamma;
+    return a;
+}
+int cb_rmsnorm_workspace(cb_ctx* ctx, int64_t rows, int C, int64_t* bytes) {
+    CB_TRY
+    require(ctx, "ctx"); require(bytes, "bytes");
+    CB_CHECK(rows >= 0 && rows < (1ll << 31) && C >= 1 && C <= RMS_MAX_C, CB_ERR_SHAPE, "rmsnorm: rows = %ld, C = %d (at most %d)", (long)rows, C, RMS_MAX_C);
+    *bytes = (int64_t)rmsnorm_bwd_ws_bytes(rows, C);
+    CB_END
+}
+int cb_rmsnorm_fwd(cb_ctx* ctx, const cb_rmsnorm_desc* d) {
+    CB_TRY
+    require(ctx, "ctx"); require(d, "desc");
+    RmsArgs a = rms_args(ctx, d);
+    const bool dry = ctx->c.dry;
+    const size_t es = dt_size(a.dt);
+    rows_check(d->x, d->ldx, a.rows, a.C, es, "rmsnorm: x", dry);
+    a.x = d->x; a.ldx = d->ldx;
+    if (d->residual) { rows_check(d->residual, d->ldres, a.rows, a.C, es, "rmsnorm: residual", dry); a.r = d->residual; a.ldr = d->ldres; }
+    if (d->h) { rows_check(d->h, d->ldh, a.rows, a.C, es, "rmsnorm: h", dry); a.h = d->h; a.ldh = d->ldh; }
+    CB_CHECK((d->y != nullptr) != (d->y_i8 != nullptr) || a.rows == 0, CB_ERR_ARG, "rmsnorm: exactly one of y and y_i8");
+    if (d->y) { rows_check(d->y, d->ldy, a.rows, a.C, es, "rmsnorm: y", dry); a.y = d->y; a.ldy = d->ldy; }
+    if (d->y_i8) {
+        i8_rows_check(d->y_i8, d->ldi8, a.rows, a.C, "rmsnorm: y_i8", dry);
+        if (!dry) require(d->scale, "scale");
+        a.q = d->y_i8; a.ldq = d->ldi8; a.scale = d->scale;
+    }
+    a.rstd = d->rstd;
+    if (a.rows == 0) return CB_STATUS_OK;
+    OnDevice on(ctx->c);
+    k_rmsnorm_fwd(ctx->c.launch(), a);
+    CB_END
+}
+int cb_rmsnorm_bwd(cb_ctx* ctx, const cb_rmsnorm_desc* d) {
+    CB_TRY
+    require(ctx, "ctx"); require(d, "desc");
+    RmsArgs a = rms_args(ctx, d);
+    const bool dry = ctx->c.dry;
+    const size_t es = dt_size(a.dt);
+    rows_check(d->h, d->ldh, a.rows, a.C, es, "rmsnorm: h", dry); a.h = d->h; a.ldh = d->ldh;
+    rows_check(d->dy, d->lddy, a.rows, a.C, es, "rmsnorm: dy", dry); a.dy = d->dy; a.lddy = d->lddy;
+    rows_check(d->dh, d->lddh, a.rows, a.C, es, "rmsnorm: dh", dry); a.dh = d->dh; a.lddh = d->lddh;
+    if (d->dres) { rows_check(d->dres, d->lddres, a.rows, a.C, es, "rmsnorm: dres", dry); a.dres = d->dres; a.lddres = d->lddres; }
+    if (!dry && a.rows > 0) require(d->rstd, "rstd");
+    a.rstd = d->rstd;
+    if (d->dgamma) {
+        const size_t need = rmsnorm_bwd_ws_bytes(a.rows, a.C);
+        CB_CHECK(d->workspace_bytes >= 0 && (size_t)d->workspace_bytes >= need && (reinterpret_cast<uintptr_t>(d->workspace) & 3) == 0, CB_ERR_ARG,
+                 "rmsnorm: workspace of %ld bytes, %zu needed", (long)d->workspace_bytes, need);
+        if (need && !dry) require(d->workspace, "workspace");
+        a.dgamma = d->dgamma; a.part = static_cast<float*>(d->workspace);
+    }
+    OnDevice on(ctx->c);
+    k_rmsnorm_bwd(ctx->c.launch(), a);
+    CB_END
+}
+int cb_quantize_rows(cb_ctx* ctx, int dtype, const void* x, int64_t ldx, int64_t rows, int C, int8_t* q, int64_t ldq, float* scale) {
+    CB_TRY
+    require(ctx, "ctx");
+    RmsArgs a;
+    a.dt = dtype_of(dtype, "quantize_rows");
+    CB_CHECK(rows >= 0 && rows < (1ll << 31) && C >= 1 && C <= I8_MAX_K, CB_ERR_SHAPE, "quantize_rows: rows = %ld, C = %d (at most %d)", (long)rows, C, I8_MAX_K);
+    rows_check(x, ldx, rows, C, dt_size(a.dt), "quantize_rows: x", ctx->c.dry);
+    i8_rows_check(q, ldq, rows, C, "quantize_rows: q", ctx->c.dry);
+    if (!ctx->c.dry && rows > 0) require(scale, "scale");
+    if (rows == 0) return CB_STATUS_OK;
+    a.rows = rows; a.C = C; a.x = x; a.ldx = ldx; a.q = q; a.ldq = ldq; a.scale = scale;
+    OnDevice on(ctx->c);
+    k_quantize_rows(ctx->c.launch(), a);
+    CB_END
+}
+static GemmI8Args gemm_i8_args(const cb_gemm_i8_desc* d) {
+    CB_CHECK(d->struct_size == (int)sizeof(cb_gemm_i8_desc), CB_ERR_ARG, "gemm_i8: desc.struct_size %d != %d — caller built against "
+             "another header (ABI %d)", d->struct_size, (int)sizeof(cb_gemm_i8_desc), CB_ABI_VERSION);
+    GemmI8Args a;
+    a.dt = dtype_of(d->dtype, "gemm_i8");
+    CB_CHECK(d->M >= 0 && d->N >= 0 && d->K >= 16 && d->K % 16 == 0 && d->K <= I8_MAX_K, CB_ERR_SHAPE, "gemm_i8: M = %d, N = %d, K = %d (a multiple of 16, at most %d)",
+             d->M, d->N, d->K, I8_MAX_K);
+    CB_CHECK((int64_t)cdiv(d->M, 64) * cdiv(d->N, 16) < (1ll << 31), CB_ERR_SHAPE, "gemm_i8: %d x %d outputs are too many for one call", d->M, d->N);
+    a.M = d->M; a.N = d->N; a.K = d->K; a.A = d->A; a.B = d->B; a.lda = d->lda; a.ldb = d->ldb; a.sa = d->a_scale; a.sb = d->b_scale;
+    a.bias = d->bias; a.R = d->R; a.ldr = d->ldr; a.C = d->C; a.ldc = d->ldc;
+    return a;
+}
+int cb_gemm_i8_workspace(cb_ctx* ctx, const cb_gemm_i8_desc* d, int64_t* bytes) {
+    CB_TRY
+    require(ctx, "ctx"); require(d, "desc"); require(bytes, "bytes");
+    *bytes = (int64_t)gemm_i8_ws_bytes(gemm_i8_args(d));
+    CB_END
+}
+int cb_gemm_i8(cb_ctx* ctx, const cb_gemm_i8_desc* d) {
+    CB_TRY
+    require(ctx, "ctx"); require(d, "desc");
+    const GemmI8Args a = gemm_i8_args(d);
+    const bool dry = ctx->c.dry;
+    i8_rows_check(d->A, d->lda, a.N ? a.M : 0, a.K, "gemm_i8: A", dry);
+    i8_rows_check(d->B, d->ldb, a.M ? a.N : 0, a.K, "gemm_i8: B", dry);
+    CB_CHECK(d->lda < (1 << 23) && d->ldb < (1 << 23), CB_ERR_SHAPE, "gemm_i8: row strides %ld, %ld (below 2^23)", (long)d->lda, (long)d->ldb);
+    if ((int64_t)a.M * a.N == 0) return CB_STATUS_OK;
+    const size_t es = dt_size(a.dt), need = gemm_i8_ws_bytes(a);
+    rows_check(d->C, d->ldc, a.M, a.N, es, "gemm_i8: C", dry);
+    if (d->R) rows_check(d->R, d->ldr, a.M, a.N, es, "gemm_i8: R", dry);
+    if (!dry) { require(d->a_scale, "a_scale"); require(d->b_scale, "b_scale"); }
+    CB_CHECK(d->workspace_bytes >= 0 && (size_t)d->workspace_bytes >= need && (reinterpret_cast<uintptr_t>(d->workspace) & 15) == 0, CB_ERR_ARG,
+             "gemm_i8: workspace of %ld bytes, %zu needed (16-byte aligned)", (long)d->workspace_bytes, need);
+    if (need && !dry) require(d->workspace, "workspace");
+    OnDevice on(ctx->c);
+    gemm_i8(ctx->c.launch(), a, d->workspace);
     CB_END
 }
 

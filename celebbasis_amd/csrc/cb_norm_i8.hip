@@ -1,0 +1,313 @@
+// cb_norm_i8.hip — root-mean-square norm with the residual's addition, in its element type or in 8 bits with a scale per row, its backward
+// pass, and plain rows brought to 8 bits.
+//
+//   h = round_T(x + r)          the residual stream as it is held; everything below is of the held value
+//   rstd = 1 / sqrt(mean(h^2) + eps);  y = h rstd g
+//   8 bits: scale = max|y| / 127, q = rint(y * (127 / max|y|))    (of the unrounded y)
+//   dh = rstd (dy g - h rstd^2 mean(dy g h)) + dres;  dg = sum over rows of dy h rstd
+// All of it is bound by memory: a row is read once and stays in registers (8 consecutive elements a thread and step) until it is written.
+#include "cb_device.h"
+#include "cb_i8.h"
+
+namespace cb {
+
+template <typename T> __device__ __forceinline__ void ld8v(const T* p, float (&v)[8]) {
+    const float4 a = ld4(p), b = ld4(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <> __device__ __forceinline__ void ld8v<bf16_t>(const bf16_t* p, float (&v)[8]) {
+    const bf16x8_t t = *reinterpret_cast<const bf16x8_t*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
+}
+template <typename T> __device__ __forceinline__ void st8v(T* p, const float (&v)[8]) {
+    st4(p, make_float4(v[0], v[1], v[2], v[3])); st4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
+}
+template <> __device__ __forceinline__ void st8v<bf16_t>(bf16_t* p, const float (&v)[8]) {
+    bf16x8_t o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (bf16_t)v[e];
+    *reinterpret_cast<bf16x8_t*>(p) = o;
+}
+// 8 elements of a row from column c on; VEC: rows of whole, aligned groups of 8. Elements at or beyond C are 0
+template <typename T, bool VEC> __device__ __forceinline__ void row_ld(const T* p, int c, int C, float (&v)[8]) {
+    if constexpr (VEC) {
+        if (c < C) { ld8v(p + c, v); return; }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < C ? ld1(p + c + e) : 0.f;
+    }
+}
+template <typename T, bool VEC> __device__ __forceinline__ void row_st(T* p, int c, int C, const float (&v)[8]) {
+    if constexpr (VEC) {
+        if (c < C) st8v(p + c, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) if (c + e < C) st1(p + c + e, v[e]);
+    }
+}
+// sums / maxima over the TPR threads of a row (64: a wave; 256: the block), the same value in all of them
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float* sh) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (TPR == 256) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = (sh[0] + sh[1]) + (sh[2] + sh[3]);
+    }
+    return v;
+}
+template <int TPR> __device__ __forceinline__ unsigned row_max(unsigned v, float* sh) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
+    if constexpr (TPR == 256) {
+        unsigned* s = reinterpret_cast<unsigned*>(sh);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = max(max(s[0], s[1]), max(s[2], s[3]));
+    }
+    return v;
+}
+// the factor 127 / amax of a row and the scale that it is held with. Magnitudes are compared as bit patterns, so that a NaN or an infinity is
+// the largest: such a row gets that as its scale and zeros as its values. A row below 2^-119 (127 / amax would overflow) is held as zeros.
+__device__ __forceinline__ float i8_factor(unsigned amax_bits, float* scale) {
+    const float amax = __uint_as_float(amax_bits);
+    if (amax_bits >= 0x7F800000u) { *scale = amax; return 0.f; }
+    if (amax < 1.5e-36f) { *scale = 0.f; return 0.f; }
+    *scale = amax / 127.f;
+    return 127.f / amax;
+}
+__device__ __forceinline__ unsigned mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+__device__ __forceinline__ int i8_of(float v, float f) { return f == 0.f ? 0 : (int)fminf(fmaxf(rintf(v * f), -127.f), 127.f); }
+// 8 values to q[c .. c+7] of a row of Cp = ceil16(C) places (the row is 16-byte aligned)
+__device__ __forceinline__ void i8_store(int8_t* q, int c, int Cp, const float (&v)[8], float f) {
+    if (c >= Cp) return;
+    int b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = i8_of(v[e], f) & 255;
+    *reinterpret_cast<uint2*>(q + c) = make_uint2((unsigned)(b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24)), (unsigned)(b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24)));
+}
+
+// NORM = false: rows to 8 bits as they are
+template <typename T, int TPR, int NV, bool VEC, bool NORM>
+__global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsArgs a) {
+    __shared__ float sh[4];
+    const long row = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    if (row >= a.rows) return;                       // TPR = 256: the whole block
+    const int t = threadIdx.x % TPR, C = a.C;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    float v[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) row_ld<T, VEC>(x, (j * TPR + t) * 8, C, v[j]);
+    if constexpr (NORM) {
+        if (a.r) {
+            const T* r = static_cast<const T*>(a.r) + row * a.ldr;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                float w[8];
+                row_ld<T, VEC>(r, (j * TPR + t) * 8, C, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = (float)(T)(v[j][e] + w[e]);
+            }
+        }
+        if (a.h) {
+            T* h = static_cast<T*>(a.h) + row * a.ldh;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) row_st<T, VEC>(h, (j * TPR + t) * 8, C, v[j]);
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = __builtin_fmaf(v[j][e], v[j][e], s);
+            ss += s;
+        }
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, sh) / (float)C + a.eps);
+        if (t == 0 && a.rstd) a.rstd[row] = rstd;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * TPR + t) * 8;
+            float g[8];
+            row_ld<float, VEC>(a.gamma, c, C, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = v[j][e] * rstd * g[e];
+        }
+        if (a.y) {
+            T* y = static_cast<T*>(a.y) + row * a.ldy;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) row_st<T, VEC>(y, (j * TPR + t) * 8, C, v[j]);
+            return;
+        }
+    }
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, mag(v[j][e]));
+    float s;
+    const float f = i8_factor(row_max<TPR>(m, sh), &s);
+    if (t == 0) a.scale[row] = s;
+    int8_t* q = a.q + row * a.ldq;
+    const int Cp = (C + 15) / 16 * 16;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) i8_store(q, (j * TPR + t) * 8, Cp, v[j], f);
+}
+// rows longer than the registers hold: read twice (the second time from the caches)
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_long_kernel(const RmsArgs a) {
+    __shared__ float sh[4];
+    const long row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const int C = a.C, Cp = (C + 15) / 16 * 16;
+    unsigned m = 0;
+    for (int c = threadIdx.x; c < C; c += 256) m = max(m, mag(ld1(x + c)));
+    float s;
+    const float f = i8_factor(row_max<256>(m, sh), &s);
+    if (threadIdx.x == 0) a.scale[row] = s;
+    int8_t* q = a.q + row * a.ldq;
+    for (int c = threadIdx.x; c < Cp; c += 256) q[c] = c < C ? (int8_t)i8_of(ld1(x + c), f) : (int8_t)0;
+}
+
+constexpr int RMS_PARTS = 512;                       // blocks of the backward pass, and rows of its partial sums of dgamma
+template <typename T, int TPR, int NV, bool VEC>
+__global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsArgs a, const int per) {
+    __shared__ float sh[4];
+    __shared__ float dgs[TPR == 64 ? NV * 64 * 8 : 8];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, C = a.C;
+    constexpr int RPB = 256 / TPR;
+    float g[NV][8], dg[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        row_ld<float, VEC>(a.gamma, (j * TPR + t) * 8, C, g[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dg[j][e] = 0.f;
+    }
+    const long r0 = (long)blockIdx.x * per, r1 = min(r0 + per, a.rows);
+    for (long row = r0 + sub; row < r1; row += RPB) {
+        const T* hp = static_cast<const T*>(a.h) + row * a.ldh;
+        const T* dp = static_cast<const T*>(a.dy) + row * a.lddy;
+        const float rstd = a.rstd[row];
+        float h[NV][8], w[NV][8], s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            row_ld<T, VEC>(hp, (j * TPR + t) * 8, C, h[j]);
+            row_ld<T, VEC>(dp, (j * TPR + t) * 8, C, w[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                h[j][e] *= rstd;                                   // normed value
+                dg[j][e] = __builtin_fmaf(w[j][e], h[j][e], dg[j][e]);
+                w[j][e] *= g[j][e];
+                s = __builtin_fmaf(w[j][e], h[j][e], s);
+            }
+        const float m = row_sum<TPR>(s, sh) / (float)C;
+        T* dh = static_cast<T*>(a.dh) + row * a.lddh;
+        const T* dr = a.dres ? static_cast<const T*>(a.dres) + row * a.lddres : nullptr;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float o[8];
+            if (dr) row_ld<T, VEC>(dr, (j * TPR + t) * 8, C, o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = rstd * (w[j][e] - h[j][e] * m);
+                o[e] = dr ? v + o[e] : v;
+            }
+            row_st<T, VEC>(dh, (j * TPR + t) * 8, C, o);
+        }
+    }
+    if (!a.part) return;
+    float* P = a.part + (long)blockIdx.x * C;
+    if constexpr (TPR == 256) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) row_st<float, false>(P, (j * TPR + t) * 8, C, dg[j]);
+    } else {
+        for (int k = 0; k < RPB; ++k) {                            // one wave after the other: a fixed order
+            if (sub == k) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int i = (j * 64 + t) * 8 + e;
+                        dgs[i] = k ? dgs[i] + dg[j][e] : dg[j][e];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < C; c += 256) P[c] = dgs[c];
+    }
+}
+// dgamma[c] = sum of the parts in order: 64 columns a block, 4 runs of parts
+__global__ __launch_bounds__(256) void rms_dgamma_kernel(const float* __restrict__ part, float* __restrict__ dgamma, int n, int C) {
+    __shared__ float sh[4][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+    float s = 0.f;
+    if (c < C) {
+        const int per = (n + 3) / 4, i1 = min(n, (w + 1) * per);
+        for (int i = w * per; i < i1; ++i) s += part[(long)i * C + c];
+    }
+    sh[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w == 0 && c < C) dgamma[c] = (sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]);
+}
+
+// ---------------------------------------------------------------- host side
+static bool al16(const void* p, long ld, size_t es) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * (long)es % 16 == 0; }
+#define RMS_GO(kernel, grid, ...)                                                        \
+    do {                                                                                 \
+        L.count();                                                                       \
+        if (!L.dry) {                                                                    \
+            hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, L.stream, __VA_ARGS__); \
+            CB_HIP(hipGetLastError());                                                   \
+        }                                                                                \
+    } while (0)
+// threads a row and groups of 8 a thread: a wave up to 2048 columns, else a block
+#define RMS_SHAPE(C, TPR, NV, ...)                                                            \
+    do {                                                                                      \
+        if ((C) <= 512) { constexpr int TPR = 64, NV = 1; __VA_ARGS__; }                      \
+        else if ((C) <= 1024) { constexpr int TPR = 64, NV = 2; __VA_ARGS__; }                \
+        else if ((C) <= 2048) { constexpr int TPR = 64, NV = 4; __VA_ARGS__; }                \
+        else if ((C) <= 4096) { constexpr int TPR = 256, NV = 2; __VA_ARGS__; }               \
+        else if ((C) <= 8192) { constexpr int TPR = 256, NV = 4; __VA_ARGS__; }               \
+        else { constexpr int TPR = 256, NV = 8; __VA_ARGS__; }                                \
+    } while (0)
+
+template <bool NORM> static void fwd_any(const Launch& L, const RmsArgs& a) {
+    const size_t es = dt_size(a.dt);
+    const bool vec = a.C % 8 == 0 && al16(a.x, a.ldx, es) && (!a.r || al16(a.r, a.ldr, es)) && (!a.h || al16(a.h, a.ldh, es)) &&
+                     (!a.y || al16(a.y, a.ldy, es)) && (!NORM || al16(a.gamma, 0, 4));
+    CB_DT_SWITCH(a.dt, T, RMS_SHAPE(a.C, TPR, NV, {
+        const unsigned grid = cdiv(a.rows, 256 / TPR);
+        if (vec) RMS_GO((rms_fwd_kernel<T, TPR, NV, true, NORM>), grid, a);
+        else RMS_GO((rms_fwd_kernel<T, TPR, NV, false, NORM>), grid, a);
+    }));
+}
+void k_rmsnorm_fwd(const Launch& L, const RmsArgs& a) { fwd_any<true>(L, a); }
+void k_quantize_rows(const Launch& L, const RmsArgs& a) {
+    if (a.C <= RMS_MAX_C) { fwd_any<false>(L, a); return; }
+    CB_DT_SWITCH(a.dt, T, RMS_GO((quantize_long_kernel<T>), (unsigned)a.rows, a));
+}
+static int bwd_per(long rows, int C) {                // rows a block: a whole number of passes of its waves
+    const int rpb = C <= 2048 ? 4 : 1;
+    return (int)rup((long)cdiv(rows, RMS_PARTS), rpb);
+}
+size_t rmsnorm_bwd_ws_bytes(long rows, int C) { return rows ? (size_t)cdiv(rows, bwd_per(rows, C)) * C * 4 : 0; }
+void k_rmsnorm_bwd(const Launch& L, const RmsArgs& a) {
+    const size_t es = dt_size(a.dt);
+    const bool vec = a.C % 8 == 0 && al16(a.h, a.ldh, es) && al16(a.dy, a.lddy, es) && al16(a.dh, a.lddh, es) && al16(a.gamma, 0, 4) &&
+                     (!a.dres || al16(a.dres, a.lddres, es));
+    const int per = bwd_per(a.rows, a.C), n = a.rows ? (int)cdiv(a.rows, per) : 0;
+    if (n) CB_DT_SWITCH(a.dt, T, RMS_SHAPE(a.C, TPR, NV, {
+        if (vec) RMS_GO((rms_bwd_kernel<T, TPR, NV, true>), (unsigned)n, a, per);
+        else RMS_GO((rms_bwd_kernel<T, TPR, NV, false>), (unsigned)n, a, per);
+    }));
+    if (a.dgamma) RMS_GO(rms_dgamma_kernel, cdiv(a.C, 64), a.part, a.dgamma, n, a.C);
+}
+
+}  // namespace cb

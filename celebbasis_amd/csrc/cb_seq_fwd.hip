@@ -7,7 +7,10 @@
 
 namespace cb {
 
-template <typename T, int DT, int QB, bool BIAS>
+// PREC (bf16 with out32): the probabilities enter P.V as the sum of two bf16 numbers, so that the unrounded output, and with it the row sums
+// dO.O of the backward pass, carry 2^-18 instead of 2^-9 of rounding: dtable adds dS over whole diagonals, where the error of a row sum does
+// not cancel (measured without it: dtable 2e-3 off).
+template <typename T, int DT, int QB, bool BIAS, bool PREC>
 __global__ __launch_bounds__(256) void seq_fwd_kernel(const SeqArgs a, const int nqb) {
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
@@ -151,6 +154,15 @@ __global__ __launch_bounds__(256) void seq_fwd_kernel(const SeqArgs a, const int
             l[qb] += seq_group_sum(ps);
         }
         seq_tmul<T, DT, QB>(o, Vs, s, l15, g);
+        if constexpr (PREC) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[qb][kt][r] -= (float)(bf16_t)s[qb][kt][r];
+            seq_tmul<T, DT, QB>(o, Vs, s, l15, g);
+        }
     }
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -219,21 +231,24 @@ SeqPlan seq_fwd_plan(const SeqArgs& a) {
     p.total = p.part + p.ml;
     return p;
 }
-template <typename T, int DT, int QB, bool BIAS>
+template <typename T, int DT, int QB, bool BIAS, bool PREC>
 static void fwd_go(const Launch& L, const SeqArgs& a) {
     using G = SeqGeo<T, DT>;
     const int nqb = (int)cdiv(a.Nq, 64 * QB);
     const int lds = 4 * G::TILE + (BIAS ? (int)rup((2 * (a.D + G::TK + 16 * QB) + 1) * 4, 16) : 0);
     L.count();
     if (L.dry) return;
-    set_dyn_lds(reinterpret_cast<const void*>(&seq_fwd_kernel<T, DT, QB, BIAS>), 160 * 1024);
-    hipLaunchKernelGGL((seq_fwd_kernel<T, DT, QB, BIAS>), dim3((unsigned)nqb * a.B * a.H, a.nsplit), dim3(256), lds, L.stream, a, nqb);
+    set_dyn_lds(reinterpret_cast<const void*>(&seq_fwd_kernel<T, DT, QB, BIAS, PREC>), 160 * 1024);
+    hipLaunchKernelGGL((seq_fwd_kernel<T, DT, QB, BIAS, PREC>), dim3((unsigned)nqb * a.B * a.H, a.nsplit), dim3(256), lds, L.stream, a, nqb);
     CB_HIP(hipGetLastError());
 }
 template <typename T, int DT>
 static void fwd_pick(const Launch& L, const SeqArgs& a, int qb) {
-    if (a.table) fwd_go<T, DT, 1, true>(L, a);
-    else fwd_go<T, DT, 1, false>(L, a);
+    if constexpr (sizeof(T) == 2) {
+        if (a.o32) { fwd_go<T, DT, 1, true, true>(L, a); return; }
+    }
+    if (a.table) fwd_go<T, DT, 1, true, false>(L, a);
+    else fwd_go<T, DT, 1, false, false>(L, a);
 }
 void seq_forward(const Launch& L, SeqArgs a, void* ws) {
     const SeqPlan p = seq_fwd_plan(a);

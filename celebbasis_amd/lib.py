@@ -87,6 +87,22 @@ class SeqAttentionDesc(_Sized):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
+class RmsNormDesc(_Sized):
+    _fields_ = [("struct_size", C.c_int), ("dtype", C.c_int), ("rows", C.c_int64), ("C", C.c_int), ("eps", C.c_float),
+                ("x", C.c_void_p), ("ldx", C.c_int64), ("residual", C.c_void_p), ("ldres", C.c_int64), ("gamma", C.c_void_p),
+                ("h", C.c_void_p), ("ldh", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64),
+                ("y_i8", C.c_void_p), ("ldi8", C.c_int64), ("scale", C.c_void_p), ("rstd", C.c_void_p),
+                ("dy", C.c_void_p), ("lddy", C.c_int64), ("dres", C.c_void_p), ("lddres", C.c_int64), ("dh", C.c_void_p), ("lddh", C.c_int64),
+                ("dgamma", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class GemmI8Desc(_Sized):
+    _fields_ = [("struct_size", C.c_int), ("dtype", C.c_int), ("M", C.c_int), ("N", C.c_int), ("K", C.c_int),
+                ("A", C.c_void_p), ("lda", C.c_int64), ("B", C.c_void_p), ("ldb", C.c_int64),
+                ("a_scale", C.c_void_p), ("b_scale", C.c_void_p), ("bias", C.c_void_p), ("R", C.c_void_p), ("ldr", C.c_int64),
+                ("C", C.c_void_p), ("ldc", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 class UNetCfg(C.Structure):
     _fields_ = [("in_channels", C.c_int), ("out_channels", C.c_int), ("model_channels", C.c_int), ("num_res_blocks", C.c_int),
                 ("channel_mult", C.c_int * 8), ("n_mult", C.c_int),
@@ -132,6 +148,7 @@ ABI_SYMBOLS = [
     "cb_trainer_create", "cb_trainer_destroy", "cb_trainer_step", "cb_trainer_get_state", "cb_trainer_set_state",
     "cb_debug_force_plan", "cb_trainer_prefetch", "cb_trainer_set_graph_replay", "cb_trainer_graph_stats", "cb_trainer_prefetch_stream", "cb_trainer_set_prefetch_stream", "cb_trainer_loss_to", "cb_celeb_head_forward", "cb_face_augment", "cb_paste_on_canvas", "cb_row_surgery_multi", "cb_trainer_share_unet", "cb_trainer_share_clip", "cb_unet_ddim_sample", "cb_ddim_update", "cb_vae_decoder_create", "cb_vae_decoder_destroy", "cb_vae_decode",
     "cb_relpos_create", "cb_relpos_destroy", "cb_relpos_bucket", "cb_seq_attention_workspace", "cb_seq_attention_fwd", "cb_seq_attention_bwd",
+    "cb_rmsnorm_workspace", "cb_rmsnorm_fwd", "cb_rmsnorm_bwd", "cb_quantize_rows", "cb_gemm_i8_workspace", "cb_gemm_i8",
 ]
 
 
@@ -179,6 +196,8 @@ _ARGTYPES = {
     "cb_vae_decode": [_P, _P, _I, _I, _I, _F, _I, _P],
     "cb_relpos_create": [_P, _I, _I, _I, _P], "cb_relpos_destroy": [_P], "cb_relpos_bucket": [_P, _L, _P],
     "cb_seq_attention_workspace": [_P, _P, _I, _P], "cb_seq_attention_fwd": [_P, _P], "cb_seq_attention_bwd": [_P, _P],
+    "cb_rmsnorm_workspace": [_P, _L, _I, _P], "cb_rmsnorm_fwd": [_P, _P], "cb_rmsnorm_bwd": [_P, _P],
+    "cb_quantize_rows": [_P, _I, _P, _L, _L, _I, _P, _L, _P], "cb_gemm_i8_workspace": [_P, _P, _P], "cb_gemm_i8": [_P, _P],
 }
 
 
@@ -798,7 +817,7 @@ def seq_attention(ctx, q, k, v, scale=None, causal=False, q_pos=None, q_len=None
     if need_grad:
         lse = torch.empty((D.B, D.heads, D.Nq), dtype=torch.float32, device=dev)
         D.lse = lse.data_ptr() or None
-        if q.dtype == torch.bfloat16:
+        if q.dtype == torch.bfloat16 and table is not None:
             out32 = torch.empty(q.shape, dtype=torch.float32, device=dev)
             D.out32 = out32.data_ptr() or None
     ws = _seq_workspace(ctx, D, False)
@@ -837,3 +856,139 @@ def seq_attention_backward(ctx, tape, dout, dq=None, dk=None, dv=None, want_dtab
     ws = _seq_workspace(ctx, D, True)
     check(load().cb_seq_attention_bwd(ctx.h, C.byref(D)))
     return g
+
+
+def _rows(t, name, C=None, dtype=None):
+    """(pointer, row stride, rows, columns) of [..., C]: two dimensions with any row stride, or a contiguous tensor of any"""
+    if t.dim() < 1 or (C is not None and t.shape[-1] != C):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected [..., {C}]")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name}: expected dtype {dtype}, got {t.dtype}")
+    n = t.shape[-1]
+    if t.dim() == 2:
+        if n > 1 and t.stride(1) != 1:
+            raise ValueError(f"{name}: rows must be contiguous")
+        return t.data_ptr() or None, t.stride(0) if t.shape[0] > 1 else n, t.shape[0], n
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: tensor must be contiguous (or two-dimensional with contiguous rows)")
+    return t.data_ptr() or None, n, t.numel() // n if n else 0, n
+
+
+def _vector(t, name, n):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous float32 values, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr() or None
+
+
+def _float_code(t, name):
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
+    return DTYPE_BF16 if t.dtype == torch.bfloat16 else DTYPE_F32
+
+
+def padded_i8(n):
+    """row length of 8-bit rows of n values: whole pieces of 16, zeros behind n"""
+    return (n + 15) // 16 * 16
+
+
+class RmsOut:
+    """y (normed, or 8-bit [..., padded_i8(C)] with `scale` [...]), h = the held residual stream (x itself without a residual), rstd [...]"""
+    __slots__ = ("y", "h", "rstd", "scale")
+
+
+def rms_norm(ctx, x, weight, residual=None, eps=1e-6, out=None, need_grad=False):
+    """Root-mean-square norm over the last dim with the residual's addition (cb_rmsnorm_fwd): h = x + residual, y = h / rms(h) * weight.
+    out="i8": y in 8 bits with a scale per row, ready for linear_i8. need_grad keeps rstd. x [..., C] fp32 or bf16, weight float32 [C] -> RmsOut."""
+    if out not in (None, "i8"):
+        raise ValueError(f"out = {out!r}: None or 'i8'")
+    _place(ctx, x=x, weight=weight, residual=residual)
+    d = RmsNormDesc()
+    d.dtype = _float_code(x, "x")
+    d.x, d.ldx, d.rows, d.C = _rows(x, "x")
+    d.eps, d.gamma = float(eps), _vector(weight, "weight", d.C)
+    lead = tuple(x.shape[:-1])
+    r = RmsOut()
+    r.h, r.scale, r.rstd = x, None, None
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
+        d.residual, d.ldres = _rows(residual, "residual", d.C, x.dtype)[:2]
+        r.h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d.h, d.ldh = r.h.data_ptr() or None, d.C
+    if out == "i8":
+        r.y = torch.empty(lead + (padded_i8(d.C),), dtype=torch.int8, device=x.device)
+        r.scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+        d.y_i8, d.ldi8, d.scale = r.y.data_ptr() or None, r.y.shape[-1], r.scale.data_ptr() or None
+    else:
+        r.y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d.y, d.ldy = r.y.data_ptr() or None, d.C
+    if need_grad:
+        r.rstd = torch.empty(lead, dtype=torch.float32, device=x.device)
+        d.rstd = r.rstd.data_ptr() or None
+    check(load().cb_rmsnorm_fwd(ctx.h, C.byref(d)))
+    return r
+
+
+def rms_norm_backward(ctx, dy, h, weight, rstd, dres=None, want_dweight=True):
+    """(dh, dweight) of rms_norm: dh is the gradient of x and of the residual alike; dres: what flows into h from elsewhere"""
+    _place(ctx, dy=dy, h=h, weight=weight, rstd=rstd, dres=dres)
+    d = RmsNormDesc()
+    d.dtype = _float_code(h, "h")
+    d.h, d.ldh, d.rows, d.C = _rows(h, "h")
+    d.gamma, d.rstd = _vector(weight, "weight", d.C), _vector(rstd, "rstd", d.rows)
+    if dy.shape != h.shape or (dres is not None and dres.shape != h.shape):
+        raise ValueError(f"dy {tuple(dy.shape)} and dres must have h's shape {tuple(h.shape)}")
+    d.dy, d.lddy = _rows(dy, "dy", d.C, h.dtype)[:2]
+    if dres is not None:
+        d.dres, d.lddres = _rows(dres, "dres", d.C, h.dtype)[:2]
+    dh = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    d.dh, d.lddh = dh.data_ptr() or None, d.C
+    dw = ws = None
+    if want_dweight:
+        dw = torch.empty(d.C, dtype=torch.float32, device=h.device)
+        n = C.c_int64()
+        check(load().cb_rmsnorm_workspace(ctx.h, d.rows, d.C, C.byref(n)))
+        ws = _workspace(ctx, n.value)
+        d.dgamma, d.workspace, d.workspace_bytes = dw.data_ptr(), None if ws is None else ws.data_ptr(), n.value
+    check(load().cb_rmsnorm_bwd(ctx.h, C.byref(d)))
+    return dh, dw
+
+
+def quantize_rows(ctx, x):
+    """rows of x [..., C] to 8 bits (cb_quantize_rows) -> (int8 [..., padded_i8(C)], scale [...]): activations by token, weights [N, K] by
+    output channel"""
+    _place(ctx, x=x)
+    code = _float_code(x, "x")
+    p, ld, rows, n = _rows(x, "x")
+    lead = tuple(x.shape[:-1])
+    q = torch.empty(lead + (padded_i8(n),), dtype=torch.int8, device=x.device)
+    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+    check(load().cb_quantize_rows(ctx.h, code, p, ld, rows, n, q.data_ptr() or None, q.shape[-1], scale.data_ptr() or None))
+    return q, scale
+
+
+def linear_i8(ctx, a, a_scale, w, w_scale, bias=None, residual=None, dtype="bf16"):
+    """a_scale * w_scale * (a . w^T) + bias + residual (cb_gemm_i8): a int8 [..., K], w int8 [N, K] (K padded by quantize_rows / rms_norm),
+    a_scale [...], w_scale [N], bias float32 [N], residual [..., N] of the output's dtype -> [..., N]"""
+    _place(ctx, a=a, a_scale=a_scale, w=w, w_scale=w_scale, bias=bias, residual=residual)
+    d = GemmI8Desc()
+    d.dtype = dtype_code(dtype)
+    if w.dim() != 2:
+        raise ValueError(f"w has shape {tuple(w.shape)}, expected [N, K]")
+    d.A, d.lda, d.M, d.K = _rows(a, "a", None, torch.int8)
+    d.B, d.ldb, d.N, _ = _rows(w, "w", d.K, torch.int8)
+    d.a_scale, d.b_scale, d.bias = _vector(a_scale, "a_scale", d.M), _vector(w_scale, "w_scale", d.N), _vector(bias, "bias", d.N)
+    out = torch.empty(tuple(a.shape[:-1]) + (d.N,), dtype=torch_dtype(d.dtype), device=a.device)
+    d.C, d.ldc = out.data_ptr() or None, d.N
+    if residual is not None:
+        if residual.shape != out.shape:
+            raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {tuple(out.shape)}")
+        d.R, d.ldr = _rows(residual, "residual", d.N, out.dtype)[:2]
+    n = C.c_int64()
+    check(load().cb_gemm_i8_workspace(ctx.h, C.byref(d), C.byref(n)))
+    ws = _workspace(ctx, n.value)
+    d.workspace, d.workspace_bytes = None if ws is None else ws.data_ptr(), n.value
+    check(load().cb_gemm_i8(ctx.h, C.byref(d)))
+    return out

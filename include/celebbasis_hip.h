@@ -211,8 +211,9 @@ typedef struct {
     const uint8_t* kv_mask; int64_t mask_stride;                             /* [B][Nk], stride of a sample, or NULL */
     const cb_relpos* relpos; const float* table;                             /* [num_buckets][heads] float32; both or neither */
     float* lse;                                  /* [B][heads][Nq] natural log; out of fwd (or NULL), into bwd */
-    float* out32;                                /* [B][Nq][heads][d] float32 or NULL: the unrounded output of a bf16 forward, kept for bwd, whose
-                                                    row sums dout.out (and with them dtable) then carry fp32 instead of bf16 rounding */
+    float* out32;                                /* [B][Nq][heads][d] float32 or NULL; bf16 with a table only (ignored otherwise): the output before its
+                                                    rounding, out of fwd into bwd. dtable needs its precision: without it the row sums dout.out,
+                                                    and dtable with them, carry bf16's rounding of `out` */
     cb_seq_tensor dout, dq, dk, dv;              /* backward: gradients are written, not accumulated */
     float* dtable;                               /* [num_buckets][heads] or NULL */
     void* workspace; int64_t workspace_bytes;    /* 16-byte aligned, at least cb_seq_attention_workspace() */
@@ -220,6 +221,50 @@ typedef struct {
 int cb_seq_attention_workspace(cb_ctx* ctx, const cb_seq_attention_desc* d, int backward, int64_t* bytes);
 int cb_seq_attention_fwd(cb_ctx* ctx, const cb_seq_attention_desc* d);
 int cb_seq_attention_bwd(cb_ctx* ctx, const cb_seq_attention_desc* d);
+
+/* Root-mean-square norm with the residual's addition (beside cb_layernorm_*): h = round_dtype(x + residual) is the residual stream as it is
+ * held; rstd = 1 / sqrt(mean(h^2) + eps); y = h rstd gamma, in dtype or in 8 bits: scale = max|y| / 127, y_i8 = rint(y 127 / max|y|) of the
+ * unrounded y, columns C .. ceil16(C) zeroed (what cb_gemm_i8 reads). A row that holds a NaN or an infinity gets it as its scale and zeros
+ * as its values; a row whose largest magnitude is below 2^-119 gets scale 0.
+ * Backward: dh = rstd (dy gamma - h rstd^2 mean(dy gamma h)) + dres, the gradient of x and of the residual alike;
+ * dgamma = sum over rows of dy h rstd, written, in a fixed order. x, h, residual may be one buffer, and dh may be dy or dres.
+ * 1 <= C <= 16384, any row strides >= C; rows of whole aligned 16-byte pieces (C % 8 == 0) take the fast path. */
+typedef struct {
+    int struct_size;                             /* = sizeof(cb_rmsnorm_desc) */
+    int dtype;                                   /* cb_dtype of x, residual, h, y, dy, dres, dh */
+    int64_t rows; int C; float eps;
+    const void* x; int64_t ldx; const void* residual; int64_t ldres;         /* residual may be NULL */
+    const float* gamma;                                                      /* [C] */
+    void* h; int64_t ldh;                        /* forward: NULL = not kept; backward: input */
+    void* y; int64_t ldy;                        /* exactly one of y and y_i8 */
+    int8_t* y_i8; int64_t ldi8; float* scale;    /* 16-byte aligned, ldi8 % 16 == 0, ldi8 >= C; scale [rows] */
+    float* rstd;                                 /* [rows]: out of fwd (or NULL), into bwd */
+    const void* dy; int64_t lddy; const void* dres; int64_t lddres; void* dh; int64_t lddh;    /* backward; dres may be NULL */
+    float* dgamma;                               /* [C] or NULL */
+    void* workspace; int64_t workspace_bytes;    /* backward: cb_rmsnorm_workspace() bytes */
+} cb_rmsnorm_desc;
+int cb_rmsnorm_workspace(cb_ctx* ctx, int64_t rows, int C, int64_t* bytes);
+int cb_rmsnorm_fwd(cb_ctx* ctx, const cb_rmsnorm_desc* d);
+int cb_rmsnorm_bwd(cb_ctx* ctx, const cb_rmsnorm_desc* d);
+/* rows of x (cb_dtype `dtype`) to 8 bits with a scale per row, as cb_rmsnorm_fwd's 8-bit output: activations by token, weights [N][K] by
+ * output channel. 1 <= C <= 131056 */
+int cb_quantize_rows(cb_ctx* ctx, int dtype, const void* x, int64_t ldx, int64_t rows, int C, int8_t* q, int64_t ldq, float* scale);
+/* C[m][n] = a_scale[m] b_scale[n] sum_k A[m][k] B[n][k] + bias[n] + R[m][n] (beside cb_gemm): 8-bit integers with a scale per token and per
+ * output channel, summed exactly in 32 bits. K % 16 == 0 (pad rows with zeros: cb_quantize_rows does), K <= 131056; A and B 16-byte aligned,
+ * lda % 16 == 0, ldb % 16 == 0, both below 2^23; any N, ldc, ldr. A scale of NaN or infinity makes its row or column NaN. C may be R. */
+typedef struct {
+    int struct_size;                             /* = sizeof(cb_gemm_i8_desc) */
+    int dtype;                                   /* cb_dtype of C and R */
+    int M, N, K;
+    const int8_t* A; int64_t lda; const int8_t* B; int64_t ldb;
+    const float* a_scale; const float* b_scale;  /* [M], [N] */
+    const float* bias;                           /* [N] or NULL */
+    const void* R; int64_t ldr;                  /* or NULL */
+    void* C; int64_t ldc;
+    void* workspace; int64_t workspace_bytes;    /* cb_gemm_i8_workspace() bytes, 16-byte aligned */
+} cb_gemm_i8_desc;
+int cb_gemm_i8_workspace(cb_ctx* ctx, const cb_gemm_i8_desc* d, int64_t* bytes);
+int cb_gemm_i8(cb_ctx* ctx, const cb_gemm_i8_desc* d);
 
 /* small ops of the step, exported for parity tests */
 int cb_timestep_embedding(cb_ctx* ctx, const int64_t* t, void* out, int B, int dim);                   /* util.py:151-171 */

@@ -110,7 +110,9 @@ class Ref:
         Dr = (do * o).sum(-1, keepdim=True)
         ds = p * (dp - Dr)
         e_dp = (d + 2) * U * torch.matmul(do.abs(), T(v64.abs()))
-        e_D = (do.abs() * ((d + 2) * U * o.abs() + o32_bound)).sum(-1, keepdim=True)
+        # the row sums dO.O: from the output as stored, or (bf16 with a table) from out32, whose probabilities carry r^2
+        o_used = (eP + (Nk + 4) * U + R * R) * pv + F * torch.matmul(vis64, v64.abs() + 1) if rel is not None and r else o32_bound + rT * (o.abs() + o32_bound)
+        e_D = (do.abs() * ((d + 2) * U * o.abs() + o_used)).sum(-1, keepdim=True)
         bs = p * (eP * (dp.abs() + Dr.abs()) + e_dp + e_D) + 4 * U * ds.abs() + F * vis64 * (dp.abs() + Dr.abs() + 1)
         a = ds.abs()
         fold = lambda x: x.view(B, Hkv, G, *x.shape[2:]).sum(2)

@@ -142,3 +142,92 @@ def test_seq_attention_descriptor_refusals(dry):
     assert so.cb_seq_attention_bwd(ctx.h, C.byref(D)) == -1 and b"dtable" in so.cb_last_error()
     D.dtable, D.dtype = None, 7
     assert so.cb_seq_attention_bwd(ctx.h, C.byref(D)) == -1
+
+
+def test_norm_and_product_descriptors_match_the_header(built_lib, tmp_path):
+    from celebbasis_amd import lib
+    if shutil.which("gcc") is None:
+        pytest.skip("no gcc")
+    pairs = [("cb_rmsnorm_desc", lib.RmsNormDesc), ("cb_gemm_i8_desc", lib.GemmI8Desc)]
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "celebbasis_hip.h"', "int main(void) {"]
+    for cname, cls in pairs:
+        lines.append(f'  printf("%zu\\n", sizeof({cname}));')
+        lines += [f'  printf("%zu\\n", offsetof({cname}, {f}));' for f, _ in cls._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    want = []
+    for _, cls in pairs:
+        want += [C.sizeof(cls)] + [getattr(cls, f).offset for f, _ in cls._fields_]
+    assert got == want
+
+
+def test_norm_accepts_and_refuses(dry):
+    lib, ctx = dry
+    x, g = torch.zeros(3, 4, 40), torch.ones(40)
+    n = lib.rms_norm(ctx, x, g, residual=x, need_grad=True)
+    assert n.y.shape == x.shape and n.rstd.shape == (3, 4)
+    dh, dg = lib.rms_norm_backward(ctx, x, n.h, g, n.rstd, dres=x)
+    assert dh.shape == x.shape and dg.shape == (40,)
+    assert lib.rms_norm(ctx, x.to(torch.bfloat16), g, out="i8").y.shape == (3, 4, 48)
+    lib.rms_norm(ctx, torch.zeros(5, 50)[:, :40], g)
+    for bad, kw, what in ((x.half(), {}, "float"), (x, dict(residual=x[:2]), "residual has shape"), (x, dict(residual=x.to(torch.bfloat16)), "residual"),
+                          (x, dict(eps=-1.0), "eps"), (x, dict(eps=float("nan")), "eps"), (x, dict(out="i4"), "i8"), (x.transpose(0, 1), {}, "contiguous"),
+                          (torch.zeros(5, 80)[:, ::2], {}, "contiguous"), (torch.zeros(2, 16385), {}, "shape|C ="), (torch.zeros(2, 39), {}, "weight")):
+        w = torch.ones(16385) if bad.shape[-1] == 16385 else g
+        with pytest.raises((ValueError, TypeError, lib.CBError), match=what):
+            lib.rms_norm(ctx, bad, w, **kw)
+    with pytest.raises(ValueError, match="shape"):
+        lib.rms_norm_backward(ctx, x[:, :3], n.h, g, n.rstd)
+    with pytest.raises(ValueError, match="rstd"):
+        lib.rms_norm_backward(ctx, x, n.h, g, n.rstd[:1])
+    so = lib.load()
+    d = lib.RmsNormDesc()
+    d.rows, d.C, d.ldx, d.ldy, d.ldi8 = 4, 40, 40, 40, 40
+    y = torch.zeros(4, 48)
+    p = lambda t: t.data_ptr()
+    d.x, d.gamma, d.y, d.y_i8 = p(y), p(g), p(y), p(y)
+    assert so.cb_rmsnorm_fwd(ctx.h, C.byref(d)) == -1 and b"exactly one" in so.cb_last_error()
+    d.y = None
+    assert so.cb_rmsnorm_fwd(ctx.h, C.byref(d)) == -3 and b"16-byte" in so.cb_last_error()       # ldi8 = 40
+    d.ldi8, d.ldx = 48, 39
+    assert so.cb_rmsnorm_fwd(ctx.h, C.byref(d)) == -3 and b"shorter" in so.cb_last_error()
+    d.ldx, d.struct_size = 40, 8
+    assert so.cb_rmsnorm_fwd(ctx.h, C.byref(d)) == -1
+    d.struct_size = C.sizeof(d)
+    d.h = d.dy = d.dh = p(y)
+    d.ldh = d.lddy = d.lddh = 40
+    d.dgamma, d.workspace_bytes = p(y), 0
+    assert so.cb_rmsnorm_bwd(ctx.h, C.byref(d)) == -1 and b"workspace" in so.cb_last_error()
+
+
+def test_rows_and_product_accept_and_refuse(dry):
+    lib, ctx = dry
+    q, s = lib.quantize_rows(ctx, torch.zeros(2, 3, 100))
+    assert q.shape == (2, 3, 112) and q.dtype == torch.int8 and s.shape == (2, 3)
+    w, ws = lib.quantize_rows(ctx, torch.zeros(50, 100))
+    assert lib.linear_i8(ctx, q, s, w, ws, bias=torch.zeros(50), residual=torch.zeros(2, 3, 50, dtype=torch.bfloat16)).shape == (2, 3, 50)
+    assert lib.linear_i8(ctx, q, s, w, ws, dtype="f32").dtype == torch.float32
+    for args, kw, what in (((q, s, w[:, :96], ws), {}, "expected"), ((q, s[:1], w, ws), {}, "a_scale"), ((q, s, w, ws.double()), {}, "w_scale"),
+                           ((q.float(), s, w, ws), {}, "int8"), ((q, s, w, ws), dict(bias=torch.zeros(49)), "bias"),
+                           ((q, s, w, ws), dict(residual=torch.zeros(2, 3, 50)), "residual"), ((q, s, w[0], ws), {}, "w has shape"),
+                           ((q[..., :100].contiguous(), s, w[:, :100].contiguous(), ws), {}, "multiple of 16"), ((q, s, w, ws), dict(dtype="f16"), "dtype")):
+        with pytest.raises((ValueError, TypeError, lib.CBError), match=what):
+            lib.linear_i8(ctx, *args, **kw)
+    with pytest.raises(lib.CBError, match="at most"):
+        lib.quantize_rows(ctx, torch.zeros(1, 131057))
+    so = lib.load()
+    d = lib.GemmI8Desc()
+    d.M, d.N, d.K, d.lda, d.ldb, d.ldc = 4, 4, 32, 40, 32, 4
+    t = torch.zeros(4, 64)
+    for k in ("A", "B", "C", "a_scale", "b_scale"):
+        setattr(d, k, t.data_ptr())
+    assert so.cb_gemm_i8(ctx.h, C.byref(d)) == -3 and b"16-byte" in so.cb_last_error()
+    d.lda, d.K = 32, 131072
+    assert so.cb_gemm_i8(ctx.h, C.byref(d)) == -3 and b"at most" in so.cb_last_error()
+    d.K, d.ldc = 32, 3
+    assert so.cb_gemm_i8(ctx.h, C.byref(d)) == -3 and b"shorter" in so.cb_last_error()
+    d.ldc, d.struct_size = 4, 1
+    assert so.cb_gemm_i8(ctx.h, C.byref(d)) == -1
