@@ -36,7 +36,7 @@ for _src in ("cb_norm_i8.hip", "cb_gemm_i8.hip"):
 # (The f2_* attention kernels drain with vmcnt(0) and do not depend on the count: scratch there is reported, not fatal.)
 if os.environ.get("CB_FLASH_ABL"):       # timing ablations of the fp32 attention backward (cb_flash.hip, FL_ABL): results are wrong under them
     EXTRA["cb_flash.hip"] = EXTRA["cb_flash.hip"] + ["-DFL_ABL=" + str(int(os.environ["CB_FLASH_ABL"]))]
-NO_SCRATCH = {"cb_gemm_glds.hip": ("gemm_glds", True), "cb_gemm_bf16_p8.hip": ("gemm_bf16_p8", True), "cb_flash_bf16_v2.hip": ("f2_", False)}
+NO_SCRATCH = {"cb_gemm_glds.hip": ("gemm_glds", True), "cb_gemm_bf16_p8.hip": ("gemm_bf16_p8", True), "cb_flash_bf16_v2.hip": ("f2_", False), "cb_gemm_i8.hip": ("gemm_i8_p8", True)}
 
 
 def source_digest():

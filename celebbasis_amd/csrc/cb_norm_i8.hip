@@ -243,18 +243,23 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsArgs a, const int
         for (int c = threadIdx.x; c < C; c += 256) P[c] = dgs[c];
     }
 }
-// dgamma[c] = sum of the parts in order: 64 columns a block, 4 runs of parts
+// dgamma[c] = sum of the parts in a fixed order: 16 columns a block (one 64-byte piece of a part), 16 runs of parts joined in LDS
 __global__ __launch_bounds__(256) void rms_dgamma_kernel(const float* __restrict__ part, float* __restrict__ dgamma, int n, int C) {
-    __shared__ float sh[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+    __shared__ float sh[16][17];
+    const int x = threadIdx.x & 15, w = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
     float s = 0.f;
     if (c < C) {
-        const int per = (n + 3) / 4, i1 = min(n, (w + 1) * per);
-        for (int i = w * per; i < i1; ++i) s += part[(long)i * C + c];
+#pragma unroll 8
+        for (int i = w; i < n; i += 16) s += part[(long)i * C + c];
     }
-    sh[w][threadIdx.x & 63] = s;
+    sh[w][x] = s;
     __syncthreads();
-    if (w == 0 && c < C) dgamma[c] = (sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]);
+    if (w == 0 && c < C) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += sh[i][x];
+        dgamma[c] = t;
+    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -307,7 +312,7 @@ void k_rmsnorm_bwd(const Launch& L, const RmsArgs& a) {
         if (vec) RMS_GO((rms_bwd_kernel<T, TPR, NV, true>), (unsigned)n, a, per);
         else RMS_GO((rms_bwd_kernel<T, TPR, NV, false>), (unsigned)n, a, per);
     }));
-    if (a.dgamma) RMS_GO(rms_dgamma_kernel, cdiv(a.C, 64), a.part, a.dgamma, n, a.C);
+    if (a.dgamma) RMS_GO(rms_dgamma_kernel, cdiv(a.C, 16), a.part, a.dgamma, n, a.C);
 }
 
 }  // namespace cb
