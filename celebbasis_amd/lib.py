@@ -6,6 +6,7 @@ calls raise.
 """
 import ctypes as C
 import os
+import struct
 
 import torch  # imported BEFORE the .so so that the process holds a single HIP runtime (torch's libamdhip64.so.7)
 
@@ -694,23 +695,50 @@ class Trainer(_Handle):
 # ---------------------------------------------------------------- sequence attention, residual RMS norm, 8-bit products
 # Outputs and workspaces of these calls come from torch's allocator on the context's stream, so the calls run on that stream and no other:
 # a caller whose current stream is another one is refused rather than raced (make the context under the stream that will capture).
+# The small calls are bound by the host: a descriptor is packed in one go (its ctypes class above documents it and is what a caller without
+# these wrappers fills), and the sizes of workspaces, which depend on the shape alone, are asked for once a shape.
+def _packer(cls):
+    code = {C.c_int: "i", C.c_int64: "q", C.c_void_p: "P", C.c_float: "f"}
+    fmt = "".join("Pqqq" if t is SeqTensor else code[t] for _, t in cls._fields_)
+    st = struct.Struct("@" + fmt)
+    assert st.size <= C.sizeof(cls) < st.size + 8, cls          # at most the padding behind the last member
+    return struct.Struct("@" + fmt + "x" * (C.sizeof(cls) - st.size)).pack, C.sizeof(cls)
+
+
+_seq_pack, _SEQ_SIZE = _packer(SeqAttentionDesc)
+_rms_pack, _RMS_SIZE = _packer(RmsNormDesc)
+_gemm_i8_pack, _GEMM_I8_SIZE = _packer(GemmI8Desc)
+_NO_TENSOR = (0, 0, 0, 0)
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _place(ctx, **tensors):
     """every given tensor is on the context's device, and the current stream is the context's"""
     if ctx.dry:
         return
+    dev = ctx.device
     for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device.index != ctx.device):
-            raise ValueError(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
-    if torch.cuda.current_stream(ctx.device).cuda_stream != ctx.stream_ptr:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} is on {t.device}, the context on cuda:{dev}")
+    if _current_stream(dev) != ctx.stream_ptr:
         raise ValueError("the current stream is not the stream the context was created on")
 
 
-def _device_of(ctx):
-    return torch.device("cpu") if ctx.dry else torch.device("cuda", ctx.device)
-
-
-def _workspace(ctx, n):
-    return torch.empty(n, dtype=torch.uint8, device=_device_of(ctx)) if n else None
+def _workspace(ctx, key, ask, device):
+    """(tensor or None, pointer, bytes) of a call's workspace; `ask` gets the size from the library the first time a shape is seen"""
+    sizes = ctx.__dict__.setdefault("_ws_sizes", {})
+    n = sizes.get(key)
+    if n is None:
+        v = C.c_int64()
+        check(ask(v))
+        if len(sizes) > 4096:
+            sizes.clear()
+        n = sizes[key] = v.value
+    if not n:
+        return None, 0, 0
+    t = torch.empty(n, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), n
 
 
 class RelPos(_Handle):
@@ -731,71 +759,72 @@ class RelPos(_Handle):
 
 
 def _seq_tensor(t, name, shape, dtype):
+    """the members of a cb_seq_tensor"""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape} ([batch, tokens, heads, d])")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)} ([batch, tokens, heads, d])")
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected dtype {dtype}, got {t.dtype}")
-    s = t.stride()
-    if s[3] != 1:
+    sb, sn, sh, sd = t.stride()
+    if sd != 1:
         raise ValueError(f"{name}: the head dim must be contiguous")
+    B, N, H, _ = shape
     # the stride of a dimension of one element says nothing: 0 passes every check
-    return SeqTensor(t.data_ptr() or None, s[1] if shape[1] > 1 else 0, s[2] if shape[2] > 1 else 0, s[0] if shape[0] > 1 else 0)
+    return (t.data_ptr(), sn if N > 1 else 0, sh if H > 1 else 0, sb if B > 1 else 0)
 
 
 def _per_sample(t, name, B):
     if t is None:
-        return None
-    if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous():
+        return 0
+    if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous int32 tensor of shape ({B},), got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 class SeqTape:
     """what the forward call leaves for its backward: the inputs (by reference), the output and its row statistics"""
-    __slots__ = ("q", "k", "v", "out", "lse", "out32", "kw")
+    __slots__ = ("q", "k", "v", "out", "lse", "out32", "table", "keep", "head", "mid", "key")
 
 
 class SeqGrads:
     __slots__ = ("dq", "dk", "dv", "dtable")
 
 
-def _seq_desc(ctx, q, k, v, scale, causal, q_pos, q_len, kv_len, kv_mask, relpos, table):
+SEQ_SHORT = 128       # key axes up to here: the backward pass makes its row sums from the probabilities and reads neither out nor out32
+
+
+def _seq_inputs(ctx, q, k, v, scale, causal, q_pos, q_len, kv_len, kv_mask, relpos, table):
+    """the descriptor's members before `out` and those between `out` and `lse`, checked; and the shape that workspaces go by"""
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q, k and v are [batch, tokens, heads, d]")
     B, Nq, H, d = q.shape
-    Nk, Hkv = k.shape[1], k.shape[2]
-    if q.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"q: expected float32 or bfloat16, got {q.dtype}")
+    _, Nk, Hkv, _ = k.shape
+    dtype = q.dtype
+    if dtype != torch.bfloat16 and dtype != torch.float32:
+        raise TypeError(f"q: expected float32 or bfloat16, got {dtype}")
     _place(ctx, q=q, k=k, v=v, q_pos=q_pos, q_len=q_len, kv_len=kv_len, kv_mask=kv_mask, table=table)
-    D = SeqAttentionDesc()
-    D.dtype = DTYPE_BF16 if q.dtype == torch.bfloat16 else DTYPE_F32
-    D.B, D.Nq, D.Nk, D.heads, D.kv_heads, D.d = B, Nq, Nk, H, Hkv, d
-    D.scale, D.causal = d ** -0.5 if scale is None else float(scale), 1 if causal else 0
-    D.q = _seq_tensor(q, "q", (B, Nq, H, d), q.dtype)
-    D.k = _seq_tensor(k, "k", (B, Nk, Hkv, d), q.dtype)
-    D.v = _seq_tensor(v, "v", (B, Nk, Hkv, d), q.dtype)
-    D.q_pos, D.q_len, D.kv_len = _per_sample(q_pos, "q_pos", B), _per_sample(q_len, "q_len", B), _per_sample(kv_len, "kv_len", B)
+    code = DTYPE_BF16 if dtype == torch.bfloat16 else DTYPE_F32
+    causal = 1 if causal else 0
+    kv = (B, Nk, Hkv, d)
+    head = ((_SEQ_SIZE, code, B, Nq, Nk, H, Hkv, d, d ** -0.5 if scale is None else float(scale), causal) + _seq_tensor(q, "q", q.shape, dtype)
+            + _seq_tensor(k, "k", kv, dtype) + _seq_tensor(v, "v", kv, dtype))
+    mask, mask_stride = 0, 0
     if kv_mask is not None:
-        if kv_mask.dtype not in (torch.bool, torch.uint8) or tuple(kv_mask.shape) != (B, Nk) or (Nk > 1 and kv_mask.stride(1) != 1):
+        if kv_mask.dtype not in (torch.bool, torch.uint8) or kv_mask.shape != (B, Nk) or (Nk > 1 and kv_mask.stride(1) != 1):
             raise ValueError(f"kv_mask: expected bool or uint8 of shape ({B}, {Nk}) with contiguous rows, got {kv_mask.dtype} {tuple(kv_mask.shape)}")
-        D.kv_mask, D.mask_stride = kv_mask.data_ptr() or None, kv_mask.stride(0)
+        mask, mask_stride = kv_mask.data_ptr(), kv_mask.stride(0)
     if (relpos is None) != (table is None):
         raise ValueError("relpos and table go together")
+    rel, tab, shape = 0, 0, None
     if relpos is not None:
-        if table.dtype != torch.float32 or tuple(table.shape) != (relpos.num_buckets, H) or not table.is_contiguous():
+        if table.dtype != torch.float32 or table.shape != (relpos.num_buckets, H) or not table.is_contiguous():
             raise ValueError(f"table: expected contiguous float32 of shape ({relpos.num_buckets}, {H}), got {table.dtype} {tuple(table.shape)}")
-        D.relpos, D.table = relpos.h, table.data_ptr()
-    return D
-
-
-def _seq_workspace(ctx, D, backward):
-    n = C.c_int64()
-    check(load().cb_seq_attention_workspace(ctx.h, C.byref(D), 1 if backward else 0, C.byref(n)))
-    ws = _workspace(ctx, n.value)
-    D.workspace, D.workspace_bytes = None if ws is None else ws.data_ptr(), n.value
-    return ws
+        if not relpos.h.value:
+            raise ValueError("the relpos handle is closed")
+        rel, tab, shape = relpos.h.value, table.data_ptr(), (relpos.num_buckets, relpos.max_distance)
+    mid = (_per_sample(q_pos, "q_pos", B), _per_sample(q_len, "q_len", B), _per_sample(kv_len, "kv_len", B), mask, mask_stride, rel, tab)
+    return head, mid, (code, B, Nq, Nk, H, Hkv, d, causal, shape)
 
 
 def seq_attention(ctx, q, k, v, scale=None, causal=False, q_pos=None, q_len=None, kv_len=None, kv_mask=None, relpos=None, table=None, out=None,
@@ -805,28 +834,33 @@ def seq_attention(ctx, q, k, v, scale=None, causal=False, q_pos=None, q_len=None
     causal: key j is visible to query i where j <= q_pos[b] + i. q_pos, q_len, kv_len: int32 [B] on the device (0, Nq, Nk by default).
     kv_mask: bool or uint8 [B, Nk], non-zero = visible. relpos + table [num_buckets, heads]: learned bias by the distance key - query.
     Rows at or beyond q_len and rows that see no key are 0.
-    Returns out [B, Nq, heads, d] (or `out`, written), with need_grad (out, tape) for seq_attention_backward."""
-    D = _seq_desc(ctx, q, k, v, scale, causal, q_pos, q_len, kv_len, kv_mask, relpos, table)
-    dev = q.device
+    Returns out [B, Nq, heads, d] (or `out`, written), with need_grad (out, tape) for seq_attention_backward. The backward call reads the
+    inputs again: they, lengths and masks included, must still hold what the forward call saw."""
+    head, mid, key = _seq_inputs(ctx, q, k, v, scale, causal, q_pos, q_len, kv_len, kv_mask, relpos, table)
+    dev, dtype, shape = q.device, q.dtype, q.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty(shape, dtype=dtype, device=dev)
     else:
         _place(ctx, out=out)
-    D.out = _seq_tensor(out, "out", tuple(q.shape), q.dtype)
+    o = _seq_tensor(out, "out", shape, dtype)
     lse = out32 = None
+    lp = op = 0
     if need_grad:
-        lse = torch.empty((D.B, D.heads, D.Nq), dtype=torch.float32, device=dev)
-        D.lse = lse.data_ptr() or None
-        if q.dtype == torch.bfloat16 and table is not None:
-            out32 = torch.empty(q.shape, dtype=torch.float32, device=dev)
-            D.out32 = out32.data_ptr() or None
-    ws = _seq_workspace(ctx, D, False)
-    check(load().cb_seq_attention_fwd(ctx.h, C.byref(D)))
+        lse = torch.empty((shape[0], shape[2], shape[1]), dtype=torch.float32, device=dev)
+        lp = lse.data_ptr()
+        if dtype == torch.bfloat16 and k.shape[1] > SEQ_SHORT:
+            out32 = torch.empty(shape, dtype=torch.float32, device=dev)
+            op = out32.data_ptr()
+    L = load()
+    mine = head + o + mid + (lp, op) + _NO_TENSOR * 4 + (0,)
+    ws, wp, wn = _workspace(ctx, ("seq", False) + key, lambda n: L.cb_seq_attention_workspace(ctx.h, _seq_pack(*mine, 0, 0), 0, C.byref(n)), dev)
+    check(L.cb_seq_attention_fwd(ctx.h, _seq_pack(*mine, wp, wn)))
     if not need_grad:
         return out
     t = SeqTape()
-    t.q, t.k, t.v, t.out, t.lse, t.out32 = q, k, v, out, lse, out32
-    t.kw = dict(scale=scale, causal=causal, q_pos=q_pos, q_len=q_len, kv_len=kv_len, kv_mask=kv_mask, relpos=relpos, table=table)
+    t.q, t.k, t.v, t.out, t.lse, t.out32, t.table = q, k, v, out, lse, out32, table
+    t.keep = (q_pos, q_len, kv_len, kv_mask, relpos)
+    t.head, t.mid, t.key = head + o, mid + (lp, op), key
     return out, t
 
 
@@ -834,58 +868,61 @@ def seq_attention_backward(ctx, tape, dout, dq=None, dk=None, dv=None, want_dtab
     """Gradients of seq_attention (cb_seq_attention_bwd) -> SeqGrads(dq, dk, dv, dtable). dq / dk / dv may be given as views to write into (slices
     of a fused projection's gradient); dk and dv are summed over the query heads that share a key / value head, dtable [num_buckets, heads]
     is float32. The call neither changes the tape nor adds to earlier results."""
-    q, k, v = tape.q, tape.k, tape.v
-    D = _seq_desc(ctx, q, k, v, **tape.kw)
-    _place(ctx, dout=dout, dq=dq, dk=dk, dv=dv)
+    q, k, table = tape.q, tape.k, tape.table
+    dtype, dev = q.dtype, q.device
+    _place(ctx, q=q, dout=dout, dq=dq, dk=dk, dv=dv)
+    if tape.keep[4] is not None and not tape.keep[4].h.value:
+        raise ValueError("the relpos handle is closed")
     g = SeqGrads()
-    g.dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if dq is None else dq
-    g.dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if dk is None else dk
-    g.dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if dv is None else dv
-    D.out = _seq_tensor(tape.out, "out", tuple(q.shape), q.dtype)
-    D.dout = _seq_tensor(dout, "dout", tuple(q.shape), q.dtype)
-    D.dq = _seq_tensor(g.dq, "dq", tuple(q.shape), q.dtype)
-    D.dk = _seq_tensor(g.dk, "dk", tuple(k.shape), q.dtype)
-    D.dv = _seq_tensor(g.dv, "dv", tuple(v.shape), q.dtype)
-    D.lse = tape.lse.data_ptr() or None
-    D.out32 = (tape.out32.data_ptr() or None) if tape.out32 is not None else None
-    table = tape.kw["table"]
-    g.dtable = None
+    g.dq = torch.empty(q.shape, dtype=dtype, device=dev) if dq is None else dq
+    g.dk = torch.empty(k.shape, dtype=dtype, device=dev) if dk is None else dk
+    g.dv = torch.empty(k.shape, dtype=dtype, device=dev) if dv is None else dv
+    grads = (_seq_tensor(dout, "dout", q.shape, dtype) + _seq_tensor(g.dq, "dq", q.shape, dtype) + _seq_tensor(g.dk, "dk", k.shape, dtype)
+             + _seq_tensor(g.dv, "dv", k.shape, dtype))
+    g.dtable, tp = None, 0
     if table is not None and want_dtable:
-        g.dtable = torch.empty(table.shape, dtype=torch.float32, device=table.device)
-        D.dtable = g.dtable.data_ptr()
-    ws = _seq_workspace(ctx, D, True)
-    check(load().cb_seq_attention_bwd(ctx.h, C.byref(D)))
+        g.dtable = torch.empty(table.shape, dtype=torch.float32, device=dev)
+        tp = g.dtable.data_ptr()
+    L = load()
+    mine = tape.head + tape.mid + grads + (tp,)
+    ws, wp, wn = _workspace(ctx, ("seq", True, tp != 0) + tape.key, lambda n: L.cb_seq_attention_workspace(ctx.h, _seq_pack(*mine, 0, 0), 1, C.byref(n)), dev)
+    check(L.cb_seq_attention_bwd(ctx.h, _seq_pack(*mine, wp, wn)))
     return g
 
 
-def _rows(t, name, C=None, dtype=None):
+def _rows(t, name, n=None, dtype=None):
     """(pointer, row stride, rows, columns) of [..., C]: two dimensions with any row stride, or a contiguous tensor of any"""
-    if t.dim() < 1 or (C is not None and t.shape[-1] != C):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected [..., {C}]")
+    shape = t.shape
+    nd = len(shape)
+    if nd < 1 or (n is not None and shape[-1] != n):
+        raise ValueError(f"{name} has shape {tuple(shape)}, expected [..., {n}]")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name}: expected dtype {dtype}, got {t.dtype}")
-    n = t.shape[-1]
-    if t.dim() == 2:
-        if n > 1 and t.stride(1) != 1:
+    n = shape[-1]
+    if nd == 2:
+        s0, s1 = t.stride()
+        if n > 1 and s1 != 1:
             raise ValueError(f"{name}: rows must be contiguous")
-        return t.data_ptr() or None, t.stride(0) if t.shape[0] > 1 else n, t.shape[0], n
+        return t.data_ptr(), s0 if shape[0] > 1 else n, shape[0], n
     if not t.is_contiguous():
         raise ValueError(f"{name}: tensor must be contiguous (or two-dimensional with contiguous rows)")
-    return t.data_ptr() or None, n, t.numel() // n if n else 0, n
+    return t.data_ptr(), n, t.numel() // n if n else 0, n
 
 
 def _vector(t, name, n):
     if t is None:
-        return None
+        return 0
     if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name}: expected {n} contiguous float32 values, got {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr() or None
+    return t.data_ptr()
 
 
 def _float_code(t, name):
-    if t.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
-    return DTYPE_BF16 if t.dtype == torch.bfloat16 else DTYPE_F32
+    if t.dtype == torch.bfloat16:
+        return DTYPE_BF16
+    if t.dtype == torch.float32:
+        return DTYPE_F32
+    raise TypeError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
 
 
 def padded_i8(n):
@@ -901,58 +938,55 @@ class RmsOut:
 def rms_norm(ctx, x, weight, residual=None, eps=1e-6, out=None, need_grad=False):
     """Root-mean-square norm over the last dim with the residual's addition (cb_rmsnorm_fwd): h = x + residual, y = h / rms(h) * weight.
     out="i8": y in 8 bits with a scale per row, ready for linear_i8. need_grad keeps rstd. x [..., C] fp32 or bf16, weight float32 [C] -> RmsOut."""
-    if out not in (None, "i8"):
+    if out is not None and out != "i8":
         raise ValueError(f"out = {out!r}: None or 'i8'")
     _place(ctx, x=x, weight=weight, residual=residual)
-    d = RmsNormDesc()
-    d.dtype = _float_code(x, "x")
-    d.x, d.ldx, d.rows, d.C = _rows(x, "x")
-    d.eps, d.gamma = float(eps), _vector(weight, "weight", d.C)
-    lead = tuple(x.shape[:-1])
+    code, dev, shape = _float_code(x, "x"), x.device, x.shape
+    xp, ldx, rows, n = _rows(x, "x")
+    lead = shape[:-1]
     r = RmsOut()
     r.h, r.scale, r.rstd = x, None, None
+    rp, ldr, hp, yp, qp, ldq, sp, tp = (0,) * 8
     if residual is not None:
-        if residual.shape != x.shape:
-            raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
-        d.residual, d.ldres = _rows(residual, "residual", d.C, x.dtype)[:2]
-        r.h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        d.h, d.ldh = r.h.data_ptr() or None, d.C
-    if out == "i8":
-        r.y = torch.empty(lead + (padded_i8(d.C),), dtype=torch.int8, device=x.device)
-        r.scale = torch.empty(lead, dtype=torch.float32, device=x.device)
-        d.y_i8, d.ldi8, d.scale = r.y.data_ptr() or None, r.y.shape[-1], r.scale.data_ptr() or None
+        if residual.shape != shape:
+            raise ValueError(f"residual has shape {tuple(residual.shape)}, x {tuple(shape)}")
+        rp, ldr = _rows(residual, "residual", n, x.dtype)[:2]
+        r.h = torch.empty(shape, dtype=x.dtype, device=dev)
+        hp = r.h.data_ptr()
+    if out is None:
+        r.y = torch.empty(shape, dtype=x.dtype, device=dev)
+        yp = r.y.data_ptr()
     else:
-        r.y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        d.y, d.ldy = r.y.data_ptr() or None, d.C
+        ldq = padded_i8(n)
+        r.y = torch.empty(lead + (ldq,), dtype=torch.int8, device=dev)
+        r.scale = torch.empty(lead, dtype=torch.float32, device=dev)
+        qp, sp = r.y.data_ptr(), r.scale.data_ptr()
     if need_grad:
-        r.rstd = torch.empty(lead, dtype=torch.float32, device=x.device)
-        d.rstd = r.rstd.data_ptr() or None
-    check(load().cb_rmsnorm_fwd(ctx.h, C.byref(d)))
+        r.rstd = torch.empty(lead, dtype=torch.float32, device=dev)
+        tp = r.rstd.data_ptr()
+    check(load().cb_rmsnorm_fwd(ctx.h, _rms_pack(_RMS_SIZE, code, rows, n, eps, xp, ldx, rp, ldr, _vector(weight, "weight", n), hp, n, yp, n, qp, ldq, sp, tp,
+                                                 0, 0, 0, 0, 0, 0, 0, 0, 0)))
     return r
 
 
 def rms_norm_backward(ctx, dy, h, weight, rstd, dres=None, want_dweight=True):
     """(dh, dweight) of rms_norm: dh is the gradient of x and of the residual alike; dres: what flows into h from elsewhere"""
     _place(ctx, dy=dy, h=h, weight=weight, rstd=rstd, dres=dres)
-    d = RmsNormDesc()
-    d.dtype = _float_code(h, "h")
-    d.h, d.ldh, d.rows, d.C = _rows(h, "h")
-    d.gamma, d.rstd = _vector(weight, "weight", d.C), _vector(rstd, "rstd", d.rows)
+    code, dev, dtype = _float_code(h, "h"), h.device, h.dtype
+    hp, ldh, rows, n = _rows(h, "h")
     if dy.shape != h.shape or (dres is not None and dres.shape != h.shape):
         raise ValueError(f"dy {tuple(dy.shape)} and dres must have h's shape {tuple(h.shape)}")
-    d.dy, d.lddy = _rows(dy, "dy", d.C, h.dtype)[:2]
-    if dres is not None:
-        d.dres, d.lddres = _rows(dres, "dres", d.C, h.dtype)[:2]
-    dh = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    d.dh, d.lddh = dh.data_ptr() or None, d.C
-    dw = ws = None
+    dyp, lddy = _rows(dy, "dy", n, dtype)[:2]
+    drp, lddr = _rows(dres, "dres", n, dtype)[:2] if dres is not None else (0, 0)
+    dh = torch.empty(h.shape, dtype=dtype, device=dev)
+    L = load()
+    dw, dwp, ws, wp, wn = None, 0, None, 0, 0
     if want_dweight:
-        dw = torch.empty(d.C, dtype=torch.float32, device=h.device)
-        n = C.c_int64()
-        check(load().cb_rmsnorm_workspace(ctx.h, d.rows, d.C, C.byref(n)))
-        ws = _workspace(ctx, n.value)
-        d.dgamma, d.workspace, d.workspace_bytes = dw.data_ptr(), None if ws is None else ws.data_ptr(), n.value
-    check(load().cb_rmsnorm_bwd(ctx.h, C.byref(d)))
+        dw = torch.empty(n, dtype=torch.float32, device=dev)
+        dwp = dw.data_ptr()
+        ws, wp, wn = _workspace(ctx, ("rms", rows, n), lambda v: L.cb_rmsnorm_workspace(ctx.h, rows, n, C.byref(v)), dev)
+    check(L.cb_rmsnorm_bwd(ctx.h, _rms_pack(_RMS_SIZE, code, rows, n, 0.0, 0, 0, 0, 0, _vector(weight, "weight", n), hp, ldh, 0, 0, 0, 0, 0, _vector(rstd, "rstd", rows),
+                                            dyp, lddy, drp, lddr, dh.data_ptr(), n, dwp, wp, wn)))
     return dh, dw
 
 
@@ -962,10 +996,10 @@ def quantize_rows(ctx, x):
     _place(ctx, x=x)
     code = _float_code(x, "x")
     p, ld, rows, n = _rows(x, "x")
-    lead = tuple(x.shape[:-1])
-    q = torch.empty(lead + (padded_i8(n),), dtype=torch.int8, device=x.device)
+    lead, ldq = x.shape[:-1], padded_i8(n)
+    q = torch.empty(lead + (ldq,), dtype=torch.int8, device=x.device)
     scale = torch.empty(lead, dtype=torch.float32, device=x.device)
-    check(load().cb_quantize_rows(ctx.h, code, p, ld, rows, n, q.data_ptr() or None, q.shape[-1], scale.data_ptr() or None))
+    check(load().cb_quantize_rows(ctx.h, code, p, ld, rows, n, q.data_ptr(), ldq, scale.data_ptr()))
     return q, scale
 
 
@@ -973,22 +1007,21 @@ def linear_i8(ctx, a, a_scale, w, w_scale, bias=None, residual=None, dtype="bf16
     """a_scale * w_scale * (a . w^T) + bias + residual (cb_gemm_i8): a int8 [..., K], w int8 [N, K] (K padded by quantize_rows / rms_norm),
     a_scale [...], w_scale [N], bias float32 [N], residual [..., N] of the output's dtype -> [..., N]"""
     _place(ctx, a=a, a_scale=a_scale, w=w, w_scale=w_scale, bias=bias, residual=residual)
-    d = GemmI8Desc()
-    d.dtype = dtype_code(dtype)
+    code = dtype_code(dtype)
     if w.dim() != 2:
         raise ValueError(f"w has shape {tuple(w.shape)}, expected [N, K]")
-    d.A, d.lda, d.M, d.K = _rows(a, "a", None, torch.int8)
-    d.B, d.ldb, d.N, _ = _rows(w, "w", d.K, torch.int8)
-    d.a_scale, d.b_scale, d.bias = _vector(a_scale, "a_scale", d.M), _vector(w_scale, "w_scale", d.N), _vector(bias, "bias", d.N)
-    out = torch.empty(tuple(a.shape[:-1]) + (d.N,), dtype=torch_dtype(d.dtype), device=a.device)
-    d.C, d.ldc = out.data_ptr() or None, d.N
+    ap, lda, m, k = _rows(a, "a", None, torch.int8)
+    bp, ldb, n, _ = _rows(w, "w", k, torch.int8)
+    dev, odt = a.device, torch_dtype(code)
+    out = torch.empty(a.shape[:-1] + (n,), dtype=odt, device=dev)
+    rp, ldr = 0, 0
     if residual is not None:
         if residual.shape != out.shape:
             raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {tuple(out.shape)}")
-        d.R, d.ldr = _rows(residual, "residual", d.N, out.dtype)[:2]
-    n = C.c_int64()
-    check(load().cb_gemm_i8_workspace(ctx.h, C.byref(d), C.byref(n)))
-    ws = _workspace(ctx, n.value)
-    d.workspace, d.workspace_bytes = None if ws is None else ws.data_ptr(), n.value
-    check(load().cb_gemm_i8(ctx.h, C.byref(d)))
+        rp, ldr = _rows(residual, "residual", n, odt)[:2]
+    L = load()
+    mine = (_GEMM_I8_SIZE, code, m, n, k, ap, lda, bp, ldb, _vector(a_scale, "a_scale", m), _vector(w_scale, "w_scale", n), _vector(bias, "bias", n), rp, ldr,
+            out.data_ptr(), n)
+    ws, wp, wn = _workspace(ctx, ("i8", m, n, k), lambda v: L.cb_gemm_i8_workspace(ctx.h, _gemm_i8_pack(*mine, 0, 0), C.byref(v)), dev)
+    check(L.cb_gemm_i8(ctx.h, _gemm_i8_pack(*mine, wp, wn)))
     return out

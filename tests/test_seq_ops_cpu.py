@@ -122,16 +122,17 @@ def test_seq_attention_descriptor_refusals(dry):
     """what the Python wrapper cannot express: a foreign struct size, a short or misaligned workspace, gradients of a table that is not there"""
     lib, ctx = dry
     q, k, v = qkv()
-    out, tape = lib.seq_attention(ctx, q, k, v, need_grad=True)
-    D = lib._seq_desc(ctx, q, k, v, **tape.kw)
-    D.out = lib._seq_tensor(out, "out", tuple(q.shape), q.dtype)
+    D = lib.SeqAttentionDesc()
+    D.B, D.Nq, D.Nk, D.heads, D.kv_heads, D.d, D.scale = 2, 5, 7, 4, 2, 16, 0.25
+    out, lse = torch.zeros_like(q), torch.zeros(2, 4, 5)
+    D.lse = lse.data_ptr()
+    for x, t in (("q", q), ("k", k), ("v", v), ("out", out), ("dout", out), ("dq", q), ("dk", k), ("dv", v)):
+        setattr(D, x, lib.SeqTensor(t.data_ptr(), t.stride(1), t.stride(2), t.stride(0)))
     so = lib.load()
     D.struct_size -= 8
     assert so.cb_seq_attention_fwd(ctx.h, C.byref(D)) == -1 and b"struct_size" in so.cb_last_error()
     D.struct_size += 8
     assert so.cb_seq_attention_fwd(ctx.h, None) == -1 and so.cb_seq_attention_fwd(None, C.byref(D)) == -1
-    for x, t in (("dout", out), ("dq", q), ("dk", k), ("dv", v)):
-        setattr(D, x, lib._seq_tensor(t, x, tuple(t.shape), t.dtype))
     need = C.c_int64()
     assert so.cb_seq_attention_workspace(ctx.h, C.byref(D), 1, C.byref(need)) == 0 and need.value > 0
     D.workspace_bytes = need.value - 1
