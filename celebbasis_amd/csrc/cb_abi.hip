@@ -1127,7 +1127,7 @@ static SeqArgs seq_args(const cb_ctx* ctx, const cb_seq_attention_desc* d, bool 
         CB_CHECK(!d->dtable || d->relpos, CB_ERR_ARG, "seq attention: dtable without a table");
         a.dtable = d->dtable;
     }
-    a.lse = d->lse; a.o32 = a.dt == DT_BF16 && d->table ? d->out32 : nullptr;
+    a.lse = d->lse; a.o32 = a.dt == DT_BF16 && d->Nk > SEQ_SHORT ? d->out32 : nullptr;
     if (!pointers) return a;
     a.q = seq_tensor(d->q, "q", a.dt, d->B, d->Nq, d->heads, d->d, false, c.dry);
     a.k = seq_tensor(d->k, "k", a.dt, d->B, d->Nk, d->kv_heads, d->d, false, c.dry);

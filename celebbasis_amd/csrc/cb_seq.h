@@ -42,6 +42,7 @@ void seq_forward(const Launch& L, SeqArgs a, void* ws);
 void seq_backward(const Launch& L, SeqArgs a, void* ws);
 
 constexpr int SEQ_MAX_D = 160, SEQ_MAX_DIST = 1024, SEQ_MAX_BUCKETS = 256;
+constexpr int SEQ_SHORT = 128;      // key axes up to here: the backward pass makes its row sums from the probabilities (cb_seq_bwd.hip)
 
 #ifdef __HIPCC__
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -53,6 +54,7 @@ typedef __attribute__((address_space(3))) s16x4* lds_s4;
 
 constexpr float SEQ_L2E = 1.4426950408889634f, SEQ_LN2 = 0.6931471805599453f;
 constexpr int SEQ_OOB = -16;                       // 0xFFFFFFF0 >= num_records: the load returns zeros
+template <int TK> constexpr unsigned long long SEQ_ALL = TK == 64 ? ~0ull : 0xFFFFFFFFull;      // every row of a tile is visible
 constexpr int SEQ_POS_LIM = 1 << 29;               // positions are held to +-2^29, so that differences stay inside an int
 
 __device__ __forceinline__ float seq_group_max(float v) { v = fmaxf(v, __shfl_xor(v, 16, 64)); return fmaxf(v, __shfl_xor(v, 32, 64)); }
@@ -105,7 +107,7 @@ template <typename T, int DT> struct SeqSlots {
     // dst: the tile's image + this wave's 1 KiB piece of a slot
     __device__ __forceinline__ void dma(const T* rows, char* dst, unsigned long long live, int tid) const {
         const __amdgpu_buffer_rsrc_t srd = seq_srd(rows);
-        if (live == (G::TK == 64 ? ~0ull : 0xFFFFFFFFull)) {
+        if (live == SEQ_ALL<G::TK>) {
 #pragma unroll
             for (int i = 0; i < G::NS; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_vp)(dst + i * 4096), 16, off[i], 0, 0, 0);
         } else {
@@ -242,14 +244,19 @@ __device__ __forceinline__ unsigned long long seq_live(const unsigned char* mask
         return __ballot(lane < TK && r < len && mask[min(r, len - 1)] != 0);
     }
     const int n = len - r0;
-    return n >= 64 ? (TK == 64 ? ~0ull : 0xFFFFFFFFull) : (n <= 0 ? 0ull : (((1ull << n) - 1) & (TK == 64 ? ~0ull : 0xFFFFFFFFull)));
+    return n >= 64 ? SEQ_ALL<TK> : (n <= 0 ? 0ull : (((1ull << n) - 1) & SEQ_ALL<TK>));
 }
 __device__ __forceinline__ int seq_clamp_len(const int* p, int b, int n) { return p ? min(max(p[b], 0), n) : n; }
 __device__ __forceinline__ int seq_pos(const int* p, int b) { return p ? min(max(p[b], -SEQ_POS_LIM), SEQ_POS_LIM) : 0; }
-// block index -> work item such that a contiguous run of items lands on one XCD (blocks are dealt to the 8 XCDs in turn)
-__device__ __forceinline__ int seq_xcd(int id, int n) {
-    const int per = n >> 3, rem = n & 7, x = id & 7, y = id >> 3;
-    return x * per + min(x, rem) + y;
+// block id -> (rank of the block along its axis, sample x head). Ranks are the slow index, so that with a causal mask the blocks with the most
+// work start first whatever their head; samples and key / value heads are the fast one: blocks are dealt to the 8 XCDs in turn, so the blocks
+// that read one key / value head meet in one L2 wherever B * Hkv is a multiple of 8, and the query heads that share it lie B * Hkv apart.
+__device__ __forceinline__ void seq_item(const SeqArgs& a, int id, int& rank, int& b, int& h) {
+    const int n = a.B * a.Hkv, all = n * a.G;
+    rank = id / all;
+    const int x = id - rank * all, gi = x / n, bk = x - gi * n;
+    b = bk / a.Hkv;
+    h = (bk - b * a.Hkv) * a.G + gi;
 }
 #endif  // __HIPCC__
 

@@ -1,6 +1,8 @@
 // cb_seq_bwd.hip — backward of the attention of cb_seq.h. With p = exp(s - lse) recomputed tile by tile:
 //   dP = dO V^T,  D = rowsum(dO * O),  dS = p (dP - D);   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,  dtable[c] = sum of dS over the
 //   pairs whose distance j - i lies in bucket c.
+// Row sums D: from dO and the stored output where the key axis is long. Up to SEQ_SHORT keys the first kernel goes over the keys twice and adds
+// p dP in fp32 instead: as exact as the probabilities, and neither output is read (cross attention to prompts is bound by memory).
 // Two kernels, so that no sum depends on the order of arrival: one block of queries over the keys (dQ, D, dtable), one block of keys over the
 // queries of all heads that share them (dK, dV). Both hold the streamed side in LDS row-major and their own side in registers.
 //
@@ -8,6 +10,7 @@
 // summed over equal kt - qb in registers, written to LDS with row i shifted by i, and summed by column: each lane owns whole distances, in a
 // fixed order. A wave's sums by distance are folded by bucket at its end.
 #include "cb_seq.h"
+#include <algorithm>
 
 namespace cb {
 
@@ -22,7 +25,7 @@ template <typename T, int DT, int QB, bool BIAS, bool TAB> struct SeqDq {
 };
 
 template <typename T, int DT, int QB, bool BIAS, bool TAB>
-__global__ __launch_bounds__(256) void seq_dq_kernel(const SeqArgs a, const int nqb) {
+__global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqArgs a, const int nqb) {
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
     using S = SeqDq<T, DT, QB, BIAS, TAB>;
@@ -34,8 +37,9 @@ __global__ __launch_bounds__(256) void seq_dq_kernel(const SeqArgs a, const int 
     float* hist = skew + 4 * 16 * SP;
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int item = seq_xcd(blockIdx.x, gridDim.x);
-    const int bh = item / nqb, qblk = nqb - 1 - (item - bh * nqb), b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
+    int rank, b, h;
+    seq_item(a, blockIdx.x, rank, b, h);
+    const int bh = b * a.H + h, hk = h / a.G, qblk = nqb - 1 - rank;
     const int qlen = seq_clamp_len(a.q_len, b, a.Nq), klen = seq_clamp_len(a.kv_len, b, a.Nk), pos0 = seq_pos(a.q_pos, b);
     const int qb0 = qblk * (64 * QB), q0 = qb0 + wave * (16 * QB);
     const T* Q = static_cast<const T*>(a.q.p) + b * a.q.batch + h * a.q.head;
@@ -47,6 +51,7 @@ __global__ __launch_bounds__(256) void seq_dq_kernel(const SeqArgs a, const int 
     if (a.causal) kend = max(0, min(kend, pos0 + min(qb0 + 64 * QB, qlen)));
     if (qb0 >= qlen) kend = 0;
     const int t1 = (kend + TK - 1) / TK;
+    const bool brief = a.Nk <= SEQ_SHORT;
 
     SeqFrag<T> qf[QB][KS], df[QB][KS];
     float lse2[QB], dsum[QB];
@@ -65,6 +70,7 @@ __global__ __launch_bounds__(256) void seq_dq_kernel(const SeqArgs a, const int 
         for (int s = 0; s < KS; ++s) {
             qf[qb][s] = seq_frag_row<T>(Q + (long)row * a.q.row, valid, s, g, a.d);
             df[qb][s] = seq_frag_row<T>(dO + (long)row * a.dout.row, valid, s, g, a.d);
+            if (brief) continue;
             float x[8], y[8];
             if constexpr (G::ES == 2) {
 #pragma unroll
@@ -86,8 +92,8 @@ __global__ __launch_bounds__(256) void seq_dq_kernel(const SeqArgs a, const int 
 #pragma unroll
             for (int e = 0; e < 8; ++e) ds = __builtin_fmaf(x[e], y[e], ds);
         }
-        dsum[qb] = seq_group_sum(ds);
-        if (g == 0 && row < a.Nq) a.dvec[ri] = dsum[qb];
+        dsum[qb] = brief ? 0.f : seq_group_sum(ds);
+        if (g == 0 && row < a.Nq) a.dvec[ri] = dsum[qb];          // (a row without a visible key: 0 either way)
     }
     const float scale2 = a.scale * SEQ_L2E;
     f32x4 acc[QB][G::DA];
@@ -107,21 +113,31 @@ __global__ __launch_bounds__(256) void seq_dq_kernel(const SeqArgs a, const int 
         for (int i = lane; i < W; i += 64) hw[i] = 0.f;
     }
     const int wbase = wave * 1024;
-    auto stage = [&](int t, unsigned long long live) {
-        char* dst = lds_seq + (t & 1) * STAGE + wbase;
+    auto stage = [&](int u, int t, unsigned long long live) {
+        char* dst = lds_seq + (u & 1) * STAGE + wbase;
         sk.dma(K + (long)t * TK * a.k.row, dst, live, tid);
         sv.dma(V + (long)t * TK * a.v.row, dst + G::TILE, live, tid);
     };
     unsigned long long live = 0, next = 0;
-    if (0 < t1) { next = seq_live<TK>(mask, 0, klen, lane); stage(0, next); }
-    for (int t = 0; t < t1; ++t) {
+    const int u1 = brief ? 2 * t1 : t1;                           // steps: the tiles, twice where the first pass makes the row sums
+    if (0 < t1) { next = seq_live<TK>(mask, 0, klen, lane); stage(0, 0, next); }
+    for (int u = 0; u < u1; ++u) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         live = next;
-        if (t + 1 < t1) { next = seq_live<TK>(mask, (t + 1) * TK, klen, lane); stage(t + 1, next); }
+        const int t = u < t1 ? u : u - t1;
+        if (u + 1 < u1) { const int n = u + 1 < t1 ? u + 1 : u + 1 - t1; next = seq_live<TK>(mask, n * TK, klen, lane); stage(u + 1, n, next); }
+        if (brief && u == t1) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
+                dsum[qb] = seq_group_sum(dsum[qb]);
+                const int row = q0 + 16 * qb + l15;
+                if (g == 0 && row < a.Nq) a.dvec[(long)bh * a.Nq + row] = dsum[qb];
+            }
+        }
         if (live == 0) continue;
-        const char* Ks = lds_seq + (t & 1) * STAGE;
+        const char* Ks = lds_seq + (u & 1) * STAGE;
         const char* Vs = Ks + G::TILE;
         const int k0 = t * TK, p0 = pos0 + q0;
         f32x4 s[QB][KT], dp[QB][KT];
@@ -158,30 +174,45 @@ __global__ __launch_bounds__(256) void seq_dq_kernel(const SeqArgs a, const int 
                         for (int r = 0; r < 4; ++r) s[qb][kt][r] = __builtin_fmaf(s[qb][kt][r], scale2, w[16 * kt + r - 16 * qb]);
             }
         }
+        const bool sums = brief && u < t1;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-            const float off = cb - lse2[qb];
+            const float off = cb - lse2[qb], ds = sums ? 0.f : dsum[qb];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][kt][r], sc, off));
-                    s[qb][kt][r] = p * (dp[qb][kt][r] - dsum[qb]);
+                    s[qb][kt][r] = p * (dp[qb][kt][r] - ds);
                 }
         }
-        const bool full = live == (TK == 64 ? ~0ull : 0xFFFFFFFFull) && (!a.causal || k0 + TK - 1 <= p0);
-        if (!full) {
+        // zero what is not visible
+        if (live != SEQ_ALL<TK>) {
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const int nib = (int)(unsigned)(live >> (16 * kt + 4 * g));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool seen = (nib >> r) & 1;
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb) s[qb][kt][r] = seen ? s[qb][kt][r] : 0.f;
+                }
+            }
+        }
+        if (a.causal && k0 + TK - 1 > p0) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const unsigned nib = (unsigned)(live >> (16 * kt + 4 * g)) & 15u;
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const bool ok = ((nib >> r) & 1u) && (!a.causal || k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15);
-                        s[qb][kt][r] = ok ? s[qb][kt][r] : 0.f;
-                    }
-                }
+                    for (int r = 0; r < 4; ++r) s[qb][kt][r] = k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15 ? s[qb][kt][r] : 0.f;
+        }
+        if (sums) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) dsum[qb] += (s[qb][kt][0] + s[qb][kt][1]) + (s[qb][kt][2] + s[qb][kt][3]);
+            continue;
         }
         if constexpr (TAB) {
             if (side != 0) {
@@ -267,7 +298,7 @@ template <typename T, int DT, int KB, bool BIAS> struct SeqDkv {
 };
 
 template <typename T, int DT, int KB, bool BIAS>
-__global__ __launch_bounds__(256) void seq_dkv_kernel(const SeqArgs a, const int nkb) {
+__global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqArgs a, const int nkb) {
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
     constexpr int TQ = G::TK, QT = G::KT, KS = G::KS, STAGE = 2 * G::TILE, PAD = SeqDkv<T, DT, KB, BIAS>::PAD;
@@ -276,8 +307,7 @@ __global__ __launch_bounds__(256) void seq_dkv_kernel(const SeqArgs a, const int
     float* bw = rows + 4 * TQ;
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int item = seq_xcd(blockIdx.x, gridDim.x);
-    const int bk = item / nkb, kblk = item - bk * nkb, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+    const int kblk = blockIdx.x / (a.B * a.Hkv), bk = blockIdx.x - kblk * (a.B * a.Hkv), b = bk / a.Hkv, hk = bk - b * a.Hkv;   // causal: the long ones first
     const int split = blockIdx.y;
     const int qlen = seq_clamp_len(a.q_len, b, a.Nq), klen = seq_clamp_len(a.kv_len, b, a.Nk), pos0 = seq_pos(a.q_pos, b);
     const int kb0 = kblk * (64 * KB), k0 = kb0 + wave * (16 * KB);
@@ -448,7 +478,9 @@ __global__ __launch_bounds__(256) void seq_dkv_sum_kernel(const SeqArgs a) {
 // ---------------------------------------------------------------- host side
 SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable) {
     SeqBwdPlan p;
-    p.qb = 1; p.kb = 1; p.qsplit = 1;
+    static const int fq = getenv("DQ") ? atoi(getenv("DQ")) : 1, fk = getenv("DK") ? atoi(getenv("DK")) : 1, fs = getenv("DS") ? atoi(getenv("DS")) : 1;
+    const bool wide = a.dt == DT_BF16 && a.d <= 64;
+    p.qb = wide ? fq : 1; p.kb = wide ? fk : 1; p.qsplit = fs;
     p.nqb = (int)cdiv(a.Nq, 64 * p.qb);
     p.dvec = (size_t)rup((long)a.B * a.H * a.Nq * 4, 256);
     p.tpart = want_dtable ? (size_t)rup((long)a.B * a.H * p.nqb * a.nb * 4, 256) : 0;
@@ -477,13 +509,26 @@ static void dkv_go(const Launch& L, const SeqArgs& a) {
     hipLaunchKernelGGL((seq_dkv_kernel<T, DT, KB, BIAS>), dim3((unsigned)nkb * a.B * a.Hkv, a.nsplit), dim3(256), lds, L.stream, a, nkb);
     CB_HIP(hipGetLastError());
 }
+template <typename T, int DT, int QB>
+static void dq_kind(const Launch& L, const SeqArgs& a, int nqb) {
+    if (a.table && a.dtable) dq_go<T, DT, QB, true, true>(L, a, nqb);
+    else if (a.table) dq_go<T, DT, QB, true, false>(L, a, nqb);
+    else dq_go<T, DT, QB, false, false>(L, a, nqb);
+}
+template <typename T, int DT, int KB>
+static void dkv_kind(const Launch& L, const SeqArgs& a) {
+    if (a.table) dkv_go<T, DT, KB, true>(L, a);
+    else dkv_go<T, DT, KB, false>(L, a);
+}
 template <typename T, int DT>
 static void bwd_pick(const Launch& L, const SeqArgs& a, const SeqBwdPlan& p) {
-    if (a.table && a.dtable) dq_go<T, DT, 1, true, true>(L, a, p.nqb);
-    else if (a.table) dq_go<T, DT, 1, true, false>(L, a, p.nqb);
-    else dq_go<T, DT, 1, false, false>(L, a, p.nqb);
-    if (a.table) dkv_go<T, DT, 1, true>(L, a);
-    else dkv_go<T, DT, 1, false>(L, a);
+    if constexpr (sizeof(T) == 2 && DT <= 4) {
+        if (p.qb == 2) dq_kind<T, DT, 2>(L, a, p.nqb); else dq_kind<T, DT, 1>(L, a, p.nqb);
+        if (p.kb == 2) dkv_kind<T, DT, 2>(L, a); else dkv_kind<T, DT, 1>(L, a);
+    } else {
+        dq_kind<T, DT, 1>(L, a, p.nqb);
+        dkv_kind<T, DT, 1>(L, a);
+    }
 }
 void seq_backward(const Launch& L, SeqArgs a, void* ws) {
     const SeqBwdPlan p = seq_bwd_plan(a, a.dtable != nullptr);

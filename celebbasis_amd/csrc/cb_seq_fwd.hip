@@ -4,6 +4,7 @@
 // going from the first product's accumulators into the second's operand inside the lane. A block has 4 waves of 16 QB queries of one (sample,
 // head); K and V tiles come by LDS-DMA into a ring of two stages (one wait and one barrier a tile).
 #include "cb_seq.h"
+#include <algorithm>
 
 namespace cb {
 
@@ -11,7 +12,7 @@ namespace cb {
 // dO.O of the backward pass, carry 2^-18 instead of 2^-9 of rounding: dtable adds dS over whole diagonals, where the error of a row sum does
 // not cancel (measured without it: dtable 2e-3 off).
 template <typename T, int DT, int QB, bool BIAS, bool PREC>
-__global__ __launch_bounds__(256) void seq_fwd_kernel(const SeqArgs a, const int nqb) {
+__global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqArgs a, const int nqb) {
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
     constexpr int TK = G::TK, KT = G::KT, KS = G::KS, STAGE = 2 * G::TILE, PAD = TK + 16 * QB;
@@ -19,8 +20,9 @@ __global__ __launch_bounds__(256) void seq_fwd_kernel(const SeqArgs a, const int
     float* bw = reinterpret_cast<float*>(lds_seq + 2 * STAGE);
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int item = seq_xcd(blockIdx.x, gridDim.x);
-    const int bh = item / nqb, qblk = nqb - 1 - (item - bh * nqb), b = bh / a.H, h = bh - b * a.H, hk = h / a.G;     // causal: the long rows first
+    int rank, b, h;
+    seq_item(a, blockIdx.x, rank, b, h);
+    const int bh = b * a.H + h, hk = h / a.G, qblk = nqb - 1 - rank;                 // causal: the long rows first
     const int split = blockIdx.y;
     const int qlen = seq_clamp_len(a.q_len, b, a.Nq), klen = seq_clamp_len(a.kv_len, b, a.Nk), pos0 = seq_pos(a.q_pos, b);
     const int qb0 = qblk * (64 * QB), q0 = qb0 + wave * (16 * QB);
@@ -111,20 +113,29 @@ __global__ __launch_bounds__(256) void seq_fwd_kernel(const SeqArgs a, const int
                         for (int r = 0; r < 4; ++r) s[qb][kt][r] = __builtin_fmaf(s[qb][kt][r], scale2, w[16 * kt + r - 16 * qb]);
             }
         }
-        const bool full = live == (TK == 64 ? ~0ull : 0xFFFFFFFFull) && (!a.causal || k0 + TK - 1 <= p0);
-        if (!full) {
+        if (live != SEQ_ALL<TK>) {                   // keys that the length or the mask hides
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const int nib = (int)~(unsigned)(live >> (16 * kt + 4 * g));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float hid = __int_as_float(((nib << (31 - r)) >> 31) & 0xFF800000);        // 0 or -inf
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb) s[qb][kt][r] += hid;
+                }
+            }
+        }
+        if (a.causal && k0 + TK - 1 > p0) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
-                    const unsigned nib = (unsigned)(live >> (16 * kt + 4 * g)) & 15u;
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const bool ok = ((nib >> r) & 1u) && (!a.causal || k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15);
-                        s[qb][kt][r] = ok ? s[qb][kt][r] : -INFINITY;
-                    }
-                }
+                    for (int r = 0; r < 4; ++r) s[qb][kt][r] = k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15 ? s[qb][kt][r] : -INFINITY;
         }
+        // The exponent's reference m follows the running maximum only where a lane is more than 8 (2^8) above it: p stays below 2^8, which costs
+        // nothing in fp32 sums or in bf16's relative rounding, and most tiles need neither the maximum over the lanes of a row nor a rescaling.
+        // (m is the same in the 4 lanes of a row.) The sum l stays apart by lane until the end.
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
             float mx = -INFINITY;
@@ -132,26 +143,25 @@ __global__ __launch_bounds__(256) void seq_fwd_kernel(const SeqArgs a, const int
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[qb][kt][r]);
-            mx = __builtin_fmaf(seq_group_max(mx), sc, cb);
-            const float mnew = fmaxf(m[qb], mx);
-            const float off = (mnew == -INFINITY) ? 0.f : cb - mnew;
-            float ps = 0.f;
-#pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][kt][r], sc, off));
-                    s[qb][kt][r] = p;
-                    ps += p;
-                }
-            if (!__all(mnew == m[qb])) {
-                const float alpha = __builtin_amdgcn_exp2f(m[qb] - (mnew == -INFINITY ? 0.f : mnew));
+            mx = __builtin_fmaf(mx, sc, cb);
+            if (__any(mx > m[qb] + 8.f)) {
+                const float mnew = fmaxf(m[qb], seq_group_max(mx));
+                const float alpha = mnew == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[qb] - mnew);
 #pragma unroll
                 for (int t2 = 0; t2 < G::DA; ++t2) o[qb][t2] *= alpha;
                 l[qb] *= alpha;
                 m[qb] = mnew;
             }
-            l[qb] += seq_group_sum(ps);
+        }
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            const float off = m[qb] == -INFINITY ? 0.f : cb - m[qb];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[qb][kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][kt][r], sc, off));
+                l[qb] += (s[qb][kt][0] + s[qb][kt][1]) + (s[qb][kt][2] + s[qb][kt][3]);
+            }
         }
         seq_tmul<T, DT, QB>(o, Vs, s, l15, g);
         if constexpr (PREC) {
@@ -167,6 +177,7 @@ __global__ __launch_bounds__(256) void seq_fwd_kernel(const SeqArgs a, const int
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
         const int row = q0 + 16 * qb + l15;
+        l[qb] = seq_group_sum(l[qb]);
         if (row >= a.Nq) continue;
         const long ri = (long)bh * a.Nq + row;
         if (row >= qlen) l[qb] = 0.f;            // a row behind the sample's last query sees nothing
@@ -220,17 +231,6 @@ __global__ __launch_bounds__(256) void seq_combine_kernel(const SeqArgs a) {
 }
 
 // ---------------------------------------------------------------- host side
-SeqPlan seq_fwd_plan(const SeqArgs& a) {
-    SeqPlan p;
-    p.qb = 1;
-    p.nsplit = 1;
-    if (p.nsplit > 1) {
-        p.part = (size_t)p.nsplit * a.B * a.H * a.Nq * a.d * 4;
-        p.ml = (size_t)p.nsplit * a.B * a.H * a.Nq * 2 * 4;
-    }
-    p.total = p.part + p.ml;
-    return p;
-}
 template <typename T, int DT, int QB, bool BIAS, bool PREC>
 static void fwd_go(const Launch& L, const SeqArgs& a) {
     using G = SeqGeo<T, DT>;
@@ -242,13 +242,48 @@ static void fwd_go(const Launch& L, const SeqArgs& a) {
     hipLaunchKernelGGL((seq_fwd_kernel<T, DT, QB, BIAS, PREC>), dim3((unsigned)nqb * a.B * a.H, a.nsplit), dim3(256), lds, L.stream, a, nqb);
     CB_HIP(hipGetLastError());
 }
+template <typename T, int DT, int QB>
+static void fwd_kind(const Launch& L, const SeqArgs& a) {
+    if constexpr (sizeof(T) == 2) {
+        if (a.o32 && a.table) { fwd_go<T, DT, QB, true, true>(L, a); return; }
+    }
+    if (a.table) fwd_go<T, DT, QB, true, false>(L, a);
+    else fwd_go<T, DT, QB, false, false>(L, a);
+}
+// query blocks of 16 a wave that the registers hold without spilling
+static int fwd_max_qb(const SeqArgs& a) {
+    const bool bf = a.dt == DT_BF16, prec = bf && a.o32 && a.table;
+    return a.d <= 64 ? (bf && !prec ? 4 : 2) : a.d <= 80 ? (bf ? 2 : 1) : a.d <= 128 ? (bf && !prec ? 2 : 1) : 1;
+}
 template <typename T, int DT>
 static void fwd_pick(const Launch& L, const SeqArgs& a, int qb) {
-    if constexpr (sizeof(T) == 2) {
-        if (a.o32) { fwd_go<T, DT, 1, true, true>(L, a); return; }
+    constexpr bool BF = sizeof(T) == 2;
+    if constexpr (BF && DT <= 4) {
+        if (qb == 4) {
+            if (a.table) fwd_go<T, DT, 4, true, false>(L, a); else fwd_go<T, DT, 4, false, false>(L, a);
+            return;
+        }
     }
-    if (a.table) fwd_go<T, DT, 1, true, false>(L, a);
-    else fwd_go<T, DT, 1, false, false>(L, a);
+    if constexpr (DT <= 4 || (BF && DT == 5)) { if (qb >= 2) { fwd_kind<T, DT, 2>(L, a); return; } }
+    if constexpr (BF && DT == 8) {
+        if (qb >= 2) {
+            if (a.table) fwd_go<T, DT, 2, true, false>(L, a); else fwd_go<T, DT, 2, false, false>(L, a);
+            return;
+        }
+    }
+    fwd_kind<T, DT, 1>(L, a);
+}
+SeqPlan seq_fwd_plan(const SeqArgs& a) {
+    SeqPlan p;
+    static const int fq = getenv("FQ") ? atoi(getenv("FQ")) : 1;
+    p.qb = std::min(fq, fwd_max_qb(a));
+    p.nsplit = 1;
+    if (p.nsplit > 1) {
+        p.part = (size_t)p.nsplit * a.B * a.H * a.Nq * a.d * 4;
+        p.ml = (size_t)p.nsplit * a.B * a.H * a.Nq * 2 * 4;
+    }
+    p.total = p.part + p.ml;
+    return p;
 }
 void seq_forward(const Launch& L, SeqArgs a, void* ws) {
     const SeqPlan p = seq_fwd_plan(a);

@@ -211,9 +211,9 @@ typedef struct {
     const uint8_t* kv_mask; int64_t mask_stride;                             /* [B][Nk], stride of a sample, or NULL */
     const cb_relpos* relpos; const float* table;                             /* [num_buckets][heads] float32; both or neither */
     float* lse;                                  /* [B][heads][Nq] natural log; out of fwd (or NULL), into bwd */
-    float* out32;                                /* [B][Nq][heads][d] float32 or NULL; bf16 with a table only (ignored otherwise): the output before its
-                                                    rounding, out of fwd into bwd. dtable needs its precision: without it the row sums dout.out,
-                                                    and dtable with them, carry bf16's rounding of `out` */
+    float* out32;                                /* [B][Nq][heads][d] float32 or NULL; bf16 with Nk > 128 only (ignored otherwise): the output before its
+                                                    rounding, out of fwd into bwd, for the row sums dout.out. Without it they, and dtable with
+                                                    them, carry bf16's rounding of `out`; for shorter key axes bwd makes them from the probabilities */
     cb_seq_tensor dout, dq, dk, dv;              /* backward: gradients are written, not accumulated */
     float* dtable;                               /* [num_buckets][heads] or NULL */
     void* workspace; int64_t workspace_bytes;    /* 16-byte aligned, at least cb_seq_attention_workspace() */
