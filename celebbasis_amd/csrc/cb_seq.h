@@ -4,9 +4,9 @@
 //   visible(i, j) = i < q_len[b]  and  j < kv_len[b]  and  mask[b][j]  and  (not causal or j <= q_pos[b] + i)
 //   s_ij = scale * q_i . k_j + table[bucket(j - q_pos[b] - i)][h] ;  o_i = sum_j softmax_j(s_ij) v_j  over the visible keys (none: o_i = 0)
 //
-// One code for fp32 and bf16. A fragment is 8 consecutive elements of a row (lane (l15, g) of a wave: row l15, elements 8g .. 8g+7 of a
-// 32-wide group of the head dim): one v_mfma_f32_16x16x32_bf16, or eight v_mfma_f32_16x16x4_f32 whose k index is g and whose i-th call takes
-// element i — a permutation of the sum over the head dim that both operands share. The accumulator of X Y^T (lane: row 4g + r of X, row l15 of
+// One code for fp32 and bf16. A fragment is 16 bytes of a row (lane (l15, g) of a wave: row l15, piece g of a group of four). bf16: 32 elements
+// of the head dim a group, one v_mfma_f32_16x16x32_bf16. fp32: 16 elements a group, four v_mfma_f32_16x16x4_f32 whose k index is g and whose
+// i-th call takes element i of the piece — a permutation of the sum over the head dim that both operands share. The accumulator of X Y^T (lane: row 4g + r of X, row l15 of
 // Y) is, packed, the second operand of the following product without any movement between lanes.
 #pragma once
 #include "cb_device.h"
@@ -31,7 +31,8 @@ struct SeqArgs {
     float* dvec = nullptr;                                                    // [B][H][Nq]: rowsum(dO * O)
     float* dtable = nullptr;                                                  // [nb][H]
     float* tpart = nullptr;                                                   // [B][H][blocks of queries][nb]
-    float* part = nullptr; float* ml = nullptr; int nsplit = 1;               // partial results of a split axis (fp32)
+    float* part = nullptr; float* ml = nullptr; int nsplit = 1;               // partial results of a split axis (fp32): keys (forward), queries (dK, dV)
+    float* partq = nullptr; int ksplit = 1;                                    // ... keys (dQ)
 };
 
 struct SeqPlan { int qb = 1, nsplit = 1; size_t part = 0, ml = 0, total = 0; };           // sizes in bytes
@@ -55,6 +56,8 @@ typedef __attribute__((address_space(3))) s16x4* lds_s4;
 constexpr float SEQ_L2E = 1.4426950408889634f, SEQ_LN2 = 0.6931471805599453f;
 constexpr int SEQ_OOB = -16;                       // 0xFFFFFFF0 >= num_records: the load returns zeros
 template <int TK> constexpr unsigned long long SEQ_ALL = TK == 64 ? ~0ull : 0xFFFFFFFFull;      // every row of a tile is visible
+// at the head of a rarely taken, wave-uniform branch: keeps its work on x inside (the compiler would turn it into selects that every tile executes)
+__device__ __forceinline__ void seq_pin(f32x4& x) { asm volatile("" : "+v"(x)); }
 constexpr int SEQ_POS_LIM = 1 << 29;               // positions are held to +-2^29, so that differences stay inside an int
 
 __device__ __forceinline__ float seq_group_max(float v) { v = fmaxf(v, __shfl_xor(v, 16, 64)); return fmaxf(v, __shfl_xor(v, 32, 64)); }
@@ -65,13 +68,13 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t seq_srd(const void* p) {
 
 template <typename T> struct SeqFrag;
 template <> struct SeqFrag<bf16_t> { bf16x8_t v; };
-template <> struct SeqFrag<float> { f32x4 v[2]; };
+template <> struct SeqFrag<float> { f32x4 v; };
 __device__ __forceinline__ f32x4 seq_mma(const SeqFrag<bf16_t>& a, const SeqFrag<bf16_t>& b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x4 seq_mma(const SeqFrag<float>& a, const SeqFrag<float>& b, f32x4 c) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i >> 2][i & 3], b.v[i >> 2][i & 3], c, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
     return c;
 }
 
@@ -79,12 +82,12 @@ __device__ __forceinline__ f32x4 seq_mma(const SeqFrag<float>& a, const SeqFrag<
 // 256 pieces; piece c of row r lies at place swz(c, r), which puts the 16 rows that a fragment read touches into 16 different bank groups.
 template <typename T, int DT> struct SeqGeo {
     static constexpr int ES = sizeof(T), EP = 16 / ES;                        // elements of a piece
-    static constexpr int KS = (DT + 1) / 2;                                   // 32-wide groups of the head dim
-    static constexpr int P = KS * 32 / EP;
-    static constexpr int TK = (ES == 4 && DT >= 8) ? 32 : 64;
+    static constexpr int KS = ES == 4 ? DT : (DT + 1) / 2;                    // groups of four pieces of a row
+    static constexpr int P = 4 * KS;
+    static constexpr int TK = (ES == 4 && DT >= 3) ? 32 : 64;                 // fp32: 64 rows would leave one block a CU
     static constexpr int KT = TK / 16;
-    static constexpr int TILE = TK * P * 16, NS = TILE / 4096;
-    static constexpr int DA = ES == 4 ? 2 * KS : DT;                          // 16-wide accumulator tiles across the head dim
+    static constexpr int TILE = TK * P * 16, NS = (TILE + 4095) / 4096, IMG = NS * 4096;     // an image takes whole slots
+    static constexpr int DA = DT;                                             // 16-wide accumulator tiles across the head dim
     static __device__ __forceinline__ int swz(int c, int r) {
         if constexpr (P % 16 == 0) return c ^ (r & 15);
         else if constexpr (P % 8 == 0) return c ^ ((r >> 1) & 7);
@@ -101,7 +104,7 @@ template <typename T, int DT> struct SeqSlots {
 #pragma unroll
         for (int i = 0; i < G::NS; ++i) {
             const int idx = tid + 256 * i, r = idx / G::P, c = G::swz(idx - r * G::P, r);
-            off[i] = (c * G::EP < d) ? (int)((long)r * ld * G::ES + c * 16) : SEQ_OOB;
+            off[i] = (r < G::TK && c * G::EP < d) ? (int)((long)r * ld * G::ES + c * 16) : SEQ_OOB;
         }
     }
     // dst: the tile's image + this wave's 1 KiB piece of a slot
@@ -114,40 +117,28 @@ template <typename T, int DT> struct SeqSlots {
 #pragma unroll
             for (int i = 0; i < G::NS; ++i) {
                 const int r = (tid + 256 * i) / G::P;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_vp)(dst + i * 4096), 16, ((live >> r) & 1ull) ? off[i] : SEQ_OOB, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_vp)(dst + i * 4096), 16, ((live >> (r & 63)) & 1ull) ? off[i] : SEQ_OOB, 0, 0, 0);
             }
         }
     }
 };
 
-// fragment of rows 16 blk + l15, 32-wide group s of the head dim
+// fragment of rows 16 blk + l15, group s of the head dim
 template <typename T, int DT>
 __device__ __forceinline__ SeqFrag<T> seq_frag_lds(const char* img, int blk, int s, int l15, int g) {
     using G = SeqGeo<T, DT>;
-    const int r = blk * 16 + l15;
     SeqFrag<T> f;
-    if constexpr (G::ES == 2) {
-        f.v = *reinterpret_cast<const bf16x8_t*>(img + (r * G::P + G::swz(4 * s + g, l15)) * 16);
-    } else {
-        f.v[0] = *reinterpret_cast<const f32x4*>(img + (r * G::P + G::swz(8 * s + 2 * g, l15)) * 16);
-        f.v[1] = *reinterpret_cast<const f32x4*>(img + (r * G::P + G::swz(8 * s + 2 * g + 1, l15)) * 16);
-    }
+    f.v = *reinterpret_cast<const decltype(f.v)*>(img + ((blk * 16 + l15) * G::P + G::swz(4 * s + g, l15)) * 16);
     return f;
 }
 // the same of a row in global memory, zeros where the row is not valid
 template <typename T>
 __device__ __forceinline__ SeqFrag<T> seq_frag_row(const T* row, bool valid, int s, int g, int d) {
     SeqFrag<T> f;
-    const int c = 32 * s + 8 * g;
-    const bool ok = valid && c < d;
-    if constexpr (sizeof(T) == 2) {
-        u32x4s v = {0u, 0u, 0u, 0u};
-        if (ok) v = *reinterpret_cast<const u32x4s*>(row + c);
-        f.v = __builtin_bit_cast(bf16x8_t, v);
-    } else {
-        f.v[0] = (f32x4){0.f, 0.f, 0.f, 0.f}; f.v[1] = f.v[0];
-        if (ok) { f.v[0] = *reinterpret_cast<const f32x4*>(row + c); f.v[1] = *reinterpret_cast<const f32x4*>(row + c + 4); }
-    }
+    const int c = (4 * s + g) * (16 / (int)sizeof(T));
+    u32x4s v = {0u, 0u, 0u, 0u};
+    if (valid && c < d) v = *reinterpret_cast<const u32x4s*>(row + c);
+    f.v = __builtin_bit_cast(decltype(f.v), v);
     return f;
 }
 
@@ -155,8 +146,8 @@ __device__ __forceinline__ SeqFrag<T> seq_frag_row(const T* row, bool valid, int
 // same tile (lane: tile rows 16 kt + 4g + r, column l15).
 //   bf16: the A operand (head-dim index l15, k slot 8g + j <-> row 32G + 4g + j, or 32G + 16 + 4g + j - 4) comes from two transposing LDS reads
 //         (a 16-lane group reads four rows of 16 elements and gets their columns).
-//   fp32: one 8-byte read of row 16 kt + 4g + r at columns 32 tt + 2 l15, + 1 feeds two calls; accumulator (tt, e) then holds column
-//         32 tt + 2 (4g + r) + e, so that a lane owns the 8 consecutive columns 32 tt + 8g .. + 7.
+//   fp32: one 8-byte read of row 16 kt + 4g + r at columns 32 tt + 2 l15, + 1 feeds two calls; accumulator 2 tt + e then holds column
+//         32 tt + 2 (4g + r) + e, so that a lane owns the 8 consecutive columns 32 tt + 8g .. + 7. An odd last tile is read by itself.
 template <typename T, int DT, int QB> using SeqAcc = f32x4[QB][SeqGeo<T, DT>::DA];
 template <typename T, int DT, int QB> using SeqScores = f32x4[QB][SeqGeo<T, DT>::KT];
 template <typename T, int DT> using SeqRow = f32x4[SeqGeo<T, DT>::DA];
@@ -193,7 +184,7 @@ __device__ __forceinline__ void seq_tmul(SeqAcc<T, DT, QB>& acc, const char* img
             for (int r = 0; r < 4; ++r) {
                 const int row = kt * 16 + 4 * g + r;
 #pragma unroll
-                for (int tt = 0; tt < G::KS; ++tt) {
+                for (int tt = 0; tt < DT / 2; ++tt) {
                     const int c = 8 * tt + (l15 >> 1);
                     const f32x2 v = *reinterpret_cast<const f32x2*>(img + (row * G::P + G::swz(c, row)) * 16 + (l15 & 1) * 8);
 #pragma unroll
@@ -202,6 +193,12 @@ __device__ __forceinline__ void seq_tmul(SeqAcc<T, DT, QB>& acc, const char* img
                         acc[qb][2 * tt + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[1], w[qb][kt][r], acc[qb][2 * tt + 1], 0, 0, 0);
                     }
                 }
+                if constexpr (DT % 2) {
+                    const int c = 4 * (DT - 1) + (l15 >> 2);
+                    const float v = *reinterpret_cast<const float*>(img + (row * G::P + G::swz(c, row)) * 16 + (l15 & 3) * 4);
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb) acc[qb][DT - 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, w[qb][kt][r], acc[qb][DT - 1], 0, 0, 0);
+                }
             }
     }
 }
@@ -209,19 +206,17 @@ __device__ __forceinline__ void seq_tmul(SeqAcc<T, DT, QB>& acc, const char* img
 template <typename T, int DT, typename F>
 __device__ __forceinline__ void seq_row4(const SeqRow<T, DT>& acc, int d, int g, F f) {
     using G = SeqGeo<T, DT>;
-    if constexpr (G::ES == 2) {
+    constexpr int PAIRS = G::ES == 2 ? 0 : DT / 2;
 #pragma unroll
-        for (int t = 0; t < G::DA; ++t) {
-            const int c = 16 * t + 4 * g;
-            if (c < d) f(c, make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]));
-        }
-    } else {
+    for (int tt = 0; tt < PAIRS; ++tt) {
+        const int c = 32 * tt + 8 * g;
+        const f32x4 e = acc[2 * tt], o = acc[2 * tt + 1];
+        if (c < d) { f(c, make_float4(e[0], o[0], e[1], o[1])); f(c + 4, make_float4(e[2], o[2], e[3], o[3])); }
+    }
 #pragma unroll
-        for (int tt = 0; tt < G::KS; ++tt) {
-            const int c = 32 * tt + 8 * g;
-            const f32x4 e = acc[2 * tt], o = acc[2 * tt + 1];
-            if (c < d) { f(c, make_float4(e[0], o[0], e[1], o[1])); f(c + 4, make_float4(e[2], o[2], e[3], o[3])); }
-        }
+    for (int t = 2 * PAIRS; t < G::DA; ++t) {
+        const int c = 16 * t + 4 * g;
+        if (c < d) f(c, make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]));
     }
 }
 

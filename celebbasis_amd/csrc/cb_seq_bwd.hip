@@ -20,7 +20,7 @@ template <typename T, int DT, int QB, bool BIAS, bool TAB> struct SeqDq {
     static constexpr int SKEW = TAB ? 4 * 16 * SP * 4 : 0;
     static int lds(int D) {
         const int w = 2 * (D + PAD) + 1;
-        return 4 * G::TILE + (BIAS ? (int)rup(w * 4, 16) : 0) + SKEW + (TAB ? 4 * w * 4 : 0);
+        return 4 * G::IMG + (BIAS ? (int)rup(w * 4, 16) : 0) + SKEW + (TAB ? 4 * w * 4 : 0);
     }
 };
 
@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
     using S = SeqDq<T, DT, QB, BIAS, TAB>;
-    constexpr int TK = G::TK, KT = G::KT, KS = G::KS, STAGE = 2 * G::TILE, PAD = S::PAD, NE = S::NE, SP = S::SP;
+    constexpr int TK = G::TK, KT = G::KT, KS = G::KS, STAGE = 2 * G::IMG, PAD = S::PAD, NE = S::NE, SP = S::SP;
     extern __shared__ __attribute__((aligned(16))) char lds_seq[];
     const int W = 2 * (a.D + PAD) + 1;
     float* bw = reinterpret_cast<float*>(lds_seq + 2 * STAGE);
@@ -50,8 +50,13 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
     int kend = klen;
     if (a.causal) kend = max(0, min(kend, pos0 + min(qb0 + 64 * QB, qlen)));
     if (qb0 >= qlen) kend = 0;
-    const int t1 = (kend + TK - 1) / TK;
     const bool brief = a.Nk <= SEQ_SHORT;
+    const int split = blockIdx.y;                                 // part of the key axis (never where `brief`)
+    int t0 = 0, t1 = (kend + TK - 1) / TK;
+    if (a.ksplit > 1) {
+        const int per = (t1 + a.ksplit - 1) / a.ksplit;
+        t0 = min(split * per, t1); t1 = min(t0 + per, t1);
+    }
 
     SeqFrag<T> qf[QB][KS], df[QB][KS];
     float lse2[QB], dsum[QB];
@@ -76,9 +81,10 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = (float)df[qb][s].v[e];
                 if (O32) {
-                    const SeqFrag<float> f = seq_frag_row<float>(O32, valid, s, g, a.d);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = f.v[e >> 2][e & 3];
+                    const int c = 32 * s + 8 * g;
+                    const bool in = valid && c < a.d;
+                    const float4 y0 = in ? ld4(O32 + c) : make_float4(0.f, 0.f, 0.f, 0.f), y1 = in ? ld4(O32 + c + 4) : y0;
+                    y[0] = y0.x; y[1] = y0.y; y[2] = y0.z; y[3] = y0.w; y[4] = y1.x; y[5] = y1.y; y[6] = y1.z; y[7] = y1.w;
                 } else {
                     const SeqFrag<T> f = seq_frag_row<T>(O, valid, s, g, a.d);
 #pragma unroll
@@ -87,13 +93,13 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
             } else {
                 const SeqFrag<T> f = seq_frag_row<T>(O, valid, s, g, a.d);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { x[e] = df[qb][s].v[e >> 2][e & 3]; y[e] = f.v[e >> 2][e & 3]; }
+                for (int e = 0; e < 4; ++e) { x[e] = df[qb][s].v[e]; y[e] = f.v[e]; }
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ds = __builtin_fmaf(x[e], y[e], ds);
+            for (int e = 0; e < G::EP; ++e) ds = __builtin_fmaf(x[e], y[e], ds);
         }
         dsum[qb] = brief ? 0.f : seq_group_sum(ds);
-        if (g == 0 && row < a.Nq) a.dvec[ri] = dsum[qb];          // (a row without a visible key: 0 either way)
+        if (g == 0 && row < a.Nq && split == 0) a.dvec[ri] = dsum[qb];          // (a row without a visible key: 0 either way)
     }
     const float scale2 = a.scale * SEQ_L2E;
     f32x4 acc[QB][G::DA];
@@ -116,19 +122,19 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
     auto stage = [&](int u, int t, unsigned long long live) {
         char* dst = lds_seq + (u & 1) * STAGE + wbase;
         sk.dma(K + (long)t * TK * a.k.row, dst, live, tid);
-        sv.dma(V + (long)t * TK * a.v.row, dst + G::TILE, live, tid);
+        sv.dma(V + (long)t * TK * a.v.row, dst + G::IMG, live, tid);
     };
     unsigned long long live = 0, next = 0;
-    const int u1 = brief ? 2 * t1 : t1;                           // steps: the tiles, twice where the first pass makes the row sums
-    if (0 < t1) { next = seq_live<TK>(mask, 0, klen, lane); stage(0, 0, next); }
+    const int n1 = t1 - t0, u1 = brief ? 2 * n1 : n1;             // steps: the tiles, twice where the first pass makes the row sums
+    if (0 < n1) { next = seq_live<TK>(mask, t0 * TK, klen, lane); stage(0, t0, next); }
     for (int u = 0; u < u1; ++u) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         live = next;
-        const int t = u < t1 ? u : u - t1;
-        if (u + 1 < u1) { const int n = u + 1 < t1 ? u + 1 : u + 1 - t1; next = seq_live<TK>(mask, n * TK, klen, lane); stage(u + 1, n, next); }
-        if (brief && u == t1) {
+        const int t = t0 + (u < n1 ? u : u - n1);
+        if (u + 1 < u1) { const int n = t0 + (u + 1 < n1 ? u + 1 : u + 1 - n1); next = seq_live<TK>(mask, n * TK, klen, lane); stage(u + 1, n, next); }
+        if (brief && u == n1) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
                 dsum[qb] = seq_group_sum(dsum[qb]);
@@ -138,7 +144,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
         }
         if (live == 0) continue;
         const char* Ks = lds_seq + (u & 1) * STAGE;
-        const char* Vs = Ks + G::TILE;
+        const char* Vs = Ks + G::IMG;
         const int k0 = t * TK, p0 = pos0 + q0;
         f32x4 s[QB][KT], dp[QB][KT];
 #pragma unroll
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
                         for (int r = 0; r < 4; ++r) s[qb][kt][r] = __builtin_fmaf(s[qb][kt][r], scale2, w[16 * kt + r - 16 * qb]);
             }
         }
-        const bool sums = brief && u < t1;
+        const bool sums = brief && u < n1;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
             const float off = cb - lse2[qb], ds = sums ? 0.f : dsum[qb];
@@ -190,6 +196,8 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
         if (live != SEQ_ALL<TK>) {
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) seq_pin(s[qb][kt]);
                 const int nib = (int)(unsigned)(live >> (16 * kt + 4 * g));
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -203,9 +211,11 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                for (int kt = 0; kt < KT; ++kt) {
+                    seq_pin(s[qb][kt]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[qb][kt][r] = k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15 ? s[qb][kt][r] : 0.f;
+                }
         }
         if (sums) {
 #pragma unroll
@@ -251,6 +261,11 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
     for (int qb = 0; qb < QB; ++qb) {
         const int row = q0 + 16 * qb + l15;
         if (row >= a.Nq) continue;
+        if (a.ksplit > 1) {
+            float* P = a.partq + (((long)split * a.B * a.H + bh) * a.Nq + row) * a.d;
+            seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(P + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
+            continue;
+        }
         T* dQ = static_cast<T*>(a.dq.p) + b * a.dq.batch + h * a.dq.head + (long)row * a.dq.row;
         seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(dQ + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
     }
@@ -262,7 +277,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
         __syncthreads();
         for (int i = tid; i < W; i += 256) hist[i] = (hist[i] + hist[W + i]) + (hist[2 * W + i] + hist[3 * W + i]);
         __syncthreads();
-        float* out = a.tpart + ((long)bh * nqb + qblk) * a.nb;
+        float* out = a.tpart + (((long)bh * a.ksplit + split) * nqb + qblk) * a.nb;
         for (int c = wave; c < a.nb; c += 4) {
             const int lo = a.brange[2 * c], hi = a.brange[2 * c + 1];           // distances + D of the bucket, [lo, hi)
             float x = 0.f;
@@ -294,14 +309,14 @@ __global__ __launch_bounds__(64) void seq_dtable_kernel(const SeqArgs a, const i
 template <typename T, int DT, int KB, bool BIAS> struct SeqDkv {
     using G = SeqGeo<T, DT>;
     static constexpr int PAD = G::TK + 16 * KB;
-    static int lds(int D) { return 4 * G::TILE + 4 * G::TK * 4 + (BIAS ? (int)rup((2 * (D + PAD) + 1) * 4, 16) : 0); }
+    static int lds(int D) { return 4 * G::IMG + 4 * G::TK * 4 + (BIAS ? (int)rup((2 * (D + PAD) + 1) * 4, 16) : 0); }
 };
 
 template <typename T, int DT, int KB, bool BIAS>
 __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqArgs a, const int nkb) {
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
-    constexpr int TQ = G::TK, QT = G::KT, KS = G::KS, STAGE = 2 * G::TILE, PAD = SeqDkv<T, DT, KB, BIAS>::PAD;
+    constexpr int TQ = G::TK, QT = G::KT, KS = G::KS, STAGE = 2 * G::IMG, PAD = SeqDkv<T, DT, KB, BIAS>::PAD;
     extern __shared__ __attribute__((aligned(16))) char lds_seq[];
     float* rows = reinterpret_cast<float*>(lds_seq + 2 * STAGE);      // [2 stages][lse, D][TQ]
     float* bw = rows + 4 * TQ;
@@ -364,7 +379,7 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
         char* dst = lds_seq + (u & 1) * STAGE + wbase;
         const unsigned long long live = seq_live<TQ>(nullptr, r0, qlen, lane);
         sq.dma(static_cast<const T*>(a.q.p) + b * a.q.batch + h * a.q.head + (long)r0 * a.q.row, dst, live, tid);
-        sd.dma(static_cast<const T*>(a.dout.p) + b * a.dout.batch + h * a.dout.head + (long)r0 * a.dout.row, dst + G::TILE, live, tid);
+        sd.dma(static_cast<const T*>(a.dout.p) + b * a.dout.batch + h * a.dout.head + (long)r0 * a.dout.row, dst + G::IMG, live, tid);
     };
     auto put = [&](int u) {
         if (tid < TQ) { float* w = rows + (u & 1) * 2 * TQ; w[tid] = ls; w[TQ + tid] = dd; }
@@ -379,7 +394,7 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
         if (BIAS && h != hcur) { seq_bias_fill(bw, a, h, PAD, tid); hcur = h; __syncthreads(); }
         if (u + 1 < u1) { fetch(u + 1); stage(u + 1); }
         const char* Qs = lds_seq + (u & 1) * STAGE;
-        const char* Ds = Qs + G::TILE;
+        const char* Ds = Qs + G::IMG;
         const float* rw = rows + (u & 1) * 2 * TQ;
         const int q0 = (tq0 + u % n1) * TQ, p0 = pos0 + q0;
         f32x4 s[KB][QT], dp[KB][QT];
@@ -423,10 +438,20 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][qt][r], sc, cb - lq[r]));
-                    if (!full) p = (k0 + 16 * kb + l15 <= p0 + 16 * qt + 4 * g + r) ? p : 0.f;
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][qt][r], sc, cb - lq[r]));
                     s[kb][qt][r] = p;
                     dp[kb][qt][r] = p * (dp[kb][qt][r] - dq[r]);
+                }
+        }
+        if (!full) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    seq_pin(s[kb][qt]); seq_pin(dp[kb][qt]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (k0 + 16 * kb + l15 > p0 + 16 * qt + 4 * g + r) { s[kb][qt][r] = 0.f; dp[kb][qt][r] = 0.f; }
                 }
         }
         seq_tmul<T, DT, KB>(dv, Ds, s, l15, g);
@@ -455,37 +480,49 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
 #endif
 }
 
-// dk, dv = sum of the parts of a split query axis, in order; one thread per 4 columns
+// gradients from the parts of a split axis, in order: dK and dV ([nsplit][2][B][Hkv][Nk][d]) or dQ ([ksplit][B][H][Nq][d]); one thread per 4 columns
 template <typename T>
-__global__ __launch_bounds__(256) void seq_dkv_sum_kernel(const SeqArgs a) {
-    const int d4 = a.d >> 2;
-    const long n = (long)a.B * a.Hkv * a.Nk, i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= 2 * n * d4) return;
+__global__ __launch_bounds__(256) void seq_sum_kernel(const float* __restrict__ part, const SeqT d0, const SeqT d1, const int nsplit, const int two, const int B, const int H,
+                                                      const int N, const int d) {
+    const int d4 = d >> 2;
+    const long n = (long)B * H * N, rows = two ? 2 * n : n, i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * d4) return;
     const long rr = i / d4;
     const int c = (int)(i - rr * d4) * 4;
-    const bool isv = rr >= n;
-    const long ri = isv ? rr - n : rr;
+    const bool second = rr >= n;
+    const long ri = second ? rr - n : rr;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float4 v = ld4(a.part + ((long)s * 2 * n + rr) * a.d + c);
+    for (int s = 0; s < nsplit; ++s) {
+        const float4 v = ld4(part + (s * rows + rr) * d + c);
         x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
     }
-    const long bk = ri / a.Nk, key = ri - bk * a.Nk, b = bk / a.Hkv, hk = bk - b * a.Hkv;
-    const SeqT& t = isv ? a.dv : a.dk;
-    st4(static_cast<T*>(t.p) + b * t.batch + hk * t.head + key * t.row + c, x);
+    const long bh = ri / N, row = ri - bh * N, b = bh / H, h = bh - b * H;
+    const SeqT& t = second ? d1 : d0;
+    st4(static_cast<T*>(t.p) + b * t.batch + h * t.head + row * t.row + c, x);
 }
 
 // ---------------------------------------------------------------- host side
 SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable) {
     SeqBwdPlan p;
-    static const int fq = getenv("DQ") ? atoi(getenv("DQ")) : 1, fk = getenv("DK") ? atoi(getenv("DK")) : 1, fs = getenv("DS") ? atoi(getenv("DS")) : 1;
-    const bool wide = a.dt == DT_BF16 && a.d <= 64;
-    p.qb = wide ? fq : 1; p.kb = wide ? fk : 1; p.qsplit = fs;
+    const bool wide = a.dt == DT_BF16 && a.d <= 64;                  // what the registers hold for 32 rows a wave
+    const long bh = (long)a.B * a.H, bk = (long)a.B * a.Hkv;
+    // measured, 16 against 32 rows a wave. dQ: 8 x 12 heads, 512 x 512 with dtable 45.6 / 39.3 us, 2 x 12 heads, 4096 causal 183 / 148 us; two passes
+    // over 77 keys 38.8 / 41.7 us. dK, dV: 384 blocks of 128 keys (8 x 12 heads, 512) 27.7 / 30.0 us, 768 (2 x 12 heads, 4096) 162 / 154 us
+    p.qb = wide && a.Nk > SEQ_SHORT ? 2 : 1;
+    p.kb = wide && bk * cdiv(a.Nk, 128) >= 768 ? 2 : 1;
     p.nqb = (int)cdiv(a.Nq, 64 * p.qb);
+    // few blocks of keys (or queries): the other axis is split into runs of at least 4 tiles. 128 blocks (64 heads, 4096 x 77, d 40): 102 us whole,
+    // 26 + 5 us in 8 parts
+    const long fill = a.dt == DT_BF16 ? 1024 : 512;
+    const long kblocks = bk * cdiv(a.Nk, 64 * p.kb), steps = (long)a.G * cdiv(a.Nq, 64);
+    p.qsplit = kblocks < 384 && steps >= 8 ? (int)std::min<long>(fill / std::max(kblocks, 1l), steps / 4) : 1;
+    const long qblocks = bh * p.nqb, tiles = cdiv(a.Nk, 64);
+    p.ksplit = qblocks < 256 && tiles >= 8 && a.Nk > SEQ_SHORT ? (int)std::min<long>(cdiv(512, std::max(qblocks, 1l)), tiles / 4) : 1;
     p.dvec = (size_t)rup((long)a.B * a.H * a.Nq * 4, 256);
-    p.tpart = want_dtable ? (size_t)rup((long)a.B * a.H * p.nqb * a.nb * 4, 256) : 0;
-    p.part = p.qsplit > 1 ? (size_t)p.qsplit * 2 * a.B * a.Hkv * a.Nk * a.d * 4 : 0;
-    p.total = p.dvec + p.tpart + p.part;
+    p.tpart = want_dtable ? (size_t)rup((long)a.B * a.H * p.ksplit * p.nqb * a.nb * 4, 256) : 0;
+    p.part = p.qsplit > 1 ? (size_t)rup((long)p.qsplit * 2 * a.B * a.Hkv * a.Nk * a.d * 4, 256) : 0;
+    p.partq = p.ksplit > 1 ? (size_t)p.ksplit * a.B * a.H * a.Nq * a.d * 4 : 0;
+    p.total = p.dvec + p.tpart + p.part + p.partq;
     return p;
 }
 template <typename T, int DT, int QB, bool BIAS, bool TAB>
@@ -495,7 +532,7 @@ static void dq_go(const Launch& L, const SeqArgs& a, int nqb) {
     if (L.dry) return;
     const int lds = SeqDq<T, DT, QB, BIAS, TAB>::lds(a.D);
     set_dyn_lds(reinterpret_cast<const void*>(&seq_dq_kernel<T, DT, QB, BIAS, TAB>), 160 * 1024);
-    hipLaunchKernelGGL((seq_dq_kernel<T, DT, QB, BIAS, TAB>), dim3((unsigned)nqb * a.B * a.H), dim3(256), lds, L.stream, a, nqb);
+    hipLaunchKernelGGL((seq_dq_kernel<T, DT, QB, BIAS, TAB>), dim3((unsigned)nqb * a.B * a.H, a.ksplit), dim3(256), lds, L.stream, a, nqb);
     CB_HIP(hipGetLastError());
 }
 template <typename T, int DT, int KB, bool BIAS>
@@ -530,27 +567,33 @@ static void bwd_pick(const Launch& L, const SeqArgs& a, const SeqBwdPlan& p) {
         dkv_kind<T, DT, 1>(L, a);
     }
 }
+static void sum_parts(const Launch& L, DType dt, const float* part, const SeqT& d0, const SeqT& d1, int nsplit, int two, int B, int H, int N, int d) {
+    const long n = (long)(two ? 2 : 1) * B * H * N * (d / 4);
+    if (!n) return;
+    L.count();
+    if (L.dry) return;
+    CB_DT_SWITCH(dt, T, hipLaunchKernelGGL((seq_sum_kernel<T>), dim3(cdiv(n, 256)), dim3(256), 0, L.stream, part, d0, d1, nsplit, two, B, H, N, d));
+    CB_HIP(hipGetLastError());
+}
 void seq_backward(const Launch& L, SeqArgs a, void* ws) {
     const SeqBwdPlan p = seq_bwd_plan(a, a.dtable != nullptr);
     char* w = static_cast<char*>(ws);
     a.dvec = reinterpret_cast<float*>(w); w += p.dvec;
     a.tpart = reinterpret_cast<float*>(w); w += p.tpart;
-    a.part = reinterpret_cast<float*>(w);
+    a.part = reinterpret_cast<float*>(w); w += p.part;
+    a.partq = reinterpret_cast<float*>(w);
     a.nsplit = p.qsplit;
+    a.ksplit = p.ksplit;
     CB_DT_SWITCH(a.dt, T, SEQ_DT_SWITCH(a.d, DT, bwd_pick<T, DT>(L, a, p)));
     if (a.dtable) {
         L.count();
         if (!L.dry) {
-            hipLaunchKernelGGL(seq_dtable_kernel, dim3(a.nb, a.H), dim3(64), 0, L.stream, a, p.nqb);
+            hipLaunchKernelGGL(seq_dtable_kernel, dim3(a.nb, a.H), dim3(64), 0, L.stream, a, p.nqb * a.ksplit);
             CB_HIP(hipGetLastError());
         }
     }
-    if (a.nsplit > 1 && (long)a.B * a.Nk) {
-        L.count();
-        if (L.dry) return;
-        CB_DT_SWITCH(a.dt, T, hipLaunchKernelGGL((seq_dkv_sum_kernel<T>), dim3(cdiv(2L * a.B * a.Hkv * a.Nk * (a.d / 4), 256)), dim3(256), 0, L.stream, a));
-        CB_HIP(hipGetLastError());
-    }
+    if (a.ksplit > 1) sum_parts(L, a.dt, a.partq, a.dq, a.dq, a.ksplit, 0, a.B, a.H, a.Nq, a.d);
+    if (a.nsplit > 1) sum_parts(L, a.dt, a.part, a.dk, a.dv, a.nsplit, 1, a.B, a.Hkv, a.Nk, a.d);
 }
 
 }  // namespace cb

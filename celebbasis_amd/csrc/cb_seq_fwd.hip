@@ -15,7 +15,7 @@ template <typename T, int DT, int QB, bool BIAS, bool PREC>
 __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqArgs a, const int nqb) {
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
-    constexpr int TK = G::TK, KT = G::KT, KS = G::KS, STAGE = 2 * G::TILE, PAD = TK + 16 * QB;
+    constexpr int TK = G::TK, KT = G::KT, KS = G::KS, STAGE = 2 * G::IMG, PAD = TK + 16 * QB;
     extern __shared__ __attribute__((aligned(16))) char lds_seq[];
     float* bw = reinterpret_cast<float*>(lds_seq + 2 * STAGE);
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
     auto stage = [&](int t, unsigned long long live) {
         char* dst = lds_seq + (t & 1) * STAGE + wbase;
         sk.dma(K + (long)t * TK * a.k.row, dst, live, tid);
-        sv.dma(V + (long)t * TK * a.v.row, dst + G::TILE, live, tid);
+        sv.dma(V + (long)t * TK * a.v.row, dst + G::IMG, live, tid);
     };
     unsigned long long live = 0, next = 0;
     if (t0 < t1) { next = seq_live<TK>(mask, t0 * TK, klen, lane); stage(t0, next); }
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
         if (t + 1 < t1) { next = seq_live<TK>(mask, (t + 1) * TK, klen, lane); stage(t + 1, next); }
         if (live == 0) continue;
         const char* Ks = lds_seq + (t & 1) * STAGE;
-        const char* Vs = Ks + G::TILE;
+        const char* Vs = Ks + G::IMG;
         const int k0 = t * TK;
         f32x4 s[QB][KT];
 #pragma unroll
@@ -116,6 +116,8 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
         if (live != SEQ_ALL<TK>) {                   // keys that the length or the mask hides
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) seq_pin(s[qb][kt]);
                 const int nib = (int)~(unsigned)(live >> (16 * kt + 4 * g));
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -129,9 +131,11 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                for (int kt = 0; kt < KT; ++kt) {
+                    seq_pin(s[qb][kt]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[qb][kt][r] = k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15 ? s[qb][kt][r] : -INFINITY;
+                }
         }
         // The exponent's reference m follows the running maximum only where a lane is more than 8 (2^8) above it: p stays below 2^8, which costs
         // nothing in fp32 sums or in bf16's relative rounding, and most tiles need neither the maximum over the lanes of a row nor a rescaling.
@@ -235,49 +239,44 @@ template <typename T, int DT, int QB, bool BIAS, bool PREC>
 static void fwd_go(const Launch& L, const SeqArgs& a) {
     using G = SeqGeo<T, DT>;
     const int nqb = (int)cdiv(a.Nq, 64 * QB);
-    const int lds = 4 * G::TILE + (BIAS ? (int)rup((2 * (a.D + G::TK + 16 * QB) + 1) * 4, 16) : 0);
+    const int lds = 4 * G::IMG + (BIAS ? (int)rup((2 * (a.D + G::TK + 16 * QB) + 1) * 4, 16) : 0);
     L.count();
     if (L.dry) return;
     set_dyn_lds(reinterpret_cast<const void*>(&seq_fwd_kernel<T, DT, QB, BIAS, PREC>), 160 * 1024);
     hipLaunchKernelGGL((seq_fwd_kernel<T, DT, QB, BIAS, PREC>), dim3((unsigned)nqb * a.B * a.H, a.nsplit), dim3(256), lds, L.stream, a, nqb);
     CB_HIP(hipGetLastError());
 }
-template <typename T, int DT, int QB>
+template <typename T, int DT>
 static void fwd_kind(const Launch& L, const SeqArgs& a) {
     if constexpr (sizeof(T) == 2) {
-        if (a.o32 && a.table) { fwd_go<T, DT, QB, true, true>(L, a); return; }
+        if (a.o32 && a.table) { fwd_go<T, DT, 1, true, true>(L, a); return; }
     }
-    if (a.table) fwd_go<T, DT, QB, true, false>(L, a);
-    else fwd_go<T, DT, QB, false, false>(L, a);
+    if (a.table) fwd_go<T, DT, 1, true, false>(L, a);
+    else fwd_go<T, DT, 1, false, false>(L, a);
 }
-// query blocks of 16 a wave that the registers hold without spilling
-static int fwd_max_qb(const SeqArgs& a) {
-    const bool bf = a.dt == DT_BF16, prec = bf && a.o32 && a.table;
-    return a.d <= 64 ? (bf && !prec ? 4 : 2) : a.d <= 80 ? (bf ? 2 : 1) : a.d <= 128 ? (bf && !prec ? 2 : 1) : 1;
-}
+// 32 queries a wave read every K and V fragment for two products instead of one; where the registers do not hold them (two-part probabilities,
+// fp32 or bf16 heads beyond 128) or the grid would not fill the chip, 16
+static bool fwd_two(const SeqArgs& a) { return a.dt == DT_BF16 ? a.d <= 128 && !(a.o32 && a.table) : a.d <= 32; }
 template <typename T, int DT>
 static void fwd_pick(const Launch& L, const SeqArgs& a, int qb) {
-    constexpr bool BF = sizeof(T) == 2;
-    if constexpr (BF && DT <= 4) {
-        if (qb == 4) {
-            if (a.table) fwd_go<T, DT, 4, true, false>(L, a); else fwd_go<T, DT, 4, false, false>(L, a);
-            return;
-        }
-    }
-    if constexpr (DT <= 4 || (BF && DT == 5)) { if (qb >= 2) { fwd_kind<T, DT, 2>(L, a); return; } }
-    if constexpr (BF && DT == 8) {
-        if (qb >= 2) {
+    if constexpr (sizeof(T) == 2 ? DT <= 8 : DT == 2) {
+        if (qb == 2) {
             if (a.table) fwd_go<T, DT, 2, true, false>(L, a); else fwd_go<T, DT, 2, false, false>(L, a);
             return;
         }
     }
-    fwd_kind<T, DT, 1>(L, a);
+    fwd_kind<T, DT>(L, a);
 }
 SeqPlan seq_fwd_plan(const SeqArgs& a) {
     SeqPlan p;
-    static const int fq = getenv("FQ") ? atoi(getenv("FQ")) : 1;
-    p.qb = std::min(fq, fwd_max_qb(a));
-    p.nsplit = 1;
+    const long bh = (long)a.B * a.H;
+    // measured, 16 against 32 queries a wave: 768 / 384 blocks (8 x 12 heads, 512 x 512, d 64) 22.4 / 25.6 us; 2048 blocks (64 heads, 4096 x 77, d 40)
+    // 24.3 / 22.0 us; 512 blocks (64 heads, 1024 x 2000, d 128) 127 / 90 us
+    p.qb = fwd_two(a) && bh * cdiv(a.Nq, 128) >= 512 ? 2 : 1;
+    // fewer blocks than CUs: the key axis is split into runs of at least 4 tiles, joined by seq_combine_kernel
+    const long blocks = bh * cdiv(a.Nq, 64 * p.qb);
+    const int tiles = (int)cdiv(a.Nk, 64);
+    p.nsplit = blocks < 256 && tiles >= 8 ? (int)std::min<long>(cdiv(512, std::max(blocks, 1l)), tiles / 4) : 1;
     if (p.nsplit > 1) {
         p.part = (size_t)p.nsplit * a.B * a.H * a.Nq * a.d * 4;
         p.ml = (size_t)p.nsplit * a.B * a.H * a.Nq * 2 * 4;

@@ -256,6 +256,28 @@ def test_relative_bias_far_distances(cb, dtype):
 
 
 @DT
+@pytest.mark.parametrize("rel", [None, (32, 128, True)])
+def test_split_axes(cb, dtype, rel):
+    """few blocks: the long axis is split over blocks, with parts that hold nothing; and the key counts where the row sums change their source"""
+    check(cb, dtype, 2, 77, 2500, 2, 1, 64, rel=rel, kv_len=[2500, 70])
+    check(cb, dtype, 1, 40, 1100, 2, 2, 40, rel=rel, causal=True, q_pos=[600], kv_len=[900])
+    check(cb, dtype, 2, 2500, 77, 2, 1, 64, rel=rel, kv_len=[77, 0])
+    m = torch.zeros(1, 1300, dtype=torch.bool, device=_dev())
+    m[0, 700:720] = True
+    check(cb, dtype, 1, 100, 1300, 2, 2, 80, rel=rel, kv_mask=m)
+    for Nk in (127, 128, 129):
+        check(cb, dtype, 1, 70, Nk, 2, 2, 32, rel=rel)
+    check(cb, dtype, 6, 2100, 70, 16, 16, 32, rel=rel)              # enough blocks for 32 queries a wave
+
+
+@DT
+def test_wide_blocks(cb, dtype):
+    """enough work for the kernels that hold 32 rows a wave, at an odd length"""
+    check(cb, dtype, 8, 650, 650, 12, 12, 64, causal=True, rel=(32, 128, False), kv_len=[650, 1, 64, 65, 333, 640, 0, 512])
+    check(cb, dtype, 4, 600, 700, 40, 10, 32, kv_len=[700, 130, 650, 9])
+
+
+@DT
 def test_table_entries_at_the_edge(cb, dtype):
     """-inf hides a bucket; the type's lowest value in every bucket leaves the plain softmax (all scores are absorbed alike)"""
     lib, ctx = cb
