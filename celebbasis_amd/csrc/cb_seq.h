@@ -40,6 +40,9 @@ struct SeqBwdPlan { int qb = 1, kb = 1, qsplit = 1, ksplit = 1, nqb = 1; size_t 
 SeqPlan seq_fwd_plan(const SeqArgs& a);
 SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable);
 void seq_forward(const Launch& L, SeqArgs a, void* ws);
+bool seq_token_takes(const SeqArgs& a);                 // one new token a sample (cb_seq_token.hip)
+int seq_token_split(const SeqArgs& a);
+void seq_token(const Launch& L, const SeqArgs& a);
 void seq_backward(const Launch& L, SeqArgs a, void* ws);
 
 constexpr int SEQ_MAX_D = 160, SEQ_MAX_DIST = 1024, SEQ_MAX_BUCKETS = 256;
@@ -220,16 +223,16 @@ __device__ __forceinline__ void seq_row4(const SeqRow<T, DT>& acc, int d, int g,
     }
 }
 
-// the bias of one head by distance, times log2(e), in LDS: bw[rel + D + pad]. Distances past D share the outermost bucket. The entries stay
-// finite in the log2 domain (a table may hold its type's lowest value): held to +-1e37; minus infinity and
-// NaN are kept.
+// the bias of head h at distance rel (within +-D), times log2(e). The entries stay finite in the log2 domain (a table may hold its type's lowest
+// value): held to +-1e37; minus infinity and NaN are kept.
+__device__ __forceinline__ float seq_bias_of(const SeqArgs& a, int h, int rel) {
+    const float b = a.table[(long)a.bmap[rel + a.D] * a.H + h];
+    return ((b == -INFINITY || b != b) ? b : fminf(fmaxf(b, -1e37f), 1e37f)) * SEQ_L2E;
+}
+// the bias of one head by distance in LDS: bw[rel + D + pad]. Distances past D share the outermost bucket.
 __device__ __forceinline__ void seq_bias_fill(float* bw, const SeqArgs& a, int h, int pad, int tid) {
     const int n = 2 * (a.D + pad) + 1;
-    for (int i = tid; i < n; i += 256) {
-        const int rel = min(max(i - (a.D + pad), -a.D), a.D);
-        const float b = a.table[(long)a.bmap[rel + a.D] * a.H + h];
-        bw[i] = ((b == -INFINITY || b != b) ? b : fminf(fmaxf(b, -1e37f), 1e37f)) * SEQ_L2E;
-    }
+    for (int i = tid; i < n; i += 256) bw[i] = seq_bias_of(a, h, min(max(i - (a.D + pad), -a.D), a.D));
 }
 // visible rows of a tile as a bit mask (wave-uniform): rows at or beyond `len` and rows that the key mask hides are clear
 template <int TK>

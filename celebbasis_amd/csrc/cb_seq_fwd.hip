@@ -270,6 +270,7 @@ static void fwd_pick(const Launch& L, const SeqArgs& a, int qb) {
 SeqPlan seq_fwd_plan(const SeqArgs& a) {
     SeqPlan p;
     const long bh = (long)a.B * a.H;
+    const bool token = seq_token_takes(a);
     // measured, 16 against 32 queries a wave: 768 / 384 blocks (8 x 12 heads, 512 x 512, d 64) 22.4 / 25.6 us; 2048 blocks (64 heads, 4096 x 77, d 40)
     // 24.3 / 22.0 us; 512 blocks (64 heads, 1024 x 2000, d 128) 127 / 90 us
     p.qb = fwd_two(a) && bh * cdiv(a.Nq, 128) >= 512 ? 2 : 1;
@@ -277,6 +278,7 @@ SeqPlan seq_fwd_plan(const SeqArgs& a) {
     const long blocks = bh * cdiv(a.Nq, 64 * p.qb);
     const int tiles = (int)cdiv(a.Nk, 64);
     p.nsplit = blocks < 256 && tiles >= 8 ? (int)std::min<long>(cdiv(512, std::max(blocks, 1l)), tiles / 4) : 1;
+    if (token) { p.qb = 0; p.nsplit = seq_token_split(a); }
     if (p.nsplit > 1) {
         p.part = (size_t)p.nsplit * a.B * a.H * a.Nq * a.d * 4;
         p.ml = (size_t)p.nsplit * a.B * a.H * a.Nq * 2 * 4;
@@ -289,7 +291,8 @@ void seq_forward(const Launch& L, SeqArgs a, void* ws) {
     a.nsplit = p.nsplit;
     a.part = static_cast<float*>(ws);
     a.ml = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part);
-    CB_DT_SWITCH(a.dt, T, SEQ_DT_SWITCH(a.d, DT, fwd_pick<T, DT>(L, a, p.qb)));
+    if (p.qb == 0) seq_token(L, a);
+    else CB_DT_SWITCH(a.dt, T, SEQ_DT_SWITCH(a.d, DT, fwd_pick<T, DT>(L, a, p.qb)));
     if (a.nsplit > 1) {
         L.count();
         if (L.dry) return;

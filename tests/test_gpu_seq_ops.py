@@ -346,6 +346,17 @@ def test_one_token_over_a_cache(cb, dtype):
 
 
 @DT
+@pytest.mark.parametrize("d", [8, 24, 40, 64, 80, 128, 160])
+@pytest.mark.parametrize("H,Hkv", [(2, 2), (4, 2), (6, 2), (8, 1), (16, 1)])
+def test_one_token_shapes(cb, dtype, d, H, Hkv):
+    """head dims and head sharing of the one-token kernel (and 16 heads on one: the tile kernel), masks, empty samples, the statistics it keeps"""
+    m = torch.rand(4, 600, generator=torch.Generator().manual_seed(3)) < 0.5
+    m[1] = False
+    check(cb, dtype, 4, 1, 600, H, Hkv, d, kv_mask=m.to(_dev()), kv_len=[600, 600, 0, 33], rel=(32, 64, True), q_pos=[300, 5, 7, 40], q_len=[1, 1, 1, 1])
+    check(cb, dtype, 2, 1, 2100, H, Hkv, d, kv_len=[2100, 257], q_len=[1, 0])
+
+
+@DT
 def test_difference_quotient(cb, dtype):
     """gradients against differences of the forward pass: the loss sum(out * w) along a random direction, in fp32 inputs"""
     if dtype == BF:
