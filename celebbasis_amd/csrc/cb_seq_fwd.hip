@@ -167,16 +167,7 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
                 l[qb] += (s[qb][kt][0] + s[qb][kt][1]) + (s[qb][kt][2] + s[qb][kt][3]);
             }
         }
-        seq_tmul<T, DT, QB>(o, Vs, s, l15, g);
-        if constexpr (PREC) {
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[qb][kt][r] -= (float)(bf16_t)s[qb][kt][r];
-            seq_tmul<T, DT, QB>(o, Vs, s, l15, g);
-        }
+        seq_tmul<T, DT, QB, PREC>(o, Vs, s, l15, g);
     }
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {

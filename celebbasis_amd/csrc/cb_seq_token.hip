@@ -76,25 +76,31 @@ __global__ __launch_bounds__(256) void seq_token_kernel(const SeqArgs a) {
             far_r[r] = seq_bias_of(a, h, a.D);
         }
     }
-    for (int t = k0 + wave * (ROWS * U); t < k1; t += STEP) {
-        u32x4s kv[U], vv[U];
-        bool ok[U];
+    // the loads of the next turn are in flight while this one is computed
+    struct Turn { u32x4s k[U], v[U]; bool ok[U]; } cur, nxt;
+    auto load = [&](int t, Turn& w) {
         const bool all = t + ROWS * U <= k1 && !mask;            // wave-uniform
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int key = t + u * ROWS + grp;
-            ok[u] = all || (key < k1 && (!mask || mask[key] != 0));
-            kv[u] = (u32x4s){0u, 0u, 0u, 0u}; vv[u] = kv[u];
-            if (ok[u] && in) {
-                kv[u] = *reinterpret_cast<const u32x4s*>(K + (long)key * a.k.row);
-                vv[u] = *reinterpret_cast<const u32x4s*>(V + (long)key * a.v.row);
+            w.ok[u] = all || (key < k1 && (!mask || mask[key] != 0));
+            w.k[u] = (u32x4s){0u, 0u, 0u, 0u}; w.v[u] = w.k[u];
+            if (w.ok[u] && in) {
+                w.k[u] = *reinterpret_cast<const u32x4s*>(K + (long)key * a.k.row);
+                w.v[u] = *reinterpret_cast<const u32x4s*>(V + (long)key * a.v.row);
             }
         }
+    };
+    int t = k0 + wave * (ROWS * U);
+    if (t < k1) load(t, cur);
+    for (; t < k1; t += STEP) {
+        if (t + STEP < k1) load(t + STEP, nxt);
+        const bool all = t + ROWS * U <= k1 && !mask;
         float s[U][R];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float x[E];
-            P::open(kv[u], x);
+            P::open(cur.k[u], x);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 float d = 0.f;
@@ -123,7 +129,7 @@ __global__ __launch_bounds__(256) void seq_token_kernel(const SeqArgs a) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int r = 0; r < R; ++r) s[u][r] = ok[u] ? s[u][r] : -INFINITY;
+                for (int r = 0; r < R; ++r) s[u][r] = cur.ok[u] ? s[u][r] : -INFINITY;
         }
         float f[R];
 #pragma unroll
@@ -141,12 +147,13 @@ __global__ __launch_bounds__(256) void seq_token_kernel(const SeqArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float x[E];
-            P::open(vv[u], x);
+            P::open(cur.v[u], x);
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[r][e] = __builtin_fmaf(s[u][r], x[e], o[r][e]);
         }
+        cur = nxt;
     }
     // join the groups of the wave, then the waves
 #pragma unroll
@@ -197,9 +204,10 @@ __global__ __launch_bounds__(256) void seq_token_kernel(const SeqArgs a) {
 // ---------------------------------------------------------------- host side
 bool seq_token_takes(const SeqArgs& a) { return a.Nq == 1 && a.G <= 8; }
 int seq_token_split(const SeqArgs& a) {
-    // about 8 blocks a CU, parts of at least 256 keys
+    // two blocks a CU, parts of at least 256 keys. Blocks 512 / 1024 / 2048: 32 x 12 heads over up to 8192 keys 121 + 5 / 120 + 5 / 116 + 8 us (kernel + join),
+    // 64 x 4 heads over up to 1500 25 + 4 / 27 + 5 / 28 + 5 us
     const long blocks = (long)a.B * a.Hkv;
-    return (int)std::max(1l, std::min<long>(cdiv(2048, std::max(blocks, 1l)), a.Nk / 256));
+    return (int)std::max(1l, std::min<long>(cdiv(512, std::max(blocks, 1l)), a.Nk / 256));
 }
 template <typename T, int PP, int R>
 static void tok_go(const Launch& L, const SeqArgs& a) {
