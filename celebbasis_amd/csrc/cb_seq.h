@@ -81,6 +81,9 @@ __device__ __forceinline__ f32x4 seq_mma(const SeqFrag<float>& a, const SeqFrag<
     return c;
 }
 
+// Waits for a fragment's load here. Without it the compiler puts that wait at the fragment's first use, inside the tile loop, where it also waits
+// for the LDS-DMA of the next tile that has just been issued: every tile then pays the memory latency (measured: forward 114 -> see cb_seq_fwd.hip).
+template <typename T> __device__ __forceinline__ void seq_arrived(SeqFrag<T>& f) { asm volatile("" : "+v"(f.v)); }
 // Geometry of one instantiation. A tile is TK rows in LDS, row-major, P pieces of 16 bytes a row, filled by LDS-DMA in lane-linear slots of
 // 256 pieces; piece c of row r lies at place swz(c, r), which puts the 16 rows that a fragment read touches into 16 different bank groups.
 template <typename T, int DT> struct SeqGeo {
@@ -244,13 +247,14 @@ __device__ __forceinline__ void seq_bias_fill(float* bw, const SeqArgs& a, int h
     const int n = 2 * (a.D + pad) + 1;
     for (int i = tid; i < n; i += 256) bw[i] = seq_bias_of(a, h, min(max(i - (a.D + pad), -a.D), a.D));
 }
-// visible rows of a tile as a bit mask (wave-uniform): rows at or beyond `len` and rows that the key mask hides are clear
-template <int TK>
-__device__ __forceinline__ unsigned long long seq_live(const unsigned char* mask, int r0, int len, int lane) {
-    if (mask) {
-        const int r = r0 + lane;
-        return __ballot(lane < TK && r < len && mask[min(r, len - 1)] != 0);
-    }
+// Visible rows of a tile as a bit mask (wave-uniform): rows at or beyond `len` and rows that the key mask hides are clear. The mask's byte of this
+// lane's row is fetched a tile ahead (seq_mask_byte), so that its latency is not paid between two tiles.
+template <int TK> __device__ __forceinline__ int seq_mask_byte(const unsigned char* mask, int r0, int len, int lane) {
+    const int r = r0 + lane;
+    return mask && lane < TK && r < len ? mask[r] : 0;
+}
+template <int TK> __device__ __forceinline__ unsigned long long seq_live(bool masked, int byte, int r0, int len) {
+    if (masked) return __ballot(byte != 0);
     const int n = len - r0;
     return n >= 64 ? SEQ_ALL<TK> : (n <= 0 ? 0ull : (((1ull << n) - 1) & SEQ_ALL<TK>));
 }

@@ -126,14 +126,31 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
     };
     unsigned long long live = 0, next = 0;
     const int n1 = t1 - t0, u1 = brief ? 2 * n1 : n1;             // steps: the tiles, twice where the first pass makes the row sums
-    if (0 < n1) { next = seq_live<TK>(mask, t0 * TK, klen, lane); stage(0, t0, next); }
+    auto tile_of = [&](int u) { return t0 + (u < n1 ? u : u - n1); };
+    int byte = 0;
+    if (0 < n1) {
+        next = seq_live<TK>(mask, seq_mask_byte<TK>(mask, t0 * TK, klen, lane), t0 * TK, klen);
+        stage(0, t0, next);
+        byte = seq_mask_byte<TK>(mask, tile_of(1) * TK, klen, lane);
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        asm volatile("" : "+v"(lse2[qb]), "+v"(dsum[qb]));
+#pragma unroll
+        for (int s = 0; s < KS; ++s) { seq_arrived(qf[qb][s]); seq_arrived(df[qb][s]); }
+    }
     for (int u = 0; u < u1; ++u) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         live = next;
-        const int t = t0 + (u < n1 ? u : u - n1);
-        if (u + 1 < u1) { const int n = t0 + (u + 1 < n1 ? u + 1 : u + 1 - n1); next = seq_live<TK>(mask, n * TK, klen, lane); stage(u + 1, n, next); }
+        const int t = tile_of(u);
+        if (u + 1 < u1) {
+            const int n = tile_of(u + 1);
+            next = seq_live<TK>(mask, byte, n * TK, klen);
+            byte = seq_mask_byte<TK>(mask, tile_of(u + 2) * TK, klen, lane);
+            stage(u + 1, n, next);
+        }
         if (brief && u == n1) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
@@ -361,42 +378,49 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
     const float scale2 = a.scale * SEQ_L2E;
     const int wbase = wave * 1024;
     float ls = 0.f, dd = 0.f;
-    // per-row numbers of a tile: fetched ahead of its DMA, written to LDS at the end of the step that fetched them
-    auto fetch = [&](int u) {
-        const int h = hk * a.G + u / n1, row = (tq0 + u % n1) * TQ + tid;
-        if (tid < TQ) {
-            ls = INFINITY; dd = 0.f;
-            if (row < qlen) {
-                const long ri = ((long)b * a.H + h) * a.Nq + row;
-                const float x = a.lse[ri];
-                ls = x == -INFINITY ? INFINITY : x * SEQ_L2E;
-                dd = a.dvec[ri];
-            }
+    // the step that is fetched next: head and query tile
+    int hn = hk * a.G, tn = tq0;
+    if (u0 < u1) { hn += u0 / n1; tn += u0 % n1; }
+    auto advance = [&]() { if (++tn == tq0 + n1) { tn = tq0; ++hn; } };
+    // per-row numbers of a tile: fetched ahead of its DMA and not looked at before the end of the step, when they are written to LDS
+    auto fetch = [&]() {
+        const int row = tn * TQ + tid;
+        ls = -INFINITY; dd = 0.f;
+        if (tid < TQ && row < qlen) {
+            const long ri = ((long)b * a.H + hn) * a.Nq + row;
+            ls = a.lse[ri];
+            dd = a.dvec[ri];
         }
     };
     auto stage = [&](int u) {
-        const int h = hk * a.G + u / n1, r0 = (tq0 + u % n1) * TQ;
+        const int r0 = tn * TQ;
         char* dst = lds_seq + (u & 1) * STAGE + wbase;
-        const unsigned long long live = seq_live<TQ>(nullptr, r0, qlen, lane);
-        sq.dma(static_cast<const T*>(a.q.p) + b * a.q.batch + h * a.q.head + (long)r0 * a.q.row, dst, live, tid);
-        sd.dma(static_cast<const T*>(a.dout.p) + b * a.dout.batch + h * a.dout.head + (long)r0 * a.dout.row, dst + G::IMG, live, tid);
+        const unsigned long long live = seq_live<TQ>(false, 0, r0, qlen);
+        sq.dma(static_cast<const T*>(a.q.p) + b * a.q.batch + hn * a.q.head + (long)r0 * a.q.row, dst, live, tid);
+        sd.dma(static_cast<const T*>(a.dout.p) + b * a.dout.batch + hn * a.dout.head + (long)r0 * a.dout.row, dst + G::IMG, live, tid);
     };
     auto put = [&](int u) {
-        if (tid < TQ) { float* w = rows + (u & 1) * 2 * TQ; w[tid] = ls; w[TQ + tid] = dd; }
+        // a row without a visible key (or behind the sample's last) has lse = -inf: with +inf in its place its probabilities are zero
+        if (tid < TQ) { float* w = rows + (u & 1) * 2 * TQ; w[tid] = ls == -INFINITY ? INFINITY : ls * SEQ_L2E; w[TQ + tid] = dd; }
     };
-    if (u0 < u1) { fetch(u0); stage(u0); put(u0); }
+    int h = hn, q0 = tn * TQ;
+    if (u0 < u1) { fetch(); stage(u0); put(u0); }
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) { seq_arrived(kf[kb][s]); seq_arrived(vf[kb][s]); }
     int hcur = -1;
     for (int u = u0; u < u1; ++u) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const int h = hk * a.G + u / n1;
+        h = hn; q0 = tn * TQ;
         if (BIAS && h != hcur) { seq_bias_fill(bw, a, h, PAD, tid); hcur = h; __syncthreads(); }
-        if (u + 1 < u1) { fetch(u + 1); stage(u + 1); }
+        if (u + 1 < u1) { advance(); fetch(); stage(u + 1); }
         const char* Qs = lds_seq + (u & 1) * STAGE;
         const char* Ds = Qs + G::IMG;
         const float* rw = rows + (u & 1) * 2 * TQ;
-        const int q0 = (tq0 + u % n1) * TQ, p0 = pos0 + q0;
+        const int p0 = pos0 + q0;
         f32x4 s[KB][QT], dp[KB][QT];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)

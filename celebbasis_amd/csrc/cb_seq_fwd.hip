@@ -69,14 +69,27 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
         sv.dma(V + (long)t * TK * a.v.row, dst + G::IMG, live, tid);
     };
     unsigned long long live = 0, next = 0;
-    if (t0 < t1) { next = seq_live<TK>(mask, t0 * TK, klen, lane); stage(t0, next); }
+    int byte = 0;
+    if (t0 < t1) {
+        next = seq_live<TK>(mask, seq_mask_byte<TK>(mask, t0 * TK, klen, lane), t0 * TK, klen);
+        stage(t0, next);
+        byte = seq_mask_byte<TK>(mask, (t0 + 1) * TK, klen, lane);
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) seq_arrived(qf[qb][s]);
     for (int t = t0; t < t1; ++t) {
         // tile t has landed for this wave and, behind the barrier, for all; everybody has read the other stage, which is filled next
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         live = next;
-        if (t + 1 < t1) { next = seq_live<TK>(mask, (t + 1) * TK, klen, lane); stage(t + 1, next); }
+        if (t + 1 < t1) {
+            next = seq_live<TK>(mask, byte, (t + 1) * TK, klen);
+            byte = seq_mask_byte<TK>(mask, (t + 2) * TK, klen, lane);
+            stage(t + 1, next);
+        }
         if (live == 0) continue;
         const char* Ks = lds_seq + (t & 1) * STAGE;
         const char* Vs = Ks + G::IMG;
