@@ -28,15 +28,16 @@ struct SeqArgs {
     float* o32 = nullptr;                                                     // [B][Nq][H][d]: the unrounded output (bf16, kept for the backward pass)
     // backward
     SeqT dout, dq, dk, dv;
-    float* dvec = nullptr;                                                    // [B][H][Nq]: rowsum(dO * O)
+    float* dvec = nullptr;                                                    // [ksplit][B][H][Nq]: row sums D (parts of them where keys are split)
     float* dtable = nullptr;                                                  // [nb][H]
-    float* tpart = nullptr;                                                   // [B][H][blocks of queries][nb]
+    int copies = 1;                                                           // of a wave's sums by distance in LDS (4 or 1)
+    float* tpart = nullptr;                                                   // [B][H][parts of queries][blocks of keys][nb]
     float* part = nullptr; float* ml = nullptr; int nsplit = 1;               // partial results of a split axis (fp32): keys (forward), queries (dK, dV)
     float* partq = nullptr; int ksplit = 1;                                    // ... keys (dQ)
 };
 
 struct SeqPlan { int qb = 1, nsplit = 1; size_t part = 0, ml = 0, total = 0; };           // sizes in bytes
-struct SeqBwdPlan { int qb = 1, kb = 1, qsplit = 1, ksplit = 1, nqb = 1; size_t dvec = 0, tpart = 0, part = 0, partq = 0, total = 0; };
+struct SeqBwdPlan { int qb = 1, kb = 1, qsplit = 1, ksplit = 1, nqb = 1, nkb = 1; size_t dvec = 0, tpart = 0, part = 0, partq = 0, total = 0; };
 SeqPlan seq_fwd_plan(const SeqArgs& a);
 SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable);
 void seq_forward(const Launch& L, SeqArgs a, void* ws);
@@ -157,24 +158,17 @@ __device__ __forceinline__ SeqFrag<T> seq_frag_row(const T* row, bool valid, int
 template <typename T, int DT, int QB> using SeqAcc = f32x4[QB][SeqGeo<T, DT>::DA];
 template <typename T, int DT, int QB> using SeqScores = f32x4[QB][SeqGeo<T, DT>::KT];
 template <typename T, int DT> using SeqRow = f32x4[SeqGeo<T, DT>::DA];
-// TWO (bf16): w enters as the sum of two bf16 numbers, the second what the first's rounding left.
-template <typename T, int DT, int QB, bool TWO = false>
+template <typename T, int DT, int QB>
 __device__ __forceinline__ void seq_tmul(SeqAcc<T, DT, QB>& acc, const char* img, const SeqScores<T, DT, QB>& w, int l15, int g) {
     using G = SeqGeo<T, DT>;
     if constexpr (G::ES == 2) {
 #pragma unroll
         for (int kg = 0; kg < G::KT / 2; ++kg) {
-            SeqFrag<bf16_t> b[QB], c[QB];
+            SeqFrag<bf16_t> b[QB];
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
                 const f32x4 x = w[qb][2 * kg], y = w[qb][2 * kg + 1];
                 b[qb].v = (bf16x8_t){(bf16_t)x[0], (bf16_t)x[1], (bf16_t)x[2], (bf16_t)x[3], (bf16_t)y[0], (bf16_t)y[1], (bf16_t)y[2], (bf16_t)y[3]};
-                if constexpr (TWO) {
-                    float rest[8];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { rest[e] = x[e] - (float)b[qb].v[e]; rest[4 + e] = y[e] - (float)b[qb].v[4 + e]; }
-                    c[qb].v = (bf16x8_t){(bf16_t)rest[0], (bf16_t)rest[1], (bf16_t)rest[2], (bf16_t)rest[3], (bf16_t)rest[4], (bf16_t)rest[5], (bf16_t)rest[6], (bf16_t)rest[7]};
-                }
             }
             const int r0 = 4 * g + (l15 >> 2), r1 = r0 + 16;             // row inside the 32-row group
             const int half = (l15 & 3) >> 1, sub = (l15 & 1) * 8;
@@ -187,10 +181,7 @@ __device__ __forceinline__ void seq_tmul(SeqAcc<T, DT, QB>& acc, const char* img
                 typedef short s16x8 __attribute__((ext_vector_type(8)));
                 a.v = __builtin_bit_cast(bf16x8_t, (s16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
 #pragma unroll
-                for (int qb = 0; qb < QB; ++qb) {
-                    acc[qb][t] = seq_mma(a, b[qb], acc[qb][t]);
-                    if constexpr (TWO) acc[qb][t] = seq_mma(a, c[qb], acc[qb][t]);
-                }
+                for (int qb = 0; qb < QB; ++qb) acc[qb][t] = seq_mma(a, b[qb], acc[qb][t]);
             }
         }
     } else {

@@ -1,40 +1,39 @@
 // cb_seq_bwd.hip — backward of the attention of cb_seq.h. With p = exp(s - lse) recomputed tile by tile:
 //   dP = dO V^T,  D = rowsum(dO * O),  dS = p (dP - D);   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,  dtable[c] = sum of dS over the
 //   pairs whose distance j - i lies in bucket c.
-// Row sums D: from dO and the stored output where the key axis is long. Up to SEQ_SHORT keys the first kernel goes over the keys twice and adds
-// p dP in fp32 instead: as exact as the probabilities, and neither output is read (cross attention to prompts is bound by memory).
-// Two kernels, so that no sum depends on the order of arrival: one block of queries over the keys (dQ, D, dtable), one block of keys over the
-// queries of all heads that share them (dK, dV). Both hold the streamed side in LDS row-major and their own side in registers.
+// Two kernels, so that no sum depends on the order of arrival: one block of queries over the keys (dQ, D), one block of keys over the queries of
+// all heads that share them (dK, dV, dtable). Both hold the streamed side in LDS row-major and their own side in registers.
+//
+// Row sums D. Up to SEQ_SHORT keys the first kernel goes over the keys twice and adds p dP in fp32 first: exact, and neither output is read
+// (cross attention to prompts is bound by memory). Longer key axes take D from dO and the stored output, whose probabilities were rounded to
+// bf16; that is good for dQ, but not for dtable, which adds dS over whole diagonals, where the error of a row sum does not cancel. So with a
+// table the first kernel also adds p dP in fp32 on its way and hands these exact sums to the second, which makes dtable.
+// (Measured, dtable of 8 x 12 heads, 512 x 512, bf16, against 64 bits: 2e-3 off with D from the output.)
 //
 // dtable: the distance is constant along the diagonals of a dS tile. Tiles past the table's range add to one number a lane. The others are
-// summed over equal kt - qb in registers, written to LDS with row i shifted by i, and summed by column: each lane owns whole distances, in a
-// fixed order. A wave's sums by distance are folded by bucket at its end.
+// summed over equal qt - kb in registers, then over the 4 rows of a lane by moving row r by r lanes (DPP, what leaves the 16 lanes belongs to
+// the next 16 distances), which leaves every lane one distance per 16 x 16 tile; these are added to sums by distance in LDS. Every wave has
+// sums of its own, and the lanes of a row index g a copy each, so that no two of them meet (where the table's range leaves no room for four
+// copies, one g after the other): the order of all additions is fixed. A wave's sums are folded by bucket at the end of each head.
+// (Measured on 8 x 12 heads, 512 x 512, where half of the tiles are near: by columns of a copy shifted row by row 54 us, by ds_add_f32 134 us.)
 #include "cb_seq.h"
 #include <algorithm>
 
 namespace cb {
 
-template <typename T, int DT, int QB, bool BIAS, bool TAB> struct SeqDq {
+template <typename T, int DT, int QB, bool BIAS> struct SeqDq {
     using G = SeqGeo<T, DT>;
-    static constexpr int PAD = G::TK + 16 * QB, NE = QB + G::KT - 1, NCOL = 16 * NE + 15, SP = NCOL + 2;
-    static constexpr int SKEW = TAB ? 4 * 16 * SP * 4 : 0;
-    static int lds(int D) {
-        const int w = 2 * (D + PAD) + 1;
-        return 4 * G::IMG + (BIAS ? (int)rup(w * 4, 16) : 0) + SKEW + (TAB ? 4 * w * 4 : 0);
-    }
+    static constexpr int PAD = G::TK + 16 * QB;
+    static int lds(int D) { return 4 * G::IMG + (BIAS ? (int)rup((2 * (D + PAD) + 1) * 4, 16) : 0); }
 };
 
-template <typename T, int DT, int QB, bool BIAS, bool TAB>
+template <typename T, int DT, int QB, bool BIAS>
 __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqArgs a, const int nqb) {
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
-    using S = SeqDq<T, DT, QB, BIAS, TAB>;
-    constexpr int TK = G::TK, KT = G::KT, KS = G::KS, STAGE = 2 * G::IMG, PAD = S::PAD, NE = S::NE, SP = S::SP;
+    constexpr int TK = G::TK, KT = G::KT, KS = G::KS, STAGE = 2 * G::IMG, PAD = SeqDq<T, DT, QB, BIAS>::PAD;
     extern __shared__ __attribute__((aligned(16))) char lds_seq[];
-    const int W = 2 * (a.D + PAD) + 1;
     float* bw = reinterpret_cast<float*>(lds_seq + 2 * STAGE);
-    float* skew = bw + ((W + 3) & ~3);
-    float* hist = skew + 4 * 16 * SP;
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int rank, b, h;
@@ -59,7 +58,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
     }
 
     SeqFrag<T> qf[QB][KS], df[QB][KS];
-    float lse2[QB], dsum[QB];
+    float lse2[QB], dsum[QB], own[QB];                            // own: the sum of p dP as this block sees it
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
         const int row = q0 + 16 * qb + l15;
@@ -99,7 +98,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
             for (int e = 0; e < G::EP; ++e) ds = __builtin_fmaf(x[e], y[e], ds);
         }
         dsum[qb] = brief ? 0.f : seq_group_sum(ds);
-        if (g == 0 && row < a.Nq && split == 0) a.dvec[ri] = dsum[qb];          // (a row without a visible key: 0 either way)
+        own[qb] = 0.f;
     }
     const float scale2 = a.scale * SEQ_L2E;
     f32x4 acc[QB][G::DA];
@@ -107,17 +106,10 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
     for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
         for (int t = 0; t < G::DA; ++t) acc[qb][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    float far_l = 0.f, far_r = 0.f;
     SeqSlots<T, DT> sk, sv;
     sk.init(a.k.row, a.d, tid);
     sv.init(a.v.row, a.d, tid);
     if constexpr (BIAS) seq_bias_fill(bw, a, h, PAD, tid);
-    float* sw = skew + wave * 16 * SP;
-    float* hw = hist + wave * W;
-    if constexpr (TAB) {
-        for (int i = lane; i < 16 * SP; i += 64) sw[i] = 0.f;
-        for (int i = lane; i < W; i += 64) hw[i] = 0.f;
-    }
     const int wbase = wave * 1024;
     auto stage = [&](int u, int t, unsigned long long live) {
         char* dst = lds_seq + (u & 1) * STAGE + wbase;
@@ -153,11 +145,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
         }
         if (brief && u == n1) {
 #pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-                dsum[qb] = seq_group_sum(dsum[qb]);
-                const int row = q0 + 16 * qb + l15;
-                if (g == 0 && row < a.Nq) a.dvec[(long)bh * a.Nq + row] = dsum[qb];
-            }
+            for (int qb = 0; qb < QB; ++qb) dsum[qb] = seq_group_sum(own[qb]);
         }
         if (live == 0) continue;
         const char* Ks = lds_seq + (u & 1) * STAGE;
@@ -181,11 +169,10 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
                 }
             }
         float cb = 0.f, sc = scale2;
-        int side = 0;                                             // -1 / 1: past the table's range on the left / right, 0: by distance
         if constexpr (BIAS) {
             const int hi = k0 + TK - 1 - p0, lo = k0 - p0 - (16 * QB - 1);
-            if (hi <= -a.D) { cb = bw[PAD]; side = -1; }
-            else if (lo >= a.D) { cb = bw[2 * a.D + PAD]; side = 1; }
+            if (hi <= -a.D) cb = bw[PAD];
+            else if (lo >= a.D) cb = bw[2 * a.D + PAD];
             else {
                 const float* w = bw + (k0 + 4 * g - p0 - l15 + a.D + PAD);
                 sc = 1.f;
@@ -197,17 +184,13 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
                         for (int r = 0; r < 4; ++r) s[qb][kt][r] = __builtin_fmaf(s[qb][kt][r], scale2, w[16 * kt + r - 16 * qb]);
             }
         }
-        const bool sums = brief && u < n1;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-            const float off = cb - lse2[qb], ds = sums ? 0.f : dsum[qb];
+            const float off = cb - lse2[qb];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][kt][r], sc, off));
-                    s[qb][kt][r] = p * (dp[qb][kt][r] - ds);
-                }
+                for (int r = 0; r < 4; ++r) s[qb][kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][kt][r], sc, off));
         }
         // zero what is not visible
         if (live != SEQ_ALL<TK>) {
@@ -234,50 +217,30 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
                     for (int r = 0; r < 4; ++r) s[qb][kt][r] = k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15 ? s[qb][kt][r] : 0.f;
                 }
         }
-        if (sums) {
+        if (brief ? u < n1 : BIAS) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt) dsum[qb] += (s[qb][kt][0] + s[qb][kt][1]) + (s[qb][kt][2] + s[qb][kt][3]);
-            continue;
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) own[qb] = __builtin_fmaf(s[qb][kt][r], dp[qb][kt][r], own[qb]);
         }
-        if constexpr (TAB) {
-            if (side != 0) {
-                float sum = 0.f;
+        if (brief && u < n1) continue;
 #pragma unroll
-                for (int qb = 0; qb < QB; ++qb)
+        for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt) sum += (s[qb][kt][0] + s[qb][kt][1]) + (s[qb][kt][2] + s[qb][kt][3]);
-                if (side < 0) far_l += sum; else far_r += sum;
-            } else {
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                for (int e = 0; e < NE; ++e) {
-                    f32x4 x = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int qb = 0; qb < QB; ++qb) {
-                        const int kt = e - (QB - 1) + qb;
-                        if (kt >= 0 && kt < KT) x += s[qb][kt];
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) sw[l15 * SP + 16 * e + 4 * g + r + 15 - l15] = x[r];
-                }
-                asm volatile("" ::: "memory");                    // one wave's LDS accesses execute in order
-                float* hb = hw + (k0 - p0 - 16 * (QB - 1) - 15 + a.D + PAD);
-                for (int c = lane; c < S::NCOL; c += 64) {
-                    float x = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x += sw[i * SP + c];
-                    hb[c] += x;
-                }
-                asm volatile("" ::: "memory");
-            }
-        }
+                for (int r = 0; r < 4; ++r) s[qb][kt][r] *= dp[qb][kt][r] - dsum[qb];
         seq_tmul<T, DT, QB>(acc, Ks, s, l15, g);
     }
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
         const int row = q0 + 16 * qb + l15;
+        // brief: dsum is the exact sum (0 where nothing is visible); with a table: the exact sum of this part of the keys; else the one from the output
+        const float D = brief ? (n1 ? dsum[qb] : 0.f) : BIAS ? seq_group_sum(own[qb]) : split == 0 ? dsum[qb] : 0.f;
         if (row >= a.Nq) continue;
+        if (g == 0) a.dvec[((long)split * a.B * a.H + bh) * a.Nq + row] = D;
         if (a.ksplit > 1) {
             float* P = a.partq + (((long)split * a.B * a.H + bh) * a.Nq + row) * a.d;
             seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(P + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
@@ -286,57 +249,46 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
         T* dQ = static_cast<T*>(a.dq.p) + b * a.dq.batch + h * a.dq.head + (long)row * a.dq.row;
         seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(dQ + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
     }
-    if constexpr (TAB) {
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { far_l += __shfl_xor(far_l, o, 64); far_r += __shfl_xor(far_r, o, 64); }
-        asm volatile("" ::: "memory");
-        if (lane == 0) { hw[0] += far_l; hw[W - 1] += far_r; }
-        __syncthreads();
-        for (int i = tid; i < W; i += 256) hist[i] = (hist[i] + hist[W + i]) + (hist[2 * W + i] + hist[3 * W + i]);
-        __syncthreads();
-        float* out = a.tpart + (((long)bh * a.ksplit + split) * nqb + qblk) * a.nb;
-        for (int c = wave; c < a.nb; c += 4) {
-            const int lo = a.brange[2 * c], hi = a.brange[2 * c + 1];           // distances + D of the bucket, [lo, hi)
-            float x = 0.f;
-            if (lo < hi) {
-                const int i0 = lo == 0 ? 0 : lo + PAD, i1 = hi == 2 * a.D + 1 ? W : hi + PAD;
-                for (int i = i0 + lane; i < i1; i += 64) x += hist[i];
-            }
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-            if (lane == 0) out[c] = x;
-        }
-    }
 #endif
 }
 
-// dtable[c][h] = sum over samples and query blocks of their parts; one wave a (bucket, head), 64-bit sums
-__global__ __launch_bounds__(64) void seq_dtable_kernel(const SeqArgs a, const int nqb) {
+// dtable[c][h] = sum of the parts of all samples and key blocks; one wave a (bucket, head), 64-bit sums
+__global__ __launch_bounds__(64) void seq_dtable_kernel(const SeqArgs a, const int n) {
     const int c = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
     double x = 0.0;
-    for (int i = lane; i < a.B * nqb; i += 64) {
-        const int b = i / nqb, y = i - b * nqb;
-        x += (double)a.tpart[(((long)b * a.H + h) * nqb + y) * a.nb + c];
+    for (int i = lane; i < a.B * n; i += 64) {
+        const int b = i / n, y = i - b * n;
+        x += (double)a.tpart[(((long)b * a.H + h) * n + y) * a.nb + c];
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
     if (lane == 0) a.dtable[(long)c * a.H + h] = (float)x;
 }
 
-template <typename T, int DT, int KB, bool BIAS> struct SeqDkv {
+// v moved between the lanes of each 16 (0 where a lane has no source)
+template <int CTRL> __device__ __forceinline__ float dpp0(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <typename T, int DT, int KB, bool BIAS, bool TAB> struct SeqDkv {
     using G = SeqGeo<T, DT>;
-    static constexpr int PAD = G::TK + 16 * KB;
-    static int lds(int D) { return 4 * G::IMG + 4 * G::TK * 4 + (BIAS ? (int)rup((2 * (D + PAD) + 1) * 4, 16) : 0); }
+    static constexpr int PAD = G::TK + 16 * KB + 16, NE = KB + G::KT - 1;
+    static int lds(int D, int copies) {
+        const int w = 2 * (D + PAD) + 1;
+        return 4 * G::IMG + 4 * G::TK * 4 + (BIAS ? (int)rup(w * 4, 16) : 0) + (TAB ? 4 * copies * w * 4 : 0);
+    }
 };
 
-template <typename T, int DT, int KB, bool BIAS>
+template <typename T, int DT, int KB, bool BIAS, bool TAB>
 __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqArgs a, const int nkb) {
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
-    constexpr int TQ = G::TK, QT = G::KT, KS = G::KS, STAGE = 2 * G::IMG, PAD = SeqDkv<T, DT, KB, BIAS>::PAD;
+    using S = SeqDkv<T, DT, KB, BIAS, TAB>;
+    constexpr int TQ = G::TK, QT = G::KT, KS = G::KS, STAGE = 2 * G::IMG, PAD = S::PAD, NE = S::NE;
     extern __shared__ __attribute__((aligned(16))) char lds_seq[];
+    const int W = 2 * (a.D + PAD) + 1;
     float* rows = reinterpret_cast<float*>(lds_seq + 2 * STAGE);      // [2 stages][lse, D][TQ]
     float* bw = rows + 4 * TQ;
+    float* hist = bw + ((W + 3) & ~3);                                // [4 waves][copies][W]
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kblk = blockIdx.x / (a.B * a.Hkv), bk = blockIdx.x - kblk * (a.B * a.Hkv), b = bk / a.Hkv, hk = bk - b * a.Hkv;   // causal: the long ones first
@@ -390,6 +342,7 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
             const long ri = ((long)b * a.H + hn) * a.Nq + row;
             ls = a.lse[ri];
             dd = a.dvec[ri];
+            for (int s = 1; s < a.ksplit; ++s) dd += a.dvec[(long)s * a.B * a.H * a.Nq + ri];
         }
     };
     auto stage = [&](int u) {
@@ -409,13 +362,58 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int s = 0; s < KS; ++s) { seq_arrived(kf[kb][s]); seq_arrived(vf[kb][s]); }
+    float far_l = 0.f, far_r = 0.f;
+    float* hw = hist + wave * a.copies * W;
+    auto clear = [&]() {
+        for (int i = lane; i < a.copies * W; i += 64) hw[i] = 0.f;
+        far_l = far_r = 0.f;
+    };
+    auto out_of = [&](int h) { return a.tpart + ((((long)b * a.H + h) * a.nsplit + split) * nkb + kblk) * a.nb; };
+    // the sums by distance of head h, folded over the waves and by bucket (all threads of the block)
+    auto fold = [&](int h) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { far_l += __shfl_xor(far_l, o, 64); far_r += __shfl_xor(far_r, o, 64); }
+        asm volatile("" ::: "memory");
+        if (lane == 0) { hw[0] += far_l; hw[W - 1] += far_r; }
+        __syncthreads();
+        for (int i = tid; i < W; i += 256) {
+            float x = hist[i];
+            for (int c = 1; c < 4 * a.copies; ++c) x += hist[c * W + i];
+            hist[i] = x;
+        }
+        __syncthreads();
+        float* out = out_of(h);
+        for (int c = wave; c < a.nb; c += 4) {
+            const int lo = a.brange[2 * c], hi = a.brange[2 * c + 1];           // distances + D of the bucket, [lo, hi)
+            float x = 0.f;
+            if (lo < hi) {
+                const int i0 = lo == 0 ? 0 : lo + PAD, i1 = hi == 2 * a.D + 1 ? W : hi + PAD;
+                for (int i = i0 + lane; i < i1; i += 64) x += hist[i];
+            }
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+            if (lane == 0) out[c] = x;
+        }
+        __syncthreads();
+    };
+    if constexpr (TAB) {
+        clear();
+        const int h0 = hk * a.G, ha = u0 < u1 ? h0 + u0 / n1 : h0 + a.G, hb = u0 < u1 ? h0 + (u1 - 1) / n1 : h0 + a.G;
+        for (int x = h0; x < h0 + a.G; ++x)                           // heads of the group that this part of the steps does not reach
+            if (x < ha || x > hb) for (int c = tid; c < a.nb; c += 256) out_of(x)[c] = 0.f;
+    }
     int hcur = -1;
     for (int u = u0; u < u1; ++u) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         h = hn; q0 = tn * TQ;
-        if (BIAS && h != hcur) { seq_bias_fill(bw, a, h, PAD, tid); hcur = h; __syncthreads(); }
+        if (BIAS && h != hcur) {
+            if (TAB && hcur >= 0) { fold(hcur); clear(); }
+            seq_bias_fill(bw, a, h, PAD, tid);
+            hcur = h;
+            __syncthreads();
+        }
         if (u + 1 < u1) { advance(); fetch(); stage(u + 1); }
         const char* Qs = lds_seq + (u & 1) * STAGE;
         const char* Ds = Qs + G::IMG;
@@ -439,10 +437,11 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
                 }
             }
         float cb = 0.f, sc = scale2;
+        int side = 0;                                             // -1 / 1: past the table's range on the left / right, 0: by distance
         if constexpr (BIAS) {
             const int hi = k0 + 16 * KB - 1 - p0, lo = k0 - p0 - (TQ - 1);
-            if (hi <= -a.D) cb = bw[PAD];
-            else if (lo >= a.D) cb = bw[2 * a.D + PAD];
+            if (hi <= -a.D) { cb = bw[PAD]; side = -1; }
+            else if (lo >= a.D) { cb = bw[2 * a.D + PAD]; side = 1; }
             else {
                 const float* w = bw + (k0 + l15 - p0 - 4 * g + a.D + PAD);
                 sc = 1.f;
@@ -478,10 +477,62 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
                         if (k0 + 16 * kb + l15 > p0 + 16 * qt + 4 * g + r) { s[kb][qt][r] = 0.f; dp[kb][qt][r] = 0.f; }
                 }
         }
+        if constexpr (TAB) {
+            // (columns of keys that are not visible hold anything)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+                if (!__all(seen[kb])) {
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt) {
+                        seq_pin(dp[kb][qt]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) dp[kb][qt][r] = seen[kb] ? dp[kb][qt][r] : 0.f;
+                    }
+                }
+            if (side != 0) {
+                float sum = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt) sum += (dp[kb][qt][0] + dp[kb][qt][1]) + (dp[kb][qt][2] + dp[kb][qt][3]);
+                if (side < 0) far_l += sum; else far_r += sum;
+            } else {
+                f32x4 x[NE];                                      // by e = qt - kb + KB - 1
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    x[e] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) {
+                        const int qt = e - (KB - 1) + kb;
+                        if (qt >= 0 && qt < QT) x[e] += dp[kb][qt];
+                    }
+                }
+                float y[NE + 1];
+                y[0] = 0.f;
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    y[e] += x[e][0] + dpp0<0x101>(x[e][1]) + dpp0<0x102>(x[e][2]) + dpp0<0x103>(x[e][3]);          // row_shl: lane l takes lane l + r
+                    y[e + 1] = dpp0<0x11F>(x[e][1]) + dpp0<0x11E>(x[e][2]) + dpp0<0x11D>(x[e][3]);                 // row_shr by 16 - r: the lanes below r
+                }
+                float* hb = hw + (k0 - p0 + l15 - 4 * g + a.D + PAD + 16 * (KB - 1)) + (a.copies == 4 ? g * W : 0);
+                auto add = [&]() {
+                    float o[NE + 1];
+#pragma unroll
+                    for (int e = 0; e <= NE; ++e) o[e] = hb[-16 * e];
+#pragma unroll
+                    for (int e = 0; e <= NE; ++e) hb[-16 * e] = o[e] + y[e];
+                };
+                asm volatile("" ::: "memory");
+                if (a.copies == 4) add();
+                else for (int q = 0; q < 4; ++q) { if (g == q) add(); asm volatile("" ::: "memory"); }
+                asm volatile("" ::: "memory");
+            }
+        }
         seq_tmul<T, DT, KB>(dv, Ds, s, l15, g);
         seq_tmul<T, DT, KB>(dk, Qs, dp, l15, g);
         if (u + 1 < u1) put(u + 1);
     }
+    if constexpr (TAB) { if (hcur >= 0) fold(hcur); }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
         const int key = k0 + 16 * kb + l15;
@@ -535,6 +586,7 @@ SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable) {
     p.qb = wide && a.Nk > SEQ_SHORT ? 2 : 1;
     p.kb = wide && bk * cdiv(a.Nk, 128) >= 768 ? 2 : 1;
     p.nqb = (int)cdiv(a.Nq, 64 * p.qb);
+    p.nkb = (int)cdiv(a.Nk, 64 * p.kb);
     // few blocks of keys (or queries): the other axis is split into runs of at least 4 tiles. 128 blocks (64 heads, 4096 x 77, d 40): 102 us whole,
     // 26 + 5 us in 8 parts
     const long fill = a.dt == DT_BF16 ? 1024 : 512;
@@ -542,44 +594,47 @@ SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable) {
     p.qsplit = kblocks < 384 && steps >= 8 ? (int)std::min<long>(fill / std::max(kblocks, 1l), steps / 4) : 1;
     const long qblocks = bh * p.nqb, tiles = cdiv(a.Nk, 64);
     p.ksplit = qblocks < 256 && tiles >= 8 && a.Nk > SEQ_SHORT ? (int)std::min<long>(cdiv(512, std::max(qblocks, 1l)), tiles / 4) : 1;
-    p.dvec = (size_t)rup((long)a.B * a.H * a.Nq * 4, 256);
-    p.tpart = want_dtable ? (size_t)rup((long)a.B * a.H * p.ksplit * p.nqb * a.nb * 4, 256) : 0;
+    p.dvec = (size_t)rup((long)p.ksplit * a.B * a.H * a.Nq * 4, 256);
+    p.tpart = want_dtable ? (size_t)rup((long)a.B * a.H * p.qsplit * p.nkb * a.nb * 4, 256) : 0;
     p.part = p.qsplit > 1 ? (size_t)rup((long)p.qsplit * 2 * a.B * a.Hkv * a.Nk * a.d * 4, 256) : 0;
     p.partq = p.ksplit > 1 ? (size_t)p.ksplit * a.B * a.H * a.Nq * a.d * 4 : 0;
     p.total = p.dvec + p.tpart + p.part + p.partq;
     return p;
 }
-template <typename T, int DT, int QB, bool BIAS, bool TAB>
+template <typename T, int DT, int QB, bool BIAS>
 static void dq_go(const Launch& L, const SeqArgs& a, int nqb) {
     if (!((long)nqb * a.B)) return;
     L.count();
     if (L.dry) return;
-    const int lds = SeqDq<T, DT, QB, BIAS, TAB>::lds(a.D);
-    set_dyn_lds(reinterpret_cast<const void*>(&seq_dq_kernel<T, DT, QB, BIAS, TAB>), 160 * 1024);
-    hipLaunchKernelGGL((seq_dq_kernel<T, DT, QB, BIAS, TAB>), dim3((unsigned)nqb * a.B * a.H, a.ksplit), dim3(256), lds, L.stream, a, nqb);
+    const int lds = SeqDq<T, DT, QB, BIAS>::lds(a.D);
+    set_dyn_lds(reinterpret_cast<const void*>(&seq_dq_kernel<T, DT, QB, BIAS>), 160 * 1024);
+    hipLaunchKernelGGL((seq_dq_kernel<T, DT, QB, BIAS>), dim3((unsigned)nqb * a.B * a.H, a.ksplit), dim3(256), lds, L.stream, a, nqb);
     CB_HIP(hipGetLastError());
 }
-template <typename T, int DT, int KB, bool BIAS>
-static void dkv_go(const Launch& L, const SeqArgs& a) {
+template <typename T, int DT, int KB, bool BIAS, bool TAB>
+static void dkv_go(const Launch& L, SeqArgs a) {
     const int nkb = (int)cdiv(a.Nk, 64 * KB);
     if (!((long)nkb * a.B)) return;
     L.count();
     if (L.dry) return;
-    const int lds = SeqDkv<T, DT, KB, BIAS>::lds(a.D);
-    set_dyn_lds(reinterpret_cast<const void*>(&seq_dkv_kernel<T, DT, KB, BIAS>), 160 * 1024);
-    hipLaunchKernelGGL((seq_dkv_kernel<T, DT, KB, BIAS>), dim3((unsigned)nkb * a.B * a.Hkv, a.nsplit), dim3(256), lds, L.stream, a, nkb);
+    using S = SeqDkv<T, DT, KB, BIAS, TAB>;
+    a.copies = S::lds(a.D, 4) <= 80 * 1024 ? 4 : 1;                  // two blocks a CU
+    const int lds = S::lds(a.D, a.copies);
+    CB_CHECK(lds <= 160 * 1024, CB_ERR_SHAPE, "seq attention: %d bytes of LDS for head dim %d and max_distance %d", lds, a.d, a.D);
+    set_dyn_lds(reinterpret_cast<const void*>(&seq_dkv_kernel<T, DT, KB, BIAS, TAB>), 160 * 1024);
+    hipLaunchKernelGGL((seq_dkv_kernel<T, DT, KB, BIAS, TAB>), dim3((unsigned)nkb * a.B * a.Hkv, a.nsplit), dim3(256), lds, L.stream, a, nkb);
     CB_HIP(hipGetLastError());
 }
 template <typename T, int DT, int QB>
 static void dq_kind(const Launch& L, const SeqArgs& a, int nqb) {
-    if (a.table && a.dtable) dq_go<T, DT, QB, true, true>(L, a, nqb);
-    else if (a.table) dq_go<T, DT, QB, true, false>(L, a, nqb);
-    else dq_go<T, DT, QB, false, false>(L, a, nqb);
+    if (a.table) dq_go<T, DT, QB, true>(L, a, nqb);
+    else dq_go<T, DT, QB, false>(L, a, nqb);
 }
 template <typename T, int DT, int KB>
 static void dkv_kind(const Launch& L, const SeqArgs& a) {
-    if (a.table) dkv_go<T, DT, KB, true>(L, a);
-    else dkv_go<T, DT, KB, false>(L, a);
+    if (a.table && a.dtable) dkv_go<T, DT, KB, true, true>(L, a);
+    else if (a.table) dkv_go<T, DT, KB, true, false>(L, a);
+    else dkv_go<T, DT, KB, false, false>(L, a);
 }
 template <typename T, int DT>
 static void bwd_pick(const Launch& L, const SeqArgs& a, const SeqBwdPlan& p) {
@@ -612,7 +667,7 @@ void seq_backward(const Launch& L, SeqArgs a, void* ws) {
     if (a.dtable) {
         L.count();
         if (!L.dry) {
-            hipLaunchKernelGGL(seq_dtable_kernel, dim3(a.nb, a.H), dim3(64), 0, L.stream, a, p.nqb * a.ksplit);
+            hipLaunchKernelGGL(seq_dtable_kernel, dim3(a.nb, a.H), dim3(64), 0, L.stream, a, p.nkb * p.qsplit);
             CB_HIP(hipGetLastError());
         }
     }

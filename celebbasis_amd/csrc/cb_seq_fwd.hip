@@ -8,10 +8,7 @@
 
 namespace cb {
 
-// PREC (bf16 with out32): the probabilities enter P.V as the sum of two bf16 numbers, so that the unrounded output, and with it the row sums
-// dO.O of the backward pass, carry 2^-18 instead of 2^-9 of rounding: dtable adds dS over whole diagonals, where the error of a row sum does
-// not cancel (measured without it: dtable 2e-3 off).
-template <typename T, int DT, int QB, bool BIAS, bool PREC>
+template <typename T, int DT, int QB, bool BIAS>
 __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqArgs a, const int nqb) {
 #ifdef __HIP_DEVICE_COMPILE__      // the host pass needs the launch stub alone
     using G = SeqGeo<T, DT>;
@@ -180,7 +177,7 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
                 l[qb] += (s[qb][kt][0] + s[qb][kt][1]) + (s[qb][kt][2] + s[qb][kt][3]);
             }
         }
-        seq_tmul<T, DT, QB, PREC>(o, Vs, s, l15, g);
+        seq_tmul<T, DT, QB>(o, Vs, s, l15, g);
     }
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -239,37 +236,29 @@ __global__ __launch_bounds__(256) void seq_combine_kernel(const SeqArgs a) {
 }
 
 // ---------------------------------------------------------------- host side
-template <typename T, int DT, int QB, bool BIAS, bool PREC>
+template <typename T, int DT, int QB, bool BIAS>
 static void fwd_go(const Launch& L, const SeqArgs& a) {
     using G = SeqGeo<T, DT>;
     const int nqb = (int)cdiv(a.Nq, 64 * QB);
     const int lds = 4 * G::IMG + (BIAS ? (int)rup((2 * (a.D + G::TK + 16 * QB) + 1) * 4, 16) : 0);
     L.count();
     if (L.dry) return;
-    set_dyn_lds(reinterpret_cast<const void*>(&seq_fwd_kernel<T, DT, QB, BIAS, PREC>), 160 * 1024);
-    hipLaunchKernelGGL((seq_fwd_kernel<T, DT, QB, BIAS, PREC>), dim3((unsigned)nqb * a.B * a.H, a.nsplit), dim3(256), lds, L.stream, a, nqb);
+    set_dyn_lds(reinterpret_cast<const void*>(&seq_fwd_kernel<T, DT, QB, BIAS>), 160 * 1024);
+    hipLaunchKernelGGL((seq_fwd_kernel<T, DT, QB, BIAS>), dim3((unsigned)nqb * a.B * a.H, a.nsplit), dim3(256), lds, L.stream, a, nqb);
     CB_HIP(hipGetLastError());
 }
-template <typename T, int DT>
-static void fwd_kind(const Launch& L, const SeqArgs& a) {
-    if constexpr (sizeof(T) == 2) {
-        if (a.o32 && a.table) { fwd_go<T, DT, 1, true, true>(L, a); return; }
-    }
-    if (a.table) fwd_go<T, DT, 1, true, false>(L, a);
-    else fwd_go<T, DT, 1, false, false>(L, a);
-}
-// 32 queries a wave read every K and V fragment for two products instead of one; where the registers do not hold them (two-part probabilities,
-// fp32 or bf16 heads beyond 128) or the grid would not fill the chip, 16
-static bool fwd_two(const SeqArgs& a) { return a.dt == DT_BF16 ? a.d <= 128 && !(a.o32 && a.table) : a.d <= 32; }
+// 32 queries a wave read every K and V fragment for two products instead of one; where the registers do not hold them (fp32, or heads beyond
+// 128) or the grid would not fill the chip, 16
+static bool fwd_two(const SeqArgs& a) { return a.dt == DT_BF16 ? a.d <= 128 : a.d <= 32; }
 template <typename T, int DT>
 static void fwd_pick(const Launch& L, const SeqArgs& a, int qb) {
     if constexpr (sizeof(T) == 2 ? DT <= 8 : DT == 2) {
         if (qb == 2) {
-            if (a.table) fwd_go<T, DT, 2, true, false>(L, a); else fwd_go<T, DT, 2, false, false>(L, a);
+            if (a.table) fwd_go<T, DT, 2, true>(L, a); else fwd_go<T, DT, 2, false>(L, a);
             return;
         }
     }
-    fwd_kind<T, DT>(L, a);
+    if (a.table) fwd_go<T, DT, 1, true>(L, a); else fwd_go<T, DT, 1, false>(L, a);
 }
 SeqPlan seq_fwd_plan(const SeqArgs& a) {
     SeqPlan p;
