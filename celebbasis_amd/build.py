@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libcelebbasis_hip.so")
 SOURCES = ["cb_gemm.hip", "cb_gemm_glds.hip", "cb_gemm_bf16_p8.hip", "cb_flash.hip", "cb_flash_bf16.hip", "cb_flash_bf16_v2.hip", "cb_kernels.hip", "cb_engine.hip", "cb_models.hip",
-           "cb_seq_fwd.hip", "cb_seq_bwd.hip", "cb_seq_token.hip", "cb_norm_i8.hip", "cb_gemm_i8.hip", "cb_abi.hip"]
+           "cb_seq_fwd.hip", "cb_seq_bwd.hip", "cb_seq_token.hip", "cb_seq_short.hip", "cb_norm_i8.hip", "cb_gemm_i8.hip", "cb_abi.hip"]
 HEADERS = ["cb_common.h", "cb_device.h", "cb_gemm_tiles.h", "cb_plan_table.inc", "cb_engine.h", "cb_models.h", "cb_seq.h", "cb_i8.h", os.path.join("..", "..", "include", "celebbasis_hip.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
          "-Wno-unused-lambda-capture", "-Wno-unused-result"]
@@ -26,9 +26,9 @@ EXTRA = {src: (["-mllvm", "-amdgpu-mfma-vgpr-form"] if os.environ.get("CB_MFMA_V
 # Packed fp32 instructions are kept out of these files: hipcc forms them from ordinary float code, and some of their forms have given wrong
 # results on this part. (The host pass does not know the feature and says so.)
 NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-for _src in ("cb_seq_fwd.hip", "cb_seq_bwd.hip"):
+for _src in ("cb_seq_fwd.hip", "cb_seq_bwd.hip", "cb_seq_short.hip"):
     EXTRA[_src] = EXTRA["cb_flash.hip"] + NO_PACKED
-for _src in ("cb_seq_token.hip", "cb_norm_i8.hip", "cb_gemm_i8.hip"):
+for _src in ("cb_seq_token.hip", "cb_seq_short.hip", "cb_norm_i8.hip", "cb_gemm_i8.hip"):
     EXTRA[_src] = NO_PACKED
 # Kernels whose software pipeline COUNTS its outstanding VMEM instructions (`s_waitcnt vmcnt(N)` + raw `s_barrier`,
 # cb_gemm_glds.hip): a register spill would add scratch loads / stores to that count and let a tile be read before it has landed.

@@ -30,7 +30,6 @@ struct SeqArgs {
     SeqT dout, dq, dk, dv;
     float* dvec = nullptr;                                                    // [ksplit][B][H][Nq]: row sums D (parts of them where keys are split)
     float* dtable = nullptr;                                                  // [nb][H]
-    int copies = 1;                                                           // of a wave's sums by distance in LDS (4 or 1)
     float* tpart = nullptr;                                                   // [B][H][parts of queries][blocks of keys][nb]
     float* part = nullptr; float* ml = nullptr; int nsplit = 1;               // partial results of a split axis (fp32): keys (forward), queries (dK, dV)
     float* partq = nullptr; int ksplit = 1;                                    // ... keys (dQ)
@@ -44,6 +43,8 @@ void seq_forward(const Launch& L, SeqArgs a, void* ws);
 bool seq_token_takes(const SeqArgs& a);                 // one new token a sample (cb_seq_token.hip)
 int seq_token_split(const SeqArgs& a);
 void seq_token(const Launch& L, const SeqArgs& a);
+bool seq_short_takes(const SeqArgs& a);                 // up to SEQ_SHORT keys (cb_seq_short.hip): forward and dQ
+void seq_short(const Launch& L, const SeqArgs& a, bool bwd);
 void seq_backward(const Launch& L, SeqArgs a, void* ws);
 
 constexpr int SEQ_MAX_D = 160, SEQ_MAX_DIST = 1024, SEQ_MAX_BUCKETS = 256;

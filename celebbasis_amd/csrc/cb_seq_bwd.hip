@@ -4,18 +4,18 @@
 // Two kernels, so that no sum depends on the order of arrival: one block of queries over the keys (dQ, D), one block of keys over the queries of
 // all heads that share them (dK, dV, dtable). Both hold the streamed side in LDS row-major and their own side in registers.
 //
-// Row sums D. Up to SEQ_SHORT keys the first kernel goes over the keys twice and adds p dP in fp32 first: exact, and neither output is read
-// (cross attention to prompts is bound by memory). Longer key axes take D from dO and the stored output, whose probabilities were rounded to
-// bf16; that is good for dQ, but not for dtable, which adds dS over whole diagonals, where the error of a row sum does not cancel. So with a
-// table the first kernel also adds p dP in fp32 on its way and hands these exact sums to the second, which makes dtable.
+// Row sums D. Up to SEQ_SHORT keys cb_seq_short.hip stands in for the first kernel and makes them from the probabilities. Longer key axes take D
+// from dO and the stored output, whose probabilities were rounded to bf16; that is good for dQ, but not for dtable, which adds dS over whole
+// diagonals, where the error of a row sum does not cancel. So with a table the first kernel also adds p dP in fp32 on its way and hands these
+// exact sums to the second, which makes dtable.
 // (Measured, dtable of 8 x 12 heads, 512 x 512, bf16, against 64 bits: 2e-3 off with D from the output.)
 //
 // dtable: the distance is constant along the diagonals of a dS tile. Tiles past the table's range add to one number a lane. The others are
 // summed over equal qt - kb in registers, then over the 4 rows of a lane by moving row r by r lanes (DPP, what leaves the 16 lanes belongs to
-// the next 16 distances), which leaves every lane one distance per 16 x 16 tile; these are added to sums by distance in LDS. Every wave has
-// sums of its own, and the lanes of a row index g a copy each, so that no two of them meet (where the table's range leaves no room for four
-// copies, one g after the other): the order of all additions is fixed. A wave's sums are folded by bucket at the end of each head.
-// (Measured on 8 x 12 heads, 512 x 512, where half of the tiles are near: by columns of a copy shifted row by row 54 us, by ds_add_f32 134 us.)
+// the next 16 distances), which leaves every lane one distance per 16 x 16 tile; these are added to sums by distance in LDS that every wave has
+// for itself, one row index g after the other, so that no two lanes meet: the order of all additions is fixed. A wave's sums are folded by
+// bucket at the end of each head. (Measured, this kernel on 8 x 12 heads, 512 x 512, where half of the tiles are near: by columns of a copy
+// shifted row by row 54 us, by ds_add_f32 134 us, with a copy of the sums for each g, which costs the third block a CU, 43 us, so 32 us.)
 #include "cb_seq.h"
 #include <algorithm>
 
@@ -49,8 +49,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
     int kend = klen;
     if (a.causal) kend = max(0, min(kend, pos0 + min(qb0 + 64 * QB, qlen)));
     if (qb0 >= qlen) kend = 0;
-    const bool brief = a.Nk <= SEQ_SHORT;
-    const int split = blockIdx.y;                                 // part of the key axis (never where `brief`)
+    const int split = blockIdx.y;                                 // part of the key axis
     int t0 = 0, t1 = (kend + TK - 1) / TK;
     if (a.ksplit > 1) {
         const int per = (t1 + a.ksplit - 1) / a.ksplit;
@@ -74,7 +73,6 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
         for (int s = 0; s < KS; ++s) {
             qf[qb][s] = seq_frag_row<T>(Q + (long)row * a.q.row, valid, s, g, a.d);
             df[qb][s] = seq_frag_row<T>(dO + (long)row * a.dout.row, valid, s, g, a.d);
-            if (brief) continue;
             float x[8], y[8];
             if constexpr (G::ES == 2) {
 #pragma unroll
@@ -97,7 +95,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
 #pragma unroll
             for (int e = 0; e < G::EP; ++e) ds = __builtin_fmaf(x[e], y[e], ds);
         }
-        dsum[qb] = brief ? 0.f : seq_group_sum(ds);
+        dsum[qb] = seq_group_sum(ds);
         own[qb] = 0.f;
     }
     const float scale2 = a.scale * SEQ_L2E;
@@ -111,19 +109,17 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
     sv.init(a.v.row, a.d, tid);
     if constexpr (BIAS) seq_bias_fill(bw, a, h, PAD, tid);
     const int wbase = wave * 1024;
-    auto stage = [&](int u, int t, unsigned long long live) {
-        char* dst = lds_seq + (u & 1) * STAGE + wbase;
+    auto stage = [&](int t, unsigned long long live) {
+        char* dst = lds_seq + (t & 1) * STAGE + wbase;
         sk.dma(K + (long)t * TK * a.k.row, dst, live, tid);
         sv.dma(V + (long)t * TK * a.v.row, dst + G::IMG, live, tid);
     };
     unsigned long long live = 0, next = 0;
-    const int n1 = t1 - t0, u1 = brief ? 2 * n1 : n1;             // steps: the tiles, twice where the first pass makes the row sums
-    auto tile_of = [&](int u) { return t0 + (u < n1 ? u : u - n1); };
     int byte = 0;
-    if (0 < n1) {
+    if (t0 < t1) {
         next = seq_live<TK>(mask, seq_mask_byte<TK>(mask, t0 * TK, klen, lane), t0 * TK, klen);
-        stage(0, t0, next);
-        byte = seq_mask_byte<TK>(mask, tile_of(1) * TK, klen, lane);
+        stage(t0, next);
+        byte = seq_mask_byte<TK>(mask, (t0 + 1) * TK, klen, lane);
     }
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -131,24 +127,18 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
 #pragma unroll
         for (int s = 0; s < KS; ++s) { seq_arrived(qf[qb][s]); seq_arrived(df[qb][s]); }
     }
-    for (int u = 0; u < u1; ++u) {
+    for (int t = t0; t < t1; ++t) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         live = next;
-        const int t = tile_of(u);
-        if (u + 1 < u1) {
-            const int n = tile_of(u + 1);
-            next = seq_live<TK>(mask, byte, n * TK, klen);
-            byte = seq_mask_byte<TK>(mask, tile_of(u + 2) * TK, klen, lane);
-            stage(u + 1, n, next);
-        }
-        if (brief && u == n1) {
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) dsum[qb] = seq_group_sum(own[qb]);
+        if (t + 1 < t1) {
+            next = seq_live<TK>(mask, byte, (t + 1) * TK, klen);
+            byte = seq_mask_byte<TK>(mask, (t + 2) * TK, klen, lane);
+            stage(t + 1, next);
         }
         if (live == 0) continue;
-        const char* Ks = lds_seq + (u & 1) * STAGE;
+        const char* Ks = lds_seq + (t & 1) * STAGE;
         const char* Vs = Ks + G::IMG;
         const int k0 = t * TK, p0 = pos0 + q0;
         f32x4 s[QB][KT], dp[QB][KT];
@@ -217,7 +207,7 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
                     for (int r = 0; r < 4; ++r) s[qb][kt][r] = k0 + 16 * kt + 4 * g + r <= p0 + 16 * qb + l15 ? s[qb][kt][r] : 0.f;
                 }
         }
-        if (brief ? u < n1 : BIAS) {
+        if constexpr (BIAS) {
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
@@ -225,7 +215,6 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
 #pragma unroll
                     for (int r = 0; r < 4; ++r) own[qb] = __builtin_fmaf(s[qb][kt][r], dp[qb][kt][r], own[qb]);
         }
-        if (brief && u < n1) continue;
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
@@ -237,8 +226,8 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
         const int row = q0 + 16 * qb + l15;
-        // brief: dsum is the exact sum (0 where nothing is visible); with a table: the exact sum of this part of the keys; else the one from the output
-        const float D = brief ? (n1 ? dsum[qb] : 0.f) : BIAS ? seq_group_sum(own[qb]) : split == 0 ? dsum[qb] : 0.f;
+        // with a table: the exact sum over this part of the keys; else the one from the output
+        const float D = BIAS ? seq_group_sum(own[qb]) : split == 0 ? dsum[qb] : 0.f;
         if (row >= a.Nq) continue;
         if (g == 0) a.dvec[((long)split * a.B * a.H + bh) * a.Nq + row] = D;
         if (a.ksplit > 1) {
@@ -272,9 +261,9 @@ template <int CTRL> __device__ __forceinline__ float dpp0(float v) {
 template <typename T, int DT, int KB, bool BIAS, bool TAB> struct SeqDkv {
     using G = SeqGeo<T, DT>;
     static constexpr int PAD = G::TK + 16 * KB + 16, NE = KB + G::KT - 1;
-    static int lds(int D, int copies) {
+    static int lds(int D) {
         const int w = 2 * (D + PAD) + 1;
-        return 4 * G::IMG + 4 * G::TK * 4 + (BIAS ? (int)rup(w * 4, 16) : 0) + (TAB ? 4 * copies * w * 4 : 0);
+        return 4 * G::IMG + 4 * G::TK * 4 + (BIAS ? (int)rup(w * 4, 16) : 0) + (TAB ? 4 * w * 4 : 0);
     }
 };
 
@@ -288,7 +277,7 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
     const int W = 2 * (a.D + PAD) + 1;
     float* rows = reinterpret_cast<float*>(lds_seq + 2 * STAGE);      // [2 stages][lse, D][TQ]
     float* bw = rows + 4 * TQ;
-    float* hist = bw + ((W + 3) & ~3);                                // [4 waves][copies][W]
+    float* hist = bw + ((W + 3) & ~3);                                // [4 waves][W]
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kblk = blockIdx.x / (a.B * a.Hkv), bk = blockIdx.x - kblk * (a.B * a.Hkv), b = bk / a.Hkv, hk = bk - b * a.Hkv;   // causal: the long ones first
@@ -356,16 +345,20 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
         // a row without a visible key (or behind the sample's last) has lse = -inf: with +inf in its place its probabilities are zero
         if (tid < TQ) { float* w = rows + (u & 1) * 2 * TQ; w[tid] = ls == -INFINITY ? INFINITY : ls * SEQ_L2E; w[TQ + tid] = dd; }
     };
-    int h = hn, q0 = tn * TQ;
-    if (u0 < u1) { fetch(); stage(u0); put(u0); }
+    int h = hn, q0 = tn * TQ, hcur = -1;
+    if (u0 < u1) {
+        fetch(); stage(u0);
+        if constexpr (BIAS) { seq_bias_fill(bw, a, h, PAD, tid); hcur = h; }
+        put(u0);
+    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int s = 0; s < KS; ++s) { seq_arrived(kf[kb][s]); seq_arrived(vf[kb][s]); }
     float far_l = 0.f, far_r = 0.f;
-    float* hw = hist + wave * a.copies * W;
+    float* hw = hist + wave * W;
     auto clear = [&]() {
-        for (int i = lane; i < a.copies * W; i += 64) hw[i] = 0.f;
+        for (int i = lane; i < W; i += 64) hw[i] = 0.f;
         far_l = far_r = 0.f;
     };
     auto out_of = [&](int h) { return a.tpart + ((((long)b * a.H + h) * a.nsplit + split) * nkb + kblk) * a.nb; };
@@ -377,22 +370,19 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
         if (lane == 0) { hw[0] += far_l; hw[W - 1] += far_r; }
         __syncthreads();
         for (int i = tid; i < W; i += 256) {
-            float x = hist[i];
-            for (int c = 1; c < 4 * a.copies; ++c) x += hist[c * W + i];
-            hist[i] = x;
+            hist[i] = (hist[i] + hist[W + i]) + (hist[2 * W + i] + hist[3 * W + i]);
         }
         __syncthreads();
         float* out = out_of(h);
-        for (int c = wave; c < a.nb; c += 4) {
+        for (int c = tid >> 3; c < a.nb; c += 32) {                  // 8 lanes a bucket
             const int lo = a.brange[2 * c], hi = a.brange[2 * c + 1];           // distances + D of the bucket, [lo, hi)
             float x = 0.f;
             if (lo < hi) {
                 const int i0 = lo == 0 ? 0 : lo + PAD, i1 = hi == 2 * a.D + 1 ? W : hi + PAD;
-                for (int i = i0 + lane; i < i1; i += 64) x += hist[i];
+                for (int i = i0 + (tid & 7); i < i1; i += 8) x += hist[i];
             }
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-            if (lane == 0) out[c] = x;
+            x += __shfl_xor(x, 1, 64); x += __shfl_xor(x, 2, 64); x += __shfl_xor(x, 4, 64);
+            if ((tid & 7) == 0) out[c] = x;
         }
         __syncthreads();
     };
@@ -402,14 +392,13 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
         for (int x = h0; x < h0 + a.G; ++x)                           // heads of the group that this part of the steps does not reach
             if (x < ha || x > hb) for (int c = tid; c < a.nb; c += 256) out_of(x)[c] = 0.f;
     }
-    int hcur = -1;
     for (int u = u0; u < u1; ++u) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         h = hn; q0 = tn * TQ;
         if (BIAS && h != hcur) {
-            if (TAB && hcur >= 0) { fold(hcur); clear(); }
+            if (TAB) { fold(hcur); clear(); }
             seq_bias_fill(bw, a, h, PAD, tid);
             hcur = h;
             __syncthreads();
@@ -514,17 +503,16 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
                     y[e] += x[e][0] + dpp0<0x101>(x[e][1]) + dpp0<0x102>(x[e][2]) + dpp0<0x103>(x[e][3]);          // row_shl: lane l takes lane l + r
                     y[e + 1] = dpp0<0x11F>(x[e][1]) + dpp0<0x11E>(x[e][2]) + dpp0<0x11D>(x[e][3]);                 // row_shr by 16 - r: the lanes below r
                 }
-                float* hb = hw + (k0 - p0 + l15 - 4 * g + a.D + PAD + 16 * (KB - 1)) + (a.copies == 4 ? g * W : 0);
-                auto add = [&]() {
+                float* hb = hw + (k0 - p0 + l15 - 4 * g + a.D + PAD + 16 * (KB - 1));
+                for (int q = 0; q < 4; ++q) {
+                    asm volatile("" ::: "memory");                // one wave's LDS accesses execute in order
+                    if (g != q) continue;
                     float o[NE + 1];
 #pragma unroll
                     for (int e = 0; e <= NE; ++e) o[e] = hb[-16 * e];
 #pragma unroll
                     for (int e = 0; e <= NE; ++e) hb[-16 * e] = o[e] + y[e];
-                };
-                asm volatile("" ::: "memory");
-                if (a.copies == 4) add();
-                else for (int q = 0; q < 4; ++q) { if (g == q) add(); asm volatile("" ::: "memory"); }
+                }
                 asm volatile("" ::: "memory");
             }
         }
@@ -581,11 +569,12 @@ SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable) {
     SeqBwdPlan p;
     const bool wide = a.dt == DT_BF16 && a.d <= 64;                  // what the registers hold for 32 rows a wave
     const long bh = (long)a.B * a.H, bk = (long)a.B * a.Hkv;
-    // measured, 16 against 32 rows a wave. dQ: 8 x 12 heads, 512 x 512 with dtable 45.6 / 39.3 us, 2 x 12 heads, 4096 causal 183 / 148 us; two passes
-    // over 77 keys 38.8 / 41.7 us. dK, dV: 384 blocks of 128 keys (8 x 12 heads, 512) 27.7 / 30.0 us, 768 (2 x 12 heads, 4096) 162 / 154 us
-    p.qb = wide && a.Nk > SEQ_SHORT ? 2 : 1;
+    // measured, 16 against 32 rows a wave, with a table. dQ: 384 blocks of 128 queries (8 x 12 heads, 512 x 512) 24.0 / 27.9 us, 768 (2 x 12 heads, 4096
+    // causal) 128 / 125 us. dK, dV: 384 blocks of 128 keys 31 / 36 us, 768 188 / 173 us
+    p.qb = wide && bh * cdiv(a.Nq, 128) >= 768 ? 2 : 1;
     p.kb = wide && bk * cdiv(a.Nk, 128) >= 768 ? 2 : 1;
     p.nqb = (int)cdiv(a.Nq, 64 * p.qb);
+    const bool brief = seq_short_takes(a);
     p.nkb = (int)cdiv(a.Nk, 64 * p.kb);
     // few blocks of keys (or queries): the other axis is split into runs of at least 4 tiles. 128 blocks (64 heads, 4096 x 77, d 40): 102 us whole,
     // 26 + 5 us in 8 parts
@@ -594,6 +583,7 @@ SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable) {
     p.qsplit = kblocks < 384 && steps >= 8 ? (int)std::min<long>(fill / std::max(kblocks, 1l), steps / 4) : 1;
     const long qblocks = bh * p.nqb, tiles = cdiv(a.Nk, 64);
     p.ksplit = qblocks < 256 && tiles >= 8 && a.Nk > SEQ_SHORT ? (int)std::min<long>(cdiv(512, std::max(qblocks, 1l)), tiles / 4) : 1;
+    if (brief) { p.qb = 0; p.ksplit = 1; }                          // cb_seq_short.hip makes dQ and D
     p.dvec = (size_t)rup((long)p.ksplit * a.B * a.H * a.Nq * 4, 256);
     p.tpart = want_dtable ? (size_t)rup((long)a.B * a.H * p.qsplit * p.nkb * a.nb * 4, 256) : 0;
     p.part = p.qsplit > 1 ? (size_t)rup((long)p.qsplit * 2 * a.B * a.Hkv * a.Nk * a.d * 4, 256) : 0;
@@ -612,14 +602,12 @@ static void dq_go(const Launch& L, const SeqArgs& a, int nqb) {
     CB_HIP(hipGetLastError());
 }
 template <typename T, int DT, int KB, bool BIAS, bool TAB>
-static void dkv_go(const Launch& L, SeqArgs a) {
+static void dkv_go(const Launch& L, const SeqArgs& a) {
     const int nkb = (int)cdiv(a.Nk, 64 * KB);
     if (!((long)nkb * a.B)) return;
     L.count();
     if (L.dry) return;
-    using S = SeqDkv<T, DT, KB, BIAS, TAB>;
-    a.copies = S::lds(a.D, 4) <= 80 * 1024 ? 4 : 1;                  // two blocks a CU
-    const int lds = S::lds(a.D, a.copies);
+    const int lds = SeqDkv<T, DT, KB, BIAS, TAB>::lds(a.D);
     CB_CHECK(lds <= 160 * 1024, CB_ERR_SHAPE, "seq attention: %d bytes of LDS for head dim %d and max_distance %d", lds, a.d, a.D);
     set_dyn_lds(reinterpret_cast<const void*>(&seq_dkv_kernel<T, DT, KB, BIAS, TAB>), 160 * 1024);
     hipLaunchKernelGGL((seq_dkv_kernel<T, DT, KB, BIAS, TAB>), dim3((unsigned)nkb * a.B * a.Hkv, a.nsplit), dim3(256), lds, L.stream, a, nkb);
@@ -639,10 +627,10 @@ static void dkv_kind(const Launch& L, const SeqArgs& a) {
 template <typename T, int DT>
 static void bwd_pick(const Launch& L, const SeqArgs& a, const SeqBwdPlan& p) {
     if constexpr (sizeof(T) == 2 && DT <= 4) {
-        if (p.qb == 2) dq_kind<T, DT, 2>(L, a, p.nqb); else dq_kind<T, DT, 1>(L, a, p.nqb);
+        if (p.qb == 2) dq_kind<T, DT, 2>(L, a, p.nqb); else if (p.qb == 1) dq_kind<T, DT, 1>(L, a, p.nqb);
         if (p.kb == 2) dkv_kind<T, DT, 2>(L, a); else dkv_kind<T, DT, 1>(L, a);
     } else {
-        dq_kind<T, DT, 1>(L, a, p.nqb);
+        if (p.qb) dq_kind<T, DT, 1>(L, a, p.nqb);
         dkv_kind<T, DT, 1>(L, a);
     }
 }
@@ -663,6 +651,7 @@ void seq_backward(const Launch& L, SeqArgs a, void* ws) {
     a.partq = reinterpret_cast<float*>(w);
     a.nsplit = p.qsplit;
     a.ksplit = p.ksplit;
+    if (p.qb == 0) seq_short(L, a, true);
     CB_DT_SWITCH(a.dt, T, SEQ_DT_SWITCH(a.d, DT, bwd_pick<T, DT>(L, a, p)));
     if (a.dtable) {
         L.count();

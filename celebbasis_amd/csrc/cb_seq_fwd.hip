@@ -272,6 +272,7 @@ SeqPlan seq_fwd_plan(const SeqArgs& a) {
     const int tiles = (int)cdiv(a.Nk, 64);
     p.nsplit = blocks < 256 && tiles >= 8 ? (int)std::min<long>(cdiv(512, std::max(blocks, 1l)), tiles / 4) : 1;
     if (token) { p.qb = 0; p.nsplit = seq_token_split(a); }
+    else if (seq_short_takes(a)) { p.qb = -1; p.nsplit = 1; }
     if (p.nsplit > 1) {
         p.part = (size_t)p.nsplit * a.B * a.H * a.Nq * a.d * 4;
         p.ml = (size_t)p.nsplit * a.B * a.H * a.Nq * 2 * 4;
@@ -285,6 +286,7 @@ void seq_forward(const Launch& L, SeqArgs a, void* ws) {
     a.part = static_cast<float*>(ws);
     a.ml = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part);
     if (p.qb == 0) seq_token(L, a);
+    else if (p.qb < 0) seq_short(L, a, false);
     else CB_DT_SWITCH(a.dt, T, SEQ_DT_SWITCH(a.d, DT, fwd_pick<T, DT>(L, a, p.qb)));
     if (a.nsplit > 1) {
         L.count();
