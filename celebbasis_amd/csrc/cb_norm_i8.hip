@@ -173,7 +173,9 @@ __global__ __launch_bounds__(256) void quantize_long_kernel(const RmsArgs a) {
     for (int c = threadIdx.x; c < Cp; c += 256) q[c] = c < C ? (int8_t)i8_of(ld1(x + c), f) : (int8_t)0;
 }
 
-constexpr int RMS_PARTS = 512;                       // blocks of the backward pass, and rows of its partial sums of dgamma
+// blocks of the backward pass, and rows of its partial sums of dgamma. 16384 x 2048 bf16, blocks 512 / 768 / 1024 / 2048: 86 / 67 / 57 / 60 us
+// (57 us: 277 MB at 4.9 TB/s, what a copy reaches) + 5 / 6 / 5 / 8 us for the join; a wave a row instead of a block 80 us at 512
+constexpr int RMS_PARTS = 1024;
 template <typename T, int TPR, int NV, bool VEC>
 __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsArgs a, const int per) {
     __shared__ float sh[4];
@@ -192,11 +194,13 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsArgs a, const int
         const T* hp = static_cast<const T*>(a.h) + row * a.ldh;
         const T* dp = static_cast<const T*>(a.dy) + row * a.lddy;
         const float rstd = a.rstd[row];
-        float h[NV][8], w[NV][8], s = 0.f;
+        const T* dr = a.dres ? static_cast<const T*>(a.dres) + row * a.lddres : nullptr;
+        float h[NV][8], w[NV][8], o[NV][8], s = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             row_ld<T, VEC>(hp, (j * TPR + t) * 8, C, h[j]);
             row_ld<T, VEC>(dp, (j * TPR + t) * 8, C, w[j]);
+            if (dr) row_ld<T, VEC>(dr, (j * TPR + t) * 8, C, o[j]);
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -209,17 +213,14 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsArgs a, const int
             }
         const float m = row_sum<TPR>(s, sh) / (float)C;
         T* dh = static_cast<T*>(a.dh) + row * a.lddh;
-        const T* dr = a.dres ? static_cast<const T*>(a.dres) + row * a.lddres : nullptr;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            float o[8];
-            if (dr) row_ld<T, VEC>(dr, (j * TPR + t) * 8, C, o);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float v = rstd * (w[j][e] - h[j][e] * m);
-                o[e] = dr ? v + o[e] : v;
+                o[j][e] = dr ? v + o[j][e] : v;
             }
-            row_st<T, VEC>(dh, (j * TPR + t) * 8, C, o);
+            row_st<T, VEC>(dh, (j * TPR + t) * 8, C, o[j]);
         }
     }
     if (!a.part) return;
@@ -283,6 +284,16 @@ static bool al16(const void* p, long ld, size_t es) { return (reinterpret_cast<u
         else { constexpr int TPR = 256, NV = 8; __VA_ARGS__; }                                \
     } while (0)
 
+// backward: a wave up to 512 columns, else a block (a row's gradient, norm and gamma parts would take a wave over 200 registers)
+#define RMS_BWD_SHAPE(C, TPR, NV, ...)                                                        \
+    do {                                                                                      \
+        if ((C) <= 512) { constexpr int TPR = 64, NV = 1; __VA_ARGS__; }                      \
+        else if ((C) <= 2048) { constexpr int TPR = 256, NV = 1; __VA_ARGS__; }               \
+        else if ((C) <= 4096) { constexpr int TPR = 256, NV = 2; __VA_ARGS__; }               \
+        else if ((C) <= 8192) { constexpr int TPR = 256, NV = 4; __VA_ARGS__; }               \
+        else { constexpr int TPR = 256, NV = 8; __VA_ARGS__; }                                \
+    } while (0)
+
 template <bool NORM> static void fwd_any(const Launch& L, const RmsArgs& a) {
     const size_t es = dt_size(a.dt);
     const bool vec = a.C % 8 == 0 && al16(a.x, a.ldx, es) && (!a.r || al16(a.r, a.ldr, es)) && (!a.h || al16(a.h, a.ldh, es)) &&
@@ -299,7 +310,7 @@ void k_quantize_rows(const Launch& L, const RmsArgs& a) {
     CB_DT_SWITCH(a.dt, T, RMS_GO((quantize_long_kernel<T>), (unsigned)a.rows, a));
 }
 static int bwd_per(long rows, int C) {                // rows a block: a whole number of passes of its waves
-    const int rpb = C <= 2048 ? 4 : 1;
+    const int rpb = C <= 512 ? 4 : 1;
     return (int)rup((long)cdiv(rows, RMS_PARTS), rpb);
 }
 size_t rmsnorm_bwd_ws_bytes(long rows, int C) { return rows ? (size_t)cdiv(rows, bwd_per(rows, C)) * C * 4 : 0; }
@@ -308,7 +319,7 @@ void k_rmsnorm_bwd(const Launch& L, const RmsArgs& a) {
     const bool vec = a.C % 8 == 0 && al16(a.h, a.ldh, es) && al16(a.dy, a.lddy, es) && al16(a.dh, a.lddh, es) && al16(a.gamma, 0, 4) &&
                      (!a.dres || al16(a.dres, a.lddres, es));
     const int per = bwd_per(a.rows, a.C), n = a.rows ? (int)cdiv(a.rows, per) : 0;
-    if (n) CB_DT_SWITCH(a.dt, T, RMS_SHAPE(a.C, TPR, NV, {
+    if (n) CB_DT_SWITCH(a.dt, T, RMS_BWD_SHAPE(a.C, TPR, NV, {
         if (vec) RMS_GO((rms_bwd_kernel<T, TPR, NV, true>), (unsigned)n, a, per);
         else RMS_GO((rms_bwd_kernel<T, TPR, NV, false>), (unsigned)n, a, per);
     }));

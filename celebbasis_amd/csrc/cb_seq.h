@@ -262,6 +262,15 @@ __device__ __forceinline__ void seq_item(const SeqArgs& a, int id, int& rank, in
     b = bk / a.Hkv;
     h = (bk - b * a.Hkv) * a.G + gi;
 }
+// The same for kernels bound by the rows of Q: the heads of a token lie side by side in memory, and a head of 40 or 80 elements ends inside a
+// 128-byte line, so the blocks of all heads of one (sample, rank) go to one XCD, one after the other. Ids past the last item: false.
+__device__ __forceinline__ bool seq_item_by_row(int B, int H, int ranks, int id, int& rank, int& b, int& h) {
+    const int x = id & 7, y = id >> 3, u = y / H * 8 + x;
+    h = y - y / H * H;
+    rank = u / B; b = u - rank * B;
+    return u < B * ranks;
+}
+inline unsigned seq_grid_by_row(long B, long H, long ranks) { return (unsigned)(cdiv(B * ranks, 8) * 8 * H); }
 #endif  // __HIPCC__
 
 #define SEQ_DT_SWITCH(d, DTC, ...)                                   \

@@ -3,7 +3,7 @@
 // All keys and values of one (sample, head) stay in LDS, and the scores of a row over all of them in registers: the softmax needs no running
 // maximum, and the row sums of the backward pass come from the probabilities in fp32 on the spot (exact; neither output is read). After K and V
 // have arrived once, the waves of a block run by themselves, each over blocks of 16 rows, with the rows of the next block in flight: bound by
-// reading Q (and dO) and writing O (dQ). Measured on 64 heads, 4096 x 77, d 40, bf16 (forward / dQ): tile kernels 27 / 41 us.
+// reading Q (and dO) and writing O (dQ). Measured on 64 heads, 4096 x 77, d 40, bf16 (forward / dQ): tile kernels 27 / 41 us, these 28 / 32.
 #include "cb_seq.h"
 #include <algorithm>
 
@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int rank, b, h;
-    seq_item(a, blockIdx.x, rank, b, h);
+    if (!seq_item_by_row(a.B, a.H, nqb, blockIdx.x, rank, b, h)) return;
     const int bh = b * a.H + h, hk = h / a.G;
     const int qlen = seq_clamp_len(a.q_len, b, a.Nq), klen = seq_clamp_len(a.kv_len, b, a.Nk), pos0 = seq_pos(a.q_pos, b);
     const T* Q = static_cast<const T*>(a.q.p) + b * a.q.batch + h * a.q.head;
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
     // this wave's blocks of 16 rows: rb, rb + 4, ...
     int rb = rank * (4 * turns) + wave;
     const int rb1 = min(rank * (4 * turns) + 4 * turns, (a.Nq + 15) / 16);
-    SeqFrag<T> qf[KS], df[KS], qn[KS], dn[KS];
+    SeqFrag<T> qf[KS], df[KS], qn[KS] = {}, dn[KS] = {};
     float lse = 0.f, lsen = 0.f;
     auto load = [&](int r, SeqFrag<T> (&q)[KS], SeqFrag<T> (&d)[KS], float& ls) {
         const int row = 16 * r + l15;
@@ -76,59 +76,81 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
         if (rb + 4 < rb1) load(rb + 4, qn, dn, lsen);
         const int q0 = 16 * rb, row = q0 + l15, p0 = pos0 + q0;
         f32x4 s[NT][1][KT], dp[NT][KT];
+        // 16 keys at a time; wave-uniform: none of them visible (nothing is computed for them), all, or some
+        auto bits = [&](int t, int kt) { return (unsigned)(live[t] >> (16 * kt)) & 0xffffu; };
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) { s[t][0][kt] = (f32x4){0.f, 0.f, 0.f, 0.f}; dp[t][kt] = s[t][0][kt]; }
-            if (live[t] == 0) continue;
-            const char* Ks = lds_seq + 2 * t * G::IMG;
+            for (int kt = 0; kt < KT; ++kt) {
+                s[t][0][kt] = (f32x4){0.f, 0.f, 0.f, 0.f}; dp[t][kt] = s[t][0][kt];
+                if (!bits(t, kt)) continue;
+                const char* Ks = lds_seq + 2 * t * G::IMG;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) {
+                for (int ks = 0; ks < KS; ++ks) {
                     s[t][0][kt] = seq_mma(seq_frag_lds<T, DT>(Ks, kt, ks, l15, g), qf[ks], s[t][0][kt]);
                     if constexpr (BWD) dp[t][kt] = seq_mma(seq_frag_lds<T, DT>(Ks + G::IMG, kt, ks, l15, g), df[ks], dp[t][kt]);
                 }
-        }
+            }
         // scores in the log2 domain, minus infinity where a key is not visible
+        float m = -INFINITY;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int k0 = t * TK, hi = k0 + TK - 1 - p0, lo = k0 - p0 - 15;
-            const bool far = !BIAS || hi <= -a.D || lo >= a.D;        // wave-uniform: one bias for the whole tile
+            const bool far = !BIAS || hi <= -a.D || lo >= a.D;        // one bias for the whole tile
             const float cb = !BIAS ? 0.f : hi <= -a.D ? bw[PAD] : lo >= a.D ? bw[2 * a.D + PAD] : 0.f;
             const float* w = bw + (far ? 0 : k0 + 4 * g - p0 - l15 + a.D + PAD);
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                const int nib = (int)(unsigned)(live[t] >> (16 * kt + 4 * g));
+                const unsigned bt = bits(t, kt);
+                if (!bt) continue;
+                f32x4& x = s[t][0][kt];
+                if (far) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float x = __builtin_fmaf(s[t][0][kt][r], scale2, far ? cb : w[16 * kt + r]);
-                    const bool ok = ((nib >> r) & 1) && (!a.causal || k0 + 16 * kt + 4 * g + r <= p0 + l15);
-                    s[t][0][kt][r] = ok ? x : -INFINITY;
+                    for (int r = 0; r < 4; ++r) x[r] = __builtin_fmaf(x[r], scale2, cb);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = __builtin_fmaf(x[r], scale2, w[16 * kt + r]);
                 }
+                if (bt != 0xffffu || (a.causal && k0 + 16 * kt + 15 > p0)) {
+                    seq_pin(x);
+                    const unsigned nib = bt >> (4 * g);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool ok = ((nib >> r) & 1) && (!a.causal || k0 + 16 * kt + 4 * g + r <= p0 + l15);
+                        x[r] = ok ? x[r] : -INFINITY;
+                    }
+                }
+                if constexpr (!BWD) m = fmaxf(m, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
             }
         }
         f32x4 o[1][G::DA];
 #pragma unroll
         for (int t = 0; t < G::DA; ++t) o[0][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        // The rows that were fetched for the next turn are waited for before this turn's results are stored: stores count as outstanding memory
+        // operations too, and a wait behind them would last until they are done (measured: forward 30 us with it, 64 heads, 4096 x 77)
+        auto next = [&]() {
+#pragma unroll
+            for (int s2 = 0; s2 < KS; ++s2) {
+                seq_arrived(qn[s2]);
+                qf[s2] = qn[s2];
+                if constexpr (BWD) { seq_arrived(dn[s2]); df[s2] = dn[s2]; }
+            }
+            if constexpr (BWD) { asm volatile("" : "+v"(lsen)); lse = lsen; }
+        };
         const long ri = (long)bh * a.Nq + row;
         if constexpr (!BWD) {
-            float m = -INFINITY, l = 0.f;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) m = fmaxf(m, s[t][0][kt][r]);
+            float l = 0.f;
             m = seq_group_max(m);
             const float off = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
+                    if (!bits(t, kt)) continue;
+                    f32x4& x = s[t][0][kt];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][0][kt][r] = __builtin_amdgcn_exp2f(s[t][0][kt][r] - off);
-                    l += (s[t][0][kt][0] + s[t][0][kt][1]) + (s[t][0][kt][2] + s[t][0][kt][3]);
+                    for (int r = 0; r < 4; ++r) x[r] = __builtin_amdgcn_exp2f(x[r] - off);
+                    l += (x[0] + x[1]) + (x[2] + x[3]);
                 }
                 if (live[t]) seq_tmul<T, DT, 1>(o, lds_seq + (2 * t + 1) * G::IMG, s[t], l15, g);
             }
@@ -136,6 +158,7 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
             if (row >= qlen) l = 0.f;
             const bool none = l == 0.f;
             const float inv = none ? 0.f : 1.f / l;
+            next();
             if (row < a.Nq) {
                 T* O = static_cast<T*>(a.o.p) + b * a.o.batch + h * a.o.head + (long)row * a.o.row;
                 seq_row4<T, DT>(o[0], a.d, g, [&](int c, float4 v) { st4(O + c, make_float4(none ? 0.f : v.x * inv, none ? 0.f : v.y * inv, none ? 0.f : v.z * inv, none ? 0.f : v.w * inv)); });
@@ -147,30 +170,32 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                for (int kt = 0; kt < KT; ++kt) {
+                    if (!bits(t, kt)) continue;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         s[t][0][kt][r] = __builtin_amdgcn_exp2f(s[t][0][kt][r] - ls2);
                         D = __builtin_fmaf(s[t][0][kt][r], dp[t][kt][r], D);
                     }
+                }
             D = seq_group_sum(D);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+                for (int kt = 0; kt < KT; ++kt) {
+                    if (!bits(t, kt)) continue;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[t][0][kt][r] *= dp[t][kt][r] - D;
+                }
                 if (live[t]) seq_tmul<T, DT, 1>(o, lds_seq + 2 * t * G::IMG, s[t], l15, g);
             }
+            next();
             if (row < a.Nq) {
                 if (g == 0) a.dvec[ri] = D;
                 T* dQ = static_cast<T*>(a.dq.p) + b * a.dq.batch + h * a.dq.head + (long)row * a.dq.row;
                 seq_row4<T, DT>(o[0], a.d, g, [&](int c, float4 v) { st4(dQ + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
             }
         }
-#pragma unroll
-        for (int s2 = 0; s2 < KS; ++s2) { qf[s2] = qn[s2]; if constexpr (BWD) df[s2] = dn[s2]; }
-        lse = lsen;
     }
 #endif
 }
@@ -180,15 +205,16 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
 bool seq_short_takes(const SeqArgs& a) { return a.Nk > 0 && a.Nk <= (a.dt == DT_F32 && a.d > 128 ? 64 : SEQ_SHORT); }
 template <typename T, int DT, int NT, bool BWD>
 static void short_go(const Launch& L, const SeqArgs& a) {
-    // blocks of 16 rows a wave: as many as leave 4 blocks (of 4 waves) a CU, at most 8
+    // blocks of 16 rows a wave: as many as leave 2 blocks (of 4 waves) a CU, at most 8. 64 heads, 4096 x 77, forward / dQ: 2 rows of blocks 30 / 40 us,
+    // 4 29 / 36, 8 28 / 32, 16 (one block a CU) 46 / 51
     const long heads = (long)a.B * a.H, rbs = cdiv(a.Nq, 16);
-    const int turns = (int)std::max(1l, std::min<long>(8, heads * rbs / (4 * 1024)));
+    const int turns = (int)std::max(1l, std::min<long>(8, heads * rbs / (4 * 512)));
     const int nqb = (int)cdiv(rbs, 4 * turns);
     if (!(heads * nqb)) return;
     L.count();
     if (L.dry) return;
     const int lds = SeqShort<T, DT, NT>::lds(a.D, a.table != nullptr);
-    const dim3 grid((unsigned)(heads * nqb));
+    const dim3 grid(seq_grid_by_row(a.B, a.H, nqb));
     if (a.table) {
         set_dyn_lds(reinterpret_cast<const void*>(&seq_short_kernel<T, DT, NT, true, BWD>), 160 * 1024);
         hipLaunchKernelGGL((seq_short_kernel<T, DT, NT, true, BWD>), grid, dim3(256), lds, L.stream, a, nqb, turns);
