@@ -1101,6 +1101,18 @@ static SeqT seq_tensor(const cb_seq_tensor& t, const char* what, DType dt, int B
     SeqT r; r.p = t.p; r.row = t.row; r.head = t.head; r.batch = t.batch;
     return r;
 }
+// what is written lies apart from what is read: blocks of one launch, and the kernels of one call, read their inputs at different times
+struct SeqRange { const char* what; uintptr_t lo, hi; };
+static SeqRange seq_range(const char* what, const SeqT& t, DType dt, int B, int N, int H, int d) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t.p);
+    if ((long)B * N * H == 0) return {what, p, p};
+    return {what, p, p + ((size_t)(B - 1) * t.batch + (size_t)(N - 1) * t.row + (size_t)(H - 1) * t.head + d) * dt_size(dt)};
+}
+static void seq_apart(const std::vector<SeqRange>& written, const std::vector<SeqRange>& read) {
+    for (auto& w : written)
+        for (auto& r : read)
+            CB_CHECK(w.lo >= r.hi || r.lo >= w.hi || w.lo == w.hi || r.lo == r.hi, CB_ERR_ARG, "seq attention: %s overlaps %s", w.what, r.what);
+}
 static SeqArgs seq_args(const cb_ctx* ctx, const cb_seq_attention_desc* d, bool bwd, bool pointers) {
     const Ctx& c = ctx->c;
     CB_CHECK(d->struct_size == (int)sizeof(cb_seq_attention_desc), CB_ERR_ARG, "seq attention: desc.struct_size %d != %d — caller built against "
@@ -1140,6 +1152,15 @@ static SeqArgs seq_args(const cb_ctx* ctx, const cb_seq_attention_desc* d, bool 
         a.dk = seq_tensor(d->dk, "dk", a.dt, d->B, d->Nk, d->kv_heads, d->d, true, c.dry);
         a.dv = seq_tensor(d->dv, "dv", a.dt, d->B, d->Nk, d->kv_heads, d->d, true, c.dry);
         if (!c.dry && (long)d->B * d->Nq > 0) require(d->lse, "lse");
+    }
+    auto q_side = [&](const char* what, const SeqT& t) { return seq_range(what, t, a.dt, d->B, d->Nq, d->heads, d->d); };
+    auto k_side = [&](const char* what, const SeqT& t) { return seq_range(what, t, a.dt, d->B, d->Nk, d->kv_heads, d->d); };
+    const std::vector<SeqRange> in = {q_side("q", a.q), k_side("k", a.k), k_side("v", a.v)};
+    if (!bwd) seq_apart({q_side("out", a.o)}, in);
+    else {
+        const std::vector<SeqRange> grads = {q_side("dq", a.dq), k_side("dk", a.dk), k_side("dv", a.dv)};
+        seq_apart(grads, in);
+        seq_apart(grads, {q_side("out", a.o), q_side("dout", a.dout)});
     }
     return a;
 }

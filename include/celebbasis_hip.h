@@ -200,7 +200,9 @@ typedef struct { void* p; int64_t row, head, batch; } cb_seq_tensor; /* [batch][
  * that are not visible are 0. What K, V hold in places hidden by kv_len or kv_mask, and Q, dout in rows beyond q_len, is never used (it may be
  * NaN). A table entry of -inf hides its bucket. A one-token call over a cache: Nq = 1, q_pos[b] = kv_len[b] - 1.
  * kv_heads divides heads; head h reads key / value head h / (heads / kv_heads). d % 8 == 0, d <= 160. Pointers 16-byte aligned, strides
- * multiples of 16 bytes, row strides below 2^22 elements; out, dq, dk, dv must not overlap themselves. Inputs may have stride 0. */
+ * multiples of 16 bytes, row strides below 2^22 elements; out, dq, dk, dv must not overlap themselves, and their address ranges not those of
+ * the inputs (dq, dk and dv may be slices of one buffer). Inputs may have stride 0. The backward call reads the inputs again, lengths and mask
+ * included: they hold what the forward call saw. */
 typedef struct {
     int struct_size;                             /* = sizeof(cb_seq_attention_desc) */
     int dtype;                                   /* cb_dtype of q, k, v, out, dout, dq, dk, dv */

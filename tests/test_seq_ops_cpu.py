@@ -118,15 +118,30 @@ def test_seq_attention_refusals(dry, change, exc):
         lib.seq_attention(ctx, q, k, v, **kw)
 
 
+def test_seq_attention_refuses_results_over_inputs(dry):
+    lib, ctx = dry
+    q, k, v = qkv()
+    with pytest.raises(lib.CBError, match="out overlaps q"):
+        lib.seq_attention(ctx, q, k, v, out=q)
+    out, tape = lib.seq_attention(ctx, q, k, v, need_grad=True)
+    do = torch.zeros_like(out)
+    for kw, what in ((dict(dq=q), "dq overlaps q"), (dict(dk=k), "dk overlaps k"), (dict(dv=k), "dv overlaps k"), (dict(dq=do), "dq overlaps dout"), (dict(dq=out), "dq overlaps out")):
+        with pytest.raises(lib.CBError, match=what):
+            lib.seq_attention_backward(ctx, tape, do, **kw)
+    same = torch.zeros(2, 7, 4, 16)                                   # dk and dv as slices of one buffer
+    lib.seq_attention_backward(ctx, tape, do, dk=same[:, :, :2], dv=same[:, :, 2:])
+
+
 def test_seq_attention_descriptor_refusals(dry):
     """what the Python wrapper cannot express: a foreign struct size, a short or misaligned workspace, gradients of a table that is not there"""
     lib, ctx = dry
     q, k, v = qkv()
     D = lib.SeqAttentionDesc()
     D.B, D.Nq, D.Nk, D.heads, D.kv_heads, D.d, D.scale = 2, 5, 7, 4, 2, 16, 0.25
-    out, lse = torch.zeros_like(q), torch.zeros(2, 4, 5)
+    out, lse, keep = torch.zeros_like(q), torch.zeros(2, 4, 5), []
     D.lse = lse.data_ptr()
-    for x, t in (("q", q), ("k", k), ("v", v), ("out", out), ("dout", out), ("dq", q), ("dk", k), ("dv", v)):
+    for x, t in (("q", q), ("k", k), ("v", v), ("out", out), ("dout", out.clone()), ("dq", q.clone()), ("dk", k.clone()), ("dv", v.clone())):
+        keep.append(t)
         setattr(D, x, lib.SeqTensor(t.data_ptr(), t.stride(1), t.stride(2), t.stride(0)))
     so = lib.load()
     D.struct_size -= 8
