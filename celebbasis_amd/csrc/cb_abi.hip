@@ -1306,7 +1306,8 @@ static GemmI8Args gemm_i8_args(const cb_gemm_i8_desc* d) {
 int cb_gemm_i8_workspace(cb_ctx* ctx, const cb_gemm_i8_desc* d, int64_t* bytes) {
     CB_TRY
     require(ctx, "ctx"); require(d, "desc"); require(bytes, "bytes");
-    *bytes = (int64_t)gemm_i8_ws_bytes(gemm_i8_args(d));
+    const GemmI8Args a = gemm_i8_args(d);
+    *bytes = (int64_t)a.M * a.N == 0 ? 0 : (int64_t)gemm_i8_ws_bytes(a);
     CB_END
 }
 int cb_gemm_i8(cb_ctx* ctx, const cb_gemm_i8_desc* d) {

@@ -247,3 +247,31 @@ def test_rows_and_product_accept_and_refuse(dry):
     assert so.cb_gemm_i8(ctx.h, C.byref(d)) == -3 and b"shorter" in so.cb_last_error()
     d.ldc, d.struct_size = 4, 1
     assert so.cb_gemm_i8(ctx.h, C.byref(d)) == -1
+
+
+@pytest.mark.parametrize("m,n", [(0, 70), (70, 0), (0, 0), (300, 0)])
+def test_product_of_nothing(dry, m, n):
+    """no rows or no outputs: nothing to ask a workspace for, nothing to divide a split by"""
+    lib, ctx = dry
+    k = 8192
+    d = lib.GemmI8Desc()
+    d.M, d.N, d.K, d.lda, d.ldb, d.ldc = m, n, k, k, k, max(n, 1)
+    t = torch.zeros(16, dtype=torch.int32)
+    for name in ("A", "B", "C", "a_scale", "b_scale"):
+        setattr(d, name, t.data_ptr())
+    need = C.c_int64(-1)
+    assert lib.load().cb_gemm_i8_workspace(ctx.h, C.byref(d), C.byref(need)) == 0 and need.value == 0
+    assert lib.load().cb_gemm_i8(ctx.h, C.byref(d)) == 0
+    got = lib.linear_i8(ctx, torch.zeros(m, k, dtype=torch.int8), torch.zeros(m), torch.zeros(n, k, dtype=torch.int8), torch.zeros(n))
+    assert got.shape == (m, n)
+
+
+@pytest.mark.parametrize("b,h,nq,nk", [(0, 4, 9, 9), (2, 4, 0, 9), (2, 4, 9, 0), (2, 4, 0, 0), (2, 4, 1, 0), (0, 4, 1, 300), (2, 4, 300, 0), (2, 4, 0, 300)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_of_nothing(dry, dtype, b, h, nq, nk):
+    """empty samples, queries or keys pass through the plans of both directions"""
+    lib, ctx = dry
+    q, k, v = torch.zeros(b, nq, h, 64, dtype=dtype), torch.zeros(b, nk, 2, 64, dtype=dtype), torch.zeros(b, nk, 2, 64, dtype=dtype)
+    out, tape = lib.seq_attention(ctx, q, k, v, need_grad=True)
+    g = lib.seq_attention_backward(ctx, tape, torch.zeros_like(out))
+    assert out.shape == q.shape and g.dq.shape == q.shape and g.dk.shape == k.shape and g.dv.shape == v.shape
