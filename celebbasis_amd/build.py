@@ -36,7 +36,8 @@ for _src in ("cb_seq_token.hip", "cb_seq_short.hip", "cb_norm_i8.hip", "cb_gemm_
 # (The f2_* attention kernels drain with vmcnt(0) and do not depend on the count: scratch there is reported, not fatal.)
 if os.environ.get("CB_FLASH_ABL"):       # timing ablations of the fp32 attention backward (cb_flash.hip, FL_ABL): results are wrong under them
     EXTRA["cb_flash.hip"] = EXTRA["cb_flash.hip"] + ["-DFL_ABL=" + str(int(os.environ["CB_FLASH_ABL"]))]
-NO_SCRATCH = {"cb_gemm_glds.hip": ("gemm_glds", True), "cb_gemm_bf16_p8.hip": ("gemm_bf16_p8", True), "cb_flash_bf16_v2.hip": ("f2_", False), "cb_gemm_i8.hip": ("gemm_i8_p8", True)}
+NO_SCRATCH = {"cb_gemm_glds.hip": ("gemm_glds", True), "cb_gemm_bf16_p8.hip": ("gemm_bf16_p8", True), "cb_flash_bf16_v2.hip": ("f2_", False)}
+NO_SCRATCH_I8 = {"cb_gemm_i8.hip": ("_p8_", True)}
 
 
 def source_digest():
@@ -137,7 +138,7 @@ def _build_locked(verbose, force):
             print(f"[celebbasis_amd.build] WARNING: {hipcc} rejects {' '.join(extra)}; building {src} without it "
                   "(attention accumulators in AGPR form: correct, a few percent slower)", flush=True)
             extra = []
-        guard, fatal = NO_SCRATCH.get(src, (None, False))
+        guard, fatal = {**NO_SCRATCH, **NO_SCRATCH_I8}.get(src, (None, False))
         if guard:
             extra += ["-Rpass-analysis=kernel-resource-usage"]
         # the RESOLVED flag set is part of the object's cache key
