@@ -389,13 +389,24 @@ static I8Plan i8_plan(const GemmI8Args& a) {
     const long t256 = (long)cdiv(a.M, 256) * cdiv(a.N, 256), t128 = (long)cdiv(a.M, 128) * cdiv(a.N, 128), t64 = (long)cdiv(a.M, 64) * cdiv(a.N, 64);
     const int nk = (int)cdiv(a.K, 128);
     p.per = nk;
-    if (a.M <= 64) { p.kind = I8_FEW; return p; }
-    if (t256 >= 192) { p.kind = I8_256; return p; }
+    // All figures in us, replayed from a graph, weights not in cache. Few tokens: the kernel for them reads the tokens once per 16 weight rows, so it
+    // is taken up to 64 tokens and M N K = 1.5 x 2^30; it / the 64 tile: M N K = 2^26.6 (17 tokens, 2304 x 768) 3.4 / 6.3, 2^29 (32, 4096 x 4096)
+    // 8.8 / 15.3, 2^30 (16, 8192 x 8192) 18.2 / 21.4, 1.5 x 2^30 (16, 24576 x 4096) 28.0 / 30.6, 2^31 (64, 8192 x 4096) 17.8 / 19.7 but (32, 8192 x
+    // 8192) 26.2 / 22.6, 2^32 (64, 4096 x 16384) 50.6 / 27.5
+    if (a.M <= 64 && (long)a.M * a.N * a.K <= 3L << 29) { p.kind = I8_FEW; return p; }
+    // 256 against 128 tiles (us of a call): 128 of them (1024 x 8192 x 4096) 48.4 / 41.1, 160 (2560 x 4096 x 4096) 50.8 / 60.1, 196 (3584 x 3584 x
+    // 4096) 55.0 / 70.4
+    if (t256 >= 160) { p.kind = I8_256; return p; }
+    // 128 against 64 tiles: 192 of them (128 x 24576 x 4096) 68 / 34, 256 (512 x 8192 x 4096) 33.8 / 35.2, (512 x 8192 x 8192) 61 / 66, 384 (256 x 24576
+    // x 4096) 45.6 / 62
     p.kind = t128 >= 256 ? I8_128 : I8_64;
     const long t = p.kind == I8_128 ? t128 : t64;
-    // fewer tiles than half the chip's places: split K into runs of at least 4 k-tiles
-    if (t < 256 && nk >= 8) {
-        p.nsplit = (int)std::min<long>(cdiv(512, t), nk / 4);
+    // fewer tiles than CUs: K is split into runs of at least 8 k-tiles for two blocks a CU. 64 x 4096 x 4096 (64 tiles) whole / 4 runs of 8 / 8 of 4:
+    // 26.0 / 17.9 / 20.9; 64 x 8192 x 8192 (128 tiles) whole / 4 / 8: 50 / 26 / 31. As many 64 tiles as CUs: four runs where K is long (128 x 8192 x 8192
+    // 49 / 38, 256 x 4096 x 16384 88 / 53), none where it is not (128 x 8192 x 4096 25.7 / 28.9)
+    const long runs = t < 256 ? cdiv(512, t) : p.kind == I8_64 && t == 256 && nk >= 64 ? 4 : 1;
+    if (runs > 1 && nk >= 16) {
+        p.nsplit = (int)std::min<long>(runs, nk / 8);
         p.per = (int)cdiv(nk, p.nsplit);
         p.nsplit = (int)cdiv(nk, p.per);
     }

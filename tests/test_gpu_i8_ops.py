@@ -190,6 +190,7 @@ def product64(a, b):
 SIZES = [(1, 1, 16), (1, 64, 64), (2, 7, 48), (3, 2304, 768), (4, 130, 144), (5, 768, 4096), (8, 4100, 128), (15, 33, 80), (16, 512, 2048), (17, 100, 512), (31, 257, 272),
          (32, 64, 16), (33, 1000, 256), (64, 768, 768), (65, 65, 4112), (77, 2304, 768), (128, 128, 128), (129, 127, 144), (200, 1280, 5120), (256, 256, 256),
          (300, 4096, 1024), (513, 515, 528), (616, 768, 768), (1024, 1000, 640), (2000, 333, 96),
+         (48, 2056, 16400), (250, 4090, 8208), (2500, 4100, 64),
          (2050, 2100, 400), (3500, 3600, 16), (3500, 3600, 144), (3500, 3601, 272), (4001, 3307, 528)]
 
 
