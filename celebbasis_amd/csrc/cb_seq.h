@@ -84,7 +84,7 @@ __device__ __forceinline__ f32x4 seq_mma(const SeqFrag<float>& a, const SeqFrag<
 }
 
 // Waits for a fragment's load here. Without it the compiler puts that wait at the fragment's first use, inside the tile loop, where it also waits
-// for the LDS-DMA of the next tile that has just been issued: every tile then pays the memory latency (measured: forward 114 -> see cb_seq_fwd.hip).
+// for the LDS-DMA of the next tile that has just been issued: every tile then pays the memory latency (2 x 12 heads, 4096 causal, d 64: forward 114 against 110 us).
 template <typename T> __device__ __forceinline__ void seq_arrived(SeqFrag<T>& f) { asm volatile("" : "+v"(f.v)); }
 // Geometry of one instantiation. A tile is TK rows in LDS, row-major, P pieces of 16 bytes a row, filled by LDS-DMA in lane-linear slots of
 // 256 pieces; piece c of row r lies at place swz(c, r), which puts the 16 rows that a fragment read touches into 16 different bank groups.

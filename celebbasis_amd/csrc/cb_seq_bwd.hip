@@ -16,6 +16,9 @@
 // for itself, one row index g after the other, so that no two lanes meet: the order of all additions is fixed. A wave's sums are folded by
 // bucket at the end of each head. (Measured, this kernel on 8 x 12 heads, 512 x 512, where half of the tiles are near: by columns of a copy
 // shifted row by row 54 us, by ds_add_f32 134 us, with a copy of the sums for each g, which costs the third block a CU, 43 us, so 32 us.)
+// What bounds them: vector instructions, as in the forward pass, and with 32 rows a wave two waves a SIMD to hide everything else. 2 x 12 heads, 4096
+// causal, d 64, bf16, with bias and dtable: dQ 113 - 124 us, dK/dV 166 us (scores and dP formed in both: 180 GFLOP, 0.63 PFLOP/s); fp32, 16 heads, 1023 x 333, d 80: 37 and 54 us
+// (6.1 GFLOP for both, 40 us at the rate of a large fp32 product).
 #include "cb_seq.h"
 #include <algorithm>
 

@@ -264,10 +264,11 @@ SeqPlan seq_fwd_plan(const SeqArgs& a) {
     SeqPlan p;
     const long bh = (long)a.B * a.H;
     const bool token = seq_token_takes(a);
-    // measured, 16 against 32 queries a wave: 768 / 384 blocks (8 x 12 heads, 512 x 512, d 64) 22.4 / 25.6 us; 2048 blocks (64 heads, 4096 x 77, d 40)
-    // 24.3 / 22.0 us; 512 blocks (64 heads, 1024 x 2000, d 128) 127 / 90 us
+    // measured, 16 against 32 queries a wave: 384 blocks of 128 queries (8 x 12 heads, 512 x 512, d 64) 22.4 / 25.6 us, 768 (2 x 12 heads, 4096 causal)
+    // 100 / 90 us, 512 (64 heads, 1024 x 2000, d 128) 124 / 90 us
     p.qb = fwd_two(a) && bh * cdiv(a.Nq, 128) >= 512 ? 2 : 1;
-    // fewer blocks than CUs: the key axis is split into runs of at least 4 tiles, joined by seq_combine_kernel
+    // fewer blocks than CUs: the key axis is split into runs of at least 4 tiles, joined by seq_combine_kernel (with as many blocks as CUs it does not
+    // pay: 16 heads, 1023 x 333, fp32, 29 us whole, 27 + 5 us in two parts)
     const long blocks = bh * cdiv(a.Nq, 64 * p.qb);
     const int tiles = (int)cdiv(a.Nk, 64);
     p.nsplit = blocks < 256 && tiles >= 8 ? (int)std::min<long>(cdiv(512, std::max(blocks, 1l)), tiles / 4) : 1;
