@@ -1121,7 +1121,7 @@ static SeqArgs seq_args(const cb_ctx* ctx, const cb_seq_attention_desc* d, bool 
     CB_CHECK(d->B >= 0 && d->Nq >= 0 && d->Nk >= 0 && d->heads >= 1 && d->kv_heads >= 1 && d->heads % d->kv_heads == 0, CB_ERR_SHAPE,
              "seq attention: B = %d, Nq = %d, Nk = %d, heads = %d, kv_heads = %d", d->B, d->Nq, d->Nk, d->heads, d->kv_heads);
     CB_CHECK(d->Nq <= (1 << 24) && d->Nk <= (1 << 24), CB_ERR_SHAPE, "seq attention: at most 2^24 tokens (Nq = %d, Nk = %d)", d->Nq, d->Nk);
-    CB_CHECK((int64_t)d->B * d->heads <= (1 << 20) && (int64_t)d->B * d->heads * cdiv(std::max(d->Nq, d->Nk), 64) < (1ll << 31), CB_ERR_SHAPE,
+    CB_CHECK((int64_t)d->B * d->heads <= (1 << 20) && (int64_t)d->B * d->heads * cdiv(std::max(d->Nq, d->Nk), 64) < (1ll << 24), CB_ERR_SHAPE,
              "seq attention: B * heads = %ld with %d tokens is too large for one call", (long)d->B * d->heads, std::max(d->Nq, d->Nk));
     CB_CHECK(d->d >= 8 && d->d % 8 == 0 && d->d <= SEQ_MAX_D, CB_ERR_SHAPE, "seq attention: head dim %d (a multiple of 8, at most %d)", d->d, SEQ_MAX_D);
     CB_CHECK(d->scale > 0.f && std::isfinite(d->scale), CB_ERR_ARG, "seq attention: scale = %g must be positive and finite", (double)d->scale);

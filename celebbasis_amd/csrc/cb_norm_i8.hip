@@ -295,7 +295,7 @@ static bool al16(const void* p, long ld, size_t es) { return (reinterpret_cast<u
         else { constexpr int TPR = 256, NV = 8; __VA_ARGS__; }                                \
     } while (0)
 
-template <bool NORM> static void fwd_any(const Launch& L, const RmsArgs& a) {
+template <bool NORM> static void fwd_rows(const Launch& L, const RmsArgs& a) {
     const size_t es = dt_size(a.dt);
     const bool vec = a.C % 8 == 0 && al16(a.x, a.ldx, es) && (!a.r || al16(a.r, a.ldr, es)) && (!a.h || al16(a.h, a.ldh, es)) &&
                      (!a.y || al16(a.y, a.ldy, es)) && (!NORM || al16(a.gamma, 0, 4));
@@ -305,10 +305,28 @@ template <bool NORM> static void fwd_any(const Launch& L, const RmsArgs& a) {
         else RMS_GO((rms_fwd_kernel<T, TPR, NV, false, NORM>), grid, a);
     }));
 }
-void k_rmsnorm_fwd(const Launch& L, const RmsArgs& a) { fwd_any<true>(L, a); }
+// a launch holds fewer than 2^32 threads a dimension: more rows than 2^23 go in several
+template <typename F> static void by_rows(const RmsArgs& a, F&& f) {
+    const long most = 1l << 23, es = (long)dt_size(a.dt);
+    for (long r0 = 0; r0 < a.rows; r0 += most) {
+        RmsArgs b = a;
+        b.rows = std::min(most, a.rows - r0);
+        b.x = static_cast<const char*>(a.x) + r0 * a.ldx * es;
+        if (a.r) b.r = static_cast<const char*>(a.r) + r0 * a.ldr * es;
+        if (a.h) b.h = static_cast<char*>(a.h) + r0 * a.ldh * es;
+        if (a.y) b.y = static_cast<char*>(a.y) + r0 * a.ldy * es;
+        if (a.q) b.q = a.q + r0 * a.ldq;
+        if (a.scale) b.scale = a.scale + r0;
+        if (a.rstd) b.rstd = a.rstd + r0;
+        f(b);
+    }
+}
+void k_rmsnorm_fwd(const Launch& L, const RmsArgs& a) { by_rows(a, [&](const RmsArgs& b) { fwd_rows<true>(L, b); }); }
 void k_quantize_rows(const Launch& L, const RmsArgs& a) {
-    if (a.C <= RMS_MAX_C) { fwd_any<false>(L, a); return; }
-    CB_DT_SWITCH(a.dt, T, RMS_GO((quantize_long_kernel<T>), (unsigned)a.rows, a));
+    by_rows(a, [&](const RmsArgs& b) {
+        if (b.C <= RMS_MAX_C) fwd_rows<false>(L, b);
+        else CB_DT_SWITCH(b.dt, T, RMS_GO((quantize_long_kernel<T>), (unsigned)b.rows, b));
+    });
 }
 static int bwd_per(long rows, int C) {                // rows a block: a whole number of passes of its waves
     const int rpb = C <= 512 ? 4 : 1;

@@ -204,6 +204,23 @@ def test_product_is_exact(cb, M, N, K):
     assert torch.equal(got.double(), want.float().double())               # one rounding of the whole number to fp32
 
 
+def test_more_rows_than_a_launch_holds(cb):
+    """17 million rows of 8 elements, a wave each: the first, the last and those around 2^23 and 2^24"""
+    lib, ctx = cb
+    n, c = (1 << 24) + 5, 8
+    x = torch.empty(n, c, dtype=torch.bfloat16, device=_dev())
+    at = torch.tensor([0, 1, (1 << 23) - 1, 1 << 23, (1 << 23) + 1, (1 << 24) - 1, 1 << 24, n - 1], device=_dev())
+    x.fill_(1.0)
+    x[at] = rnd(len(at), c, seed=9, dtype=torch.bfloat16)
+    g = rnd(c, seed=10)
+    few = lib.rms_norm(ctx, x[at].contiguous(), g, residual=x[at].contiguous(), need_grad=True)
+    all_ = lib.rms_norm(ctx, x, g, residual=x, need_grad=True)
+    assert torch.equal(all_.y[at], few.y) and torch.equal(all_.h[at], few.h) and torch.equal(all_.rstd[at], few.rstd)
+    q, s = lib.quantize_rows(ctx, x)
+    q0, s0 = lib.quantize_rows(ctx, x[at].contiguous())
+    assert torch.equal(q[at], q0) and torch.equal(s[at], s0)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_product_epilogue(cb, dtype, M, N, K):
@@ -217,6 +234,21 @@ def test_product_epilogue(cb, dtype, M, N, K):
     bnd = 4 * U * (v.abs() + bias.double().abs() + res.double().abs())
     within("C", got, want, bnd + rt(got.dtype) * (want.abs() + bnd))
     assert torch.equal(got, lib.linear_i8(ctx, a, sa, b, sb, bias=bias, residual=res, dtype=dtype))
+
+
+@pytest.mark.parametrize("M,N", [(40, 300), (300, 80), (300, 40000)])
+def test_product_offsets_past_31_bits(cb, M, N):
+    """300 rows that lie 2^23 - 16 bytes apart: the same numbers as in a small buffer"""
+    lib, ctx = cb
+    a, b = i8(M, 128, seed=5), i8(N, 128, seed=6)
+    one = torch.ones(max(M, N), device=_dev())
+    want = lib.linear_i8(ctx, a, one[:M], b, one[:N], dtype="f32")
+    far = torch.empty(300, (1 << 23) - 16, dtype=torch.int8, device=_dev())
+    if M == 300:
+        a = far[:, :128].copy_(a)
+    else:
+        b = far[:, :128].copy_(b)
+    assert torch.equal(lib.linear_i8(ctx, a, one[:M], b, one[:N], dtype="f32"), want)
 
 
 def test_product_largest_sum_and_strides(cb):
