@@ -338,6 +338,26 @@ def test_strides_and_fused_buffers(cb, dtype):
     assert torch.equal(lib.seq_attention(ctx, *one), lib.seq_attention(ctx, *[x.contiguous() for x in one]))
 
 
+@pytest.mark.parametrize("Nq", [1, 70])
+def test_offsets_past_32_bits(cb, Nq):
+    """keys, values and their gradients of one sample 5 GB apart: the same numbers as in a small buffer"""
+    lib, ctx = cb
+    N, H, d, row = 5000, 2, 64, 1 << 19
+    far = torch.empty(N, row, dtype=torch.bfloat16, device=_dev())
+    view = lambda buf, at: buf[:, at:at + H * d].unflatten(1, (H, d))[None]
+    q, k, v = rnd(1, Nq, H, d, dtype=torch.bfloat16), rnd(1, N, H, d, seed=1, dtype=torch.bfloat16), rnd(1, N, H, d, seed=2, dtype=torch.bfloat16)
+    kf, vf = view(far, 0), view(far, 1024)
+    kf.copy_(k); vf.copy_(v)
+    do = rnd(1, Nq, H, d, seed=3, dtype=torch.bfloat16)
+    want, t0 = lib.seq_attention(ctx, q, k, v, need_grad=True)
+    got, t1 = lib.seq_attention(ctx, q, kf, vf, need_grad=True)
+    assert torch.equal(want, got)
+    g0 = lib.seq_attention_backward(ctx, t0, do)
+    grad = torch.empty(N, row, dtype=torch.bfloat16, device=_dev())
+    g1 = lib.seq_attention_backward(ctx, t1, do, dk=view(grad, 512), dv=view(grad, 4096))
+    assert torch.equal(g0.dq, g1.dq) and torch.equal(g0.dk, view(grad, 512)) and torch.equal(g0.dv, view(grad, 4096))
+
+
 @DT
 def test_one_token_over_a_cache(cb, dtype):
     check(cb, dtype, 6, 1, 700, 4, 2, 64, rel=(32, 128, False), causal=True, kv_len=[700, 1, 129, 640, 0, 333], q_pos=[699, 0, 128, 639, -1, 332], grad=False)
