@@ -59,6 +59,8 @@ typedef __attribute__((address_space(3))) void* lds_vp;
 typedef __attribute__((address_space(3))) s16x4* lds_s4;
 
 constexpr float SEQ_L2E = 1.4426950408889634f, SEQ_LN2 = 0.6931471805599453f;
+// log2 magnitudes from here on share fp32's 24 bits with what they are added to (a half step of 2^12 is 2^-12): kept apart from it
+constexpr float SEQ_BIG = 4096.f;
 constexpr int SEQ_OOB = -16;                       // 0xFFFFFFF0 >= num_records: the load returns zeros
 template <int TK> constexpr unsigned long long SEQ_ALL = TK == 64 ? ~0ull : 0xFFFFFFFFull;      // every row of a tile is visible
 // at the head of a rarely taken, wave-uniform branch: keeps its work on x inside (the compiler would turn it into selects that every tile executes)
@@ -238,6 +240,11 @@ __device__ __forceinline__ float seq_bias_of(const SeqArgs& a, int h, int rel) {
 __device__ __forceinline__ void seq_bias_fill(float* bw, const SeqArgs& a, int h, int pad, int tid) {
     const int n = 2 * (a.D + pad) + 1;
     for (int i = tid; i < n; i += 256) bw[i] = seq_bias_of(a, h, min(max(i - (a.D + pad), -a.D), a.D));
+}
+// Distance from which a tile's bias is one number that is added behind the maximum of its scores: the table's range, or none where a number at
+// its ends is -inf (which hides the tile) or too large to be held in fp32 together with a score: there the maximum has to be that of the rounded sums.
+__device__ __forceinline__ int seq_bias_far(const SeqArgs& a, int h) {
+    return __builtin_amdgcn_readfirstlane(fabsf(seq_bias_of(a, h, -a.D)) < SEQ_BIG && fabsf(seq_bias_of(a, h, a.D)) < SEQ_BIG ? a.D : 1 << 30);
 }
 // Visible rows of a tile as a bit mask (wave-uniform): rows at or beyond `len` and rows that the key mask hides are clear. The mask's byte of this
 // lane's row is fetched a tile ahead (seq_mask_byte), so that its latency is not paid between two tiles.

@@ -58,7 +58,11 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
     SeqSlots<T, DT> sk, sv;
     sk.init(a.k.row, a.d, tid);
     sv.init(a.v.row, a.d, tid);
-    if constexpr (BIAS) seq_bias_fill(bw, a, h, PAD, tid);
+    int far = 0;
+    if constexpr (BIAS) {
+        seq_bias_fill(bw, a, h, PAD, tid);
+        far = seq_bias_far(a, h);
+    }
     const int wbase = wave * 1024;
     auto stage = [&](int t, unsigned long long live) {
         char* dst = lds_seq + (t & 1) * STAGE + wbase;
@@ -105,15 +109,16 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
                 for (int qb = 0; qb < QB; ++qb) s[qb][kt] = seq_mma(kf, qf[qb][ks], s[qb][kt]);
             }
         // the bias: one number for the whole tile where every distance is past the table's range, else by distance from LDS; s is then in the
-        // log2 domain already (sc = 1)
+        // log2 domain already (sc = 1). (Tiles past the range that come here all the same are moved to where bw holds that number throughout.)
         const int p0 = pos0 + q0;
         float cb = 0.f, sc = scale2;
         if constexpr (BIAS) {
             const int hi = k0 + TK - 1 - p0, lo = k0 - p0 - (16 * QB - 1);
-            if (hi <= -a.D) cb = bw[PAD];
-            else if (lo >= a.D) cb = bw[2 * a.D + PAD];
+            if (hi <= -far) cb = bw[PAD];
+            else if (lo >= far) cb = bw[2 * a.D + PAD];
             else {
-                const float* w = bw + (k0 + 4 * g - p0 - l15 + a.D + PAD);
+                const int at = min(max(k0 - p0, -(a.D + TK - 1)), a.D + 16 * QB - 1);
+                const float* w = bw + (at + 4 * g - l15 + a.D + PAD);
                 sc = 1.f;
 #pragma unroll
                 for (int qb = 0; qb < QB; ++qb)

@@ -1,0 +1,156 @@
+"""GPU tests of the sequence attention at the edges of its definition: table entries of -inf and of very large magnitude over whole key tiles.
+
+Bounds as in test_gpu_seq_ops.py (u = 2^-24, r = 2^-8 for bf16 operands and results). A table entry b of magnitude 1e8 and more takes every score
+|s| < ulp(b) / 2 up whole: s + b rounds to b, so all keys of such entries weigh alike; against keys of ordinary entries their weight is 0 exactly. What is
+left of a probability's error is that of the ordinary scores (2 (d + 8) u of their magnitude), of a logarithm of at most 16 (2^-20 before the
+exponential, ln 2 2^-20 behind it) and of the exponentials: 2^-19 in all."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_seq_ops import BF, F, R, U, buckets, rnd, within
+
+pytestmark = pytest.mark.gpu
+DT = pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["f32", "bf16"])
+LOWEST = torch.finfo(torch.float32).min
+
+
+def _dev():
+    return torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module")
+def cb(built_lib):
+    from celebbasis_amd import lib
+    ctx = lib.Context()
+    yield lib, ctx
+    ctx.sync()
+
+
+T = lambda x: x.transpose(-1, -2).contiguous()  # noqa: E731
+
+
+def check_table(cb, dtype, B, Nq, Nk, H, d, rel, table, causal=False, q_pos=None, kv_mask=None, scale=None, amp=1.0, seed=0, grad=True):
+    """forward and backward with the given table against 64 bits (one key head a query head)"""
+    lib, ctx = cb
+    dev = _dev()
+    q, k = rnd(B, Nq, H, d, seed=seed, dtype=dtype, scale=amp), rnd(B, Nk, H, d, seed=seed + 1, dtype=dtype, scale=amp)
+    v, do = rnd(B, Nk, H, d, seed=seed + 2, dtype=dtype), rnd(B, Nq, H, d, seed=seed + 3, dtype=dtype)
+    scale = d ** -0.5 if scale is None else scale
+    pos32 = torch.tensor(q_pos, dtype=torch.int32, device=dev) if q_pos is not None else None
+    rp = lib.RelPos(ctx, *rel)
+    nb, D, two = rel
+    i, j = torch.arange(Nq, device=dev), torch.arange(Nk, device=dev)
+    at = (i[None] + (pos32.long()[:, None] if pos32 is not None else 0)).expand(B, Nq)
+    dist = j[None, None] - at[:, :, None]
+    ok = torch.ones(B, Nq, Nk, dtype=torch.bool, device=dev)
+    if causal:
+        ok &= dist <= 0
+    if kv_mask is not None:
+        ok &= kv_mask[:, None]
+    bk = buckets(dist, nb, D, two)
+    bias = table.double()[bk].permute(0, 3, 1, 2)
+    q64, k64, v64, do64 = (x.double().transpose(1, 2).contiguous() for x in (q, k, v, do))
+    s = torch.matmul(q64, T(k64)) * scale
+    mag = torch.matmul(q64.abs(), T(k64.abs())) * scale + bias.abs()
+    huge = bias.abs() >= 1e8                                             # -inf among them
+    s = torch.where(huge, bias, s + bias).masked_fill(~ok[:, None], -math.inf)
+    top = s.amax(-1, keepdim=True)
+    e = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
+    tot = e.sum(-1, keepdim=True)
+    p = torch.where(tot > 0, e / tot, 0.0)
+    none = (tot == 0)[..., 0]                                            # rows that see nothing
+    plain = ok[:, None] & ~huge
+    eP = 2 * (d + 8) * U * (float(mag[plain].max()) if plain.any() else 0.0) + 2.0 ** -19
+    r, rT = (R, R) if dtype == BF else (0.0, U)
+    vis = ok[:, None].double().expand_as(p)
+    o = torch.matmul(p, v64)
+    ob = (eP + (Nk + 4) * U + r) * torch.matmul(p, v64.abs()) + F * torch.matmul(vis, v64.abs() + 1)
+    ob = ob + rT * (o.abs() + ob)
+    dp = torch.matmul(do64, T(v64))
+    Dr = (do64 * o).sum(-1, keepdim=True)
+    ds = p * (dp - Dr)
+    e_dp = (d + 2) * U * torch.matmul(do64.abs(), T(v64.abs()))
+    e_D = (do64.abs() * ((d + 2) * U * o.abs() + ob)).sum(-1, keepdim=True)
+    bs = p * (eP * (dp.abs() + Dr.abs()) + e_dp + e_D) + 4 * U * ds.abs() + F * vis * (dp.abs() + Dr.abs() + 1)
+    a = ds.abs()
+    dq = torch.matmul(ds, k64) * scale
+    dqb = scale * torch.matmul(bs + (r + (Nk + 4) * U) * (a + bs) + F * vis, k64.abs() + 1)
+    dk = torch.matmul(T(ds), q64) * scale
+    dkb = scale * torch.matmul(T(bs + (r + (Nq + 4) * U) * (a + bs) + F * vis), q64.abs() + 1)
+    dv = torch.matmul(T(p), do64)
+    dvb = torch.matmul(T(p * (eP + r + (Nq + 4) * U) + F * vis), do64.abs() + 1)
+
+    out, tape = lib.seq_attention(ctx, q, k, v, scale=scale, causal=causal, q_pos=pos32, kv_mask=kv_mask, relpos=rp, table=table, need_grad=True)
+    heads = lambda x: x.transpose(1, 2)                                   # noqa: E731
+    within("out", out, heads(o), heads(ob))
+    assert not heads(out)[none].any() and (tape.lse[none] == -math.inf).all() and torch.isfinite(tape.lse[~none]).all()
+    bare = lib.seq_attention(ctx, q, k, v, scale=scale, causal=causal, q_pos=pos32, kv_mask=kv_mask, relpos=rp, table=table)
+    assert torch.equal(bare, out)
+    if not grad:
+        return
+    g = lib.seq_attention_backward(ctx, tape, do)
+    for name, got, want, bnd in (("dq", g.dq, dq, dqb), ("dk", g.dk, dk, dkb), ("dv", g.dv, dv, dvb)):
+        within(name, got, heads(want), heads(bnd + rT * (want.abs() + bnd)))
+    hot = torch.nn.functional.one_hot(bk, nb).double().reshape(-1, nb).t().contiguous()
+    by_bucket = lambda x: torch.matmul(hot, x.permute(0, 2, 3, 1).reshape(-1, H).contiguous())      # noqa: E731
+    within("dtable", g.dtable, by_bucket(ds), by_bucket(bs) + (4096 + 64) * U * by_bucket(a) + F)
+    assert not heads(g.dq)[none].any()
+    again = lib.seq_attention_backward(ctx, tape, do)
+    assert all(torch.equal(getattr(g, n), getattr(again, n)) for n in ("dq", "dk", "dv", "dtable"))
+
+
+def _table(rel, H, value, which, seed=7):
+    """a random table whose outermost buckets, or all of them, hold `value`"""
+    nb, _, two = rel
+    t = rnd(nb, H, seed=seed)
+    if which == "all":
+        t[:] = value
+    else:
+        t[nb // 2 - 1 if two else nb - 1] = value
+        if two:
+            t[nb - 1] = value
+    return t
+
+
+# keys in one short tile run, over tiles whole, over tiles split, and with 32 rows a wave (bf16)
+SHAPES = [(2, 90, 100, 2), (2, 90, 200, 2), (1, 100, 700, 2), (8, 700, 700, 12)]
+
+
+@DT
+@pytest.mark.parametrize("value", [-math.inf, LOWEST, -1e9])
+@pytest.mark.parametrize("B,Nq,Nk,H", SHAPES)
+def test_outermost_bucket_hidden(cb, dtype, value, B, Nq, Nk, H):
+    """a window: keys past the table's range carry -inf (or next to nothing) while near ones are ordinary; small and large scores"""
+    for rel, causal in (((32, 64, True), False), ((32, 64, False), True)):
+        t = _table(rel, H, value, "outer")
+        check_table(cb, dtype, B, Nq, Nk, H, 64, rel, t, causal=causal, grad=value == -math.inf)
+        if value != -1e9:                      # (scores of hundreds are not absorbed by 1e9)
+            check_table(cb, dtype, B, Nq, Nk, H, 64, rel, t, causal=causal, amp=6.0, scale=1.0, grad=value == -math.inf)
+
+
+@DT
+@pytest.mark.parametrize("value", [-math.inf, LOWEST, -1e9])
+def test_rows_that_see_only_hidden_buckets(cb, dtype, value):
+    """queries far from every key, and a key mask that leaves far keys alone"""
+    rel = (32, 64, True)
+    t = _table(rel, 2, value, "outer")
+    for Nk in (100, 200, 700):
+        check_table(cb, dtype, 4, 70, Nk, 2, 64, rel, t, q_pos=[0, 2000, -2000, 300], grad=value == -math.inf)
+        m = torch.zeros(2, Nk, dtype=torch.bool, device=_dev())
+        m[:, Nk - 20:] = True
+        check_table(cb, dtype, 2, Nk - 10, Nk, 2, 64, rel, t, kv_mask=m, grad=value == -math.inf)
+    check_table(cb, dtype, 16, 520, 700, 16, 40, rel, _table(rel, 16, value, "outer"), q_pos=[1500] * 8 + [0] * 8, grad=value == -math.inf)
+
+
+@DT
+@pytest.mark.parametrize("value", [LOWEST, -1e30, -1e9, 1e9, -math.inf])
+@pytest.mark.parametrize("B,Nq,Nk,H", SHAPES)
+def test_every_bucket_alike(cb, dtype, value, B, Nq, Nk, H):
+    """all entries take the scores up whole: every visible key weighs the same"""
+    rel, g = (32, 64, True), value == -math.inf
+    check_table(cb, dtype, B, Nq, Nk, H, 64, rel, _table(rel, H, value, "all"), grad=g)
+    check_table(cb, dtype, B, Nq, Nk, H, 40, (16, 700, False), _table((16, 700, False), H, value, "all"), causal=True, grad=g)
+    if abs(value) != 1e9:
+        check_table(cb, dtype, B, Nq, Nk, H, 64, rel, _table(rel, H, value, "all"), amp=6.0, scale=1.0, grad=g)
