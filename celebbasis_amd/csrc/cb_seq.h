@@ -29,6 +29,7 @@ struct SeqArgs {
     // backward
     SeqT dout, dq, dk, dv;
     float* dvec = nullptr;                                                    // [ksplit][B][H][Nq]: row sums D (parts of them where keys are split)
+    float* stat = nullptr;                                                    // [2][B][H][Nq]: what the exponents of a row are taken off, and log2 of the sum where that is not in it (seq_row_stats)
     float* dtable = nullptr;                                                  // [nb][H]
     float* tpart = nullptr;                                                   // [B][H][parts of queries][blocks of keys][nb]
     float* part = nullptr; float* ml = nullptr; int nsplit = 1;               // partial results of a split axis (fp32): keys (forward), queries (dK, dV)
@@ -36,7 +37,7 @@ struct SeqArgs {
 };
 
 struct SeqPlan { int qb = 1, nsplit = 1; size_t part = 0, ml = 0, total = 0; };           // sizes in bytes
-struct SeqBwdPlan { int qb = 1, kb = 1, qsplit = 1, ksplit = 1, nqb = 1, nkb = 1; size_t dvec = 0, tpart = 0, part = 0, partq = 0, total = 0; };
+struct SeqBwdPlan { int qb = 1, kb = 1, qsplit = 1, ksplit = 1, nqb = 1, nkb = 1; size_t dvec = 0, stat = 0, tpart = 0, part = 0, partq = 0, total = 0; };
 SeqPlan seq_fwd_plan(const SeqArgs& a);
 SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable);
 void seq_forward(const Launch& L, SeqArgs a, void* ws);
@@ -245,6 +246,38 @@ __device__ __forceinline__ void seq_bias_fill(float* bw, const SeqArgs& a, int h
 // its ends is -inf (which hides the tile) or too large to be held in fp32 together with a score: there the maximum has to be that of the rounded sums.
 __device__ __forceinline__ int seq_bias_far(const SeqArgs& a, int h) {
     return __builtin_amdgcn_readfirstlane(fabsf(seq_bias_of(a, h, -a.D)) < SEQ_BIG && fabsf(seq_bias_of(a, h, a.D)) < SEQ_BIG ? a.D : 1 << 30);
+}
+// Statistics of rows in the backward pass. p = exp2(x - lse) needs lse = m + log2(l) to a fraction of one; where the row's maximum m is large (a table's
+// lowest values, very large scores) fp32 drops log2(l) beside it, and p would be n times too large for n equal keys. For such rows the maximum and
+// log2 of the sum are made anew, once, from the scores as the tile loops round them, and kept as two numbers: p = exp2((x - m) - log2 l).
+__device__ __forceinline__ bool seq_row_big(float lse2) { return fabsf(lse2) >= SEQ_BIG && lse2 != INFINITY; }
+// (x - m) - lg, with x - m held to what a maximum leaves; NaN stays
+__device__ __forceinline__ float seq_exponent(float x, float m, float lg) { const float y = x - m; return (y > 0.f ? 0.f : y) - lg; }
+// m and lg of the 16 rows that a wave holds in qf (row l15 at position p0 + l15), over the keys below kend; straight from memory: a rare path
+template <typename T, int KS, bool BIAS>
+__device__ __forceinline__ void seq_row_stats(const SeqArgs& a, const T* K, const unsigned char* mask, int kend, int h, int p0, const SeqFrag<T> (&qf)[KS], int l15, int g, float& m, float& lg) {
+    float mx = -INFINITY, l = 0.f;
+    for (int k0 = 0; k0 < kend; k0 += 16) {
+        const int key = k0 + l15;
+        const bool in = key < kend && (!mask || mask[key] != 0);
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x = seq_mma(seq_frag_row<T>(K + (long)key * a.k.row, in, s, g, a.d), qf[s], x);
+        const unsigned seen = (unsigned)__ballot(in) >> (4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int rel = k0 + 4 * g + r - p0 - l15;
+            const float b = BIAS ? seq_bias_of(a, h, min(max(rel, -a.D), a.D)) : 0.f;
+            x[r] = ((seen >> r) & 1) && (!a.causal || rel <= 0) ? __builtin_fmaf(x[r], a.scale * SEQ_L2E, b) : -INFINITY;
+        }
+        const float mn = fmaxf(mx, seq_group_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])))), off = mn == -INFINITY ? 0.f : mn;
+        l *= __builtin_amdgcn_exp2f(mx - off);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f(x[r] - off);
+        mx = mn;
+    }
+    m = mx == -INFINITY ? INFINITY : mx;          // (nothing visible: probabilities of zero)
+    lg = mx == -INFINITY ? 0.f : __builtin_amdgcn_logf(seq_group_sum(l));
 }
 // Visible rows of a tile as a bit mask (wave-uniform): rows at or beyond `len` and rows that the key mask hides are clear. The mask's byte of this
 // lane's row is fetched a tile ahead (seq_mask_byte), so that its latency is not paid between two tiles.

@@ -101,6 +101,19 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
         dsum[qb] = seq_group_sum(ds);
         own[qb] = 0.f;
     }
+    float lg[QB];
+    bool rare = false;                                            // some row of the wave has its statistics in two numbers
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        lg[qb] = 0.f;
+        const bool big = seq_row_big(lse2[qb]);
+        if (__any(big)) {
+            float m, l;
+            seq_row_stats<T, KS, BIAS>(a, K, mask, kend, h, pos0 + q0 + 16 * qb, qf[qb], l15, g, m, l);
+            if (big) { lse2[qb] = m; lg[qb] = l; }
+            rare = true;
+        }
+    }
     const float scale2 = a.scale * SEQ_L2E;
     f32x4 acc[QB][G::DA];
 #pragma unroll
@@ -177,9 +190,20 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
                         for (int r = 0; r < 4; ++r) s[qb][kt][r] = __builtin_fmaf(s[qb][kt][r], scale2, w[16 * kt + r - 16 * qb]);
             }
         }
+        if (rare) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    seq_pin(s[qb][kt]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[qb][kt][r] = seq_exponent(__builtin_fmaf(s[qb][kt][r], sc, cb), lse2[qb], lg[qb]);
+                }
+            sc = 1.f;
+        }
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-            const float off = cb - lse2[qb];
+            const float off = rare ? 0.f : cb - lse2[qb];
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -232,7 +256,11 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
         // with a table: the exact sum over this part of the keys; else the one from the output
         const float D = BIAS ? seq_group_sum(own[qb]) : split == 0 ? dsum[qb] : 0.f;
         if (row >= a.Nq) continue;
-        if (g == 0) a.dvec[((long)split * a.B * a.H + bh) * a.Nq + row] = D;
+        if (g == 0) {
+            const long ri = (long)bh * a.Nq + row, n = (long)a.B * a.H * a.Nq;
+            a.dvec[split * n + ri] = D;
+            if (split == 0) { a.stat[ri] = lse2[qb]; a.stat[n + ri] = lg[qb]; }
+        }
         if (a.ksplit > 1) {
             float* P = a.partq + (((long)split * a.B * a.H + bh) * a.Nq + row) * a.d;
             seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(P + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
@@ -266,7 +294,7 @@ template <typename T, int DT, int KB, bool BIAS, bool TAB> struct SeqDkv {
     static constexpr int PAD = G::TK + 16 * KB + 16, NE = KB + G::KT - 1;
     static int lds(int D) {
         const int w = 2 * (D + PAD) + 1;
-        return 4 * G::IMG + 4 * G::TK * 4 + (BIAS ? (int)rup(w * 4, 16) : 0) + (TAB ? 4 * w * 4 : 0);
+        return 4 * G::IMG + (8 * G::TK + 4) * 4 + (BIAS ? (int)rup(w * 4, 16) : 0) + (TAB ? 4 * w * 4 : 0);
     }
 };
 
@@ -278,8 +306,10 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
     constexpr int TQ = G::TK, QT = G::KT, KS = G::KS, STAGE = 2 * G::IMG, PAD = S::PAD, NE = S::NE;
     extern __shared__ __attribute__((aligned(16))) char lds_seq[];
     const int W = 2 * (a.D + PAD) + 1;
-    float* rows = reinterpret_cast<float*>(lds_seq + 2 * STAGE);      // [2 stages][lse, D][TQ]
-    float* bw = rows + 4 * TQ;
+    // [2 stages][lse, D, m, log2 l][TQ], [2 stages] whether some row of the tile has its statistics in two numbers: lse is 0 then, else m and log2 l unused
+    float* rows = reinterpret_cast<float*>(lds_seq + 2 * STAGE);
+    int* two = reinterpret_cast<int*>(rows + 8 * TQ);
+    float* bw = rows + 8 * TQ + 4;
     float* hist = bw + ((W + 3) & ~3);                                // [4 waves][W]
     const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -329,10 +359,10 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
     // per-row numbers of a tile: fetched ahead of its DMA and not looked at before the end of the step, when they are written to LDS
     auto fetch = [&]() {
         const int row = tn * TQ + tid;
-        ls = -INFINITY; dd = 0.f;
+        ls = INFINITY; dd = 0.f;                                  // (a row without a visible key: probabilities of zero)
         if (tid < TQ && row < qlen) {
             const long ri = ((long)b * a.H + hn) * a.Nq + row;
-            ls = a.lse[ri];
+            ls = a.stat[ri];
             dd = a.dvec[ri];
             for (int s = 1; s < a.ksplit; ++s) dd += a.dvec[(long)s * a.B * a.H * a.Nq + ri];
         }
@@ -345,8 +375,18 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
         sd.dma(static_cast<const T*>(a.dout.p) + b * a.dout.batch + hn * a.dout.head + (long)r0 * a.dout.row, dst + G::IMG, live, tid);
     };
     auto put = [&](int u) {
-        // a row without a visible key (or behind the sample's last) has lse = -inf: with +inf in its place its probabilities are zero
-        if (tid < TQ) { float* w = rows + (u & 1) * 2 * TQ; w[tid] = ls == -INFINITY ? INFINITY : ls * SEQ_L2E; w[TQ + tid] = dd; }
+        if (tid < TQ) {                                           // (one wave)
+            float* w = rows + (u & 1) * 4 * TQ;
+            const bool any = __any(seq_row_big(ls));
+            if (any) {
+                const int row = tn * TQ + tid;
+                w[2 * TQ + tid] = ls;
+                w[3 * TQ + tid] = row < qlen ? a.stat[((long)(a.B + b) * a.H + hn) * a.Nq + row] : 0.f;
+                ls = 0.f;
+            }
+            w[tid] = ls; w[TQ + tid] = dd;
+            if (tid == 0) two[u & 1] = any;
+        }
     };
     int h = hn, q0 = tn * TQ, hcur = -1;
     if (u0 < u1) {
@@ -409,7 +449,8 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
         if (u + 1 < u1) { advance(); fetch(); stage(u + 1); }
         const char* Qs = lds_seq + (u & 1) * STAGE;
         const char* Ds = Qs + G::IMG;
-        const float* rw = rows + (u & 1) * 2 * TQ;
+        const float* rw = rows + (u & 1) * 4 * TQ;
+        const int pair = two[u & 1];                              // (looked at behind the products, when it is long there)
         const int p0 = pos0 + q0;
         f32x4 s[KB][QT], dp[KB][QT];
 #pragma unroll
@@ -444,6 +485,19 @@ __global__ __launch_bounds__(256, KB > 1 ? 2 : 1) void seq_dkv_kernel(const SeqA
 #pragma unroll
                         for (int r = 0; r < 4; ++r) s[kb][qt][r] = __builtin_fmaf(s[kb][qt][r], scale2, w[16 * kb - 16 * qt - r]);
             }
+        }
+        if (__builtin_amdgcn_readfirstlane(pair)) {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+                const f32x4 m = *reinterpret_cast<const f32x4*>(rw + 2 * TQ + 16 * qt + 4 * g), l = *reinterpret_cast<const f32x4*>(rw + 3 * TQ + 16 * qt + 4 * g);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    seq_pin(s[kb][qt]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[kb][qt][r] = seq_exponent(__builtin_fmaf(s[kb][qt][r], sc, cb), m[r], l[r]);
+                }
+            }
+            sc = 1.f; cb = 0.f;
         }
         const bool full = !a.causal || k0 + 16 * KB - 1 <= p0;
 #pragma unroll
@@ -588,10 +642,11 @@ SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable) {
     p.ksplit = qblocks < 256 && tiles >= 8 && a.Nk > SEQ_SHORT ? (int)std::min<long>(cdiv(512, std::max(qblocks, 1l)), tiles / 4) : 1;
     if (brief) { p.qb = 0; p.ksplit = 1; }                          // cb_seq_short.hip makes dQ and D
     p.dvec = (size_t)rup((long)p.ksplit * a.B * a.H * a.Nq * 4, 256);
+    p.stat = (size_t)rup((long)2 * a.B * a.H * a.Nq * 4, 256);
     p.tpart = want_dtable ? (size_t)rup((long)a.B * a.H * p.qsplit * p.nkb * a.nb * 4, 256) : 0;
     p.part = p.qsplit > 1 ? (size_t)rup((long)p.qsplit * 2 * a.B * a.Hkv * a.Nk * a.d * 4, 256) : 0;
     p.partq = p.ksplit > 1 ? (size_t)p.ksplit * a.B * a.H * a.Nq * a.d * 4 : 0;
-    p.total = p.dvec + p.tpart + p.part + p.partq;
+    p.total = p.dvec + p.stat + p.tpart + p.part + p.partq;
     return p;
 }
 template <typename T, int DT, int QB, bool BIAS>
@@ -649,6 +704,7 @@ void seq_backward(const Launch& L, SeqArgs a, void* ws) {
     const SeqBwdPlan p = seq_bwd_plan(a, a.dtable != nullptr);
     char* w = static_cast<char*>(ws);
     a.dvec = reinterpret_cast<float*>(w); w += p.dvec;
+    a.stat = reinterpret_cast<float*>(w); w += p.stat;
     a.tpart = reinterpret_cast<float*>(w); w += p.tpart;
     a.part = reinterpret_cast<float*>(w); w += p.part;
     a.partq = reinterpret_cast<float*>(w);

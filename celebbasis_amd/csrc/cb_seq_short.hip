@@ -165,8 +165,38 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
                 if (g == 0 && a.lse) a.lse[ri] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * SEQ_LN2;
             }
         } else {
-            const float ls2 = lse == -INFINITY ? INFINITY : lse * SEQ_L2E;       // a row without a visible key: probabilities of zero
-            float D = 0.f;
+            float ls2 = lse == -INFINITY ? INFINITY : lse * SEQ_L2E;             // a row without a visible key: probabilities of zero
+            float m2 = ls2, lg = 0.f, D = 0.f;
+            const bool big = seq_row_big(ls2);
+            if (__any(big)) {                                                    // rows whose statistics are kept in two numbers (seq_row_stats)
+                float mx = -INFINITY, l = 0.f;
+                auto each = [&](auto&& f) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int kt = 0; kt < KT; ++kt) {
+                            if (!bits(t, kt)) continue;
+                            seq_pin(s[t][0][kt]);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) f(s[t][0][kt][r]);
+                        }
+                };
+                each([&](float x) { mx = fmaxf(mx, x); });
+                mx = seq_group_max(mx);
+                if (big) m2 = mx;
+                each([&](float x) { l += __builtin_amdgcn_exp2f(x - m2); });
+                l = seq_group_sum(l);
+                if (big) lg = __builtin_amdgcn_logf(l);
+                ls2 = 0.f;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        if (!bits(t, kt)) continue;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[t][0][kt][r] = seq_exponent(s[t][0][kt][r], m2, lg);
+                    }
+            }
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -191,7 +221,7 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
             }
             next();
             if (row < a.Nq) {
-                if (g == 0) a.dvec[ri] = D;
+                if (g == 0) { a.dvec[ri] = D; a.stat[ri] = m2; a.stat[(long)a.B * a.H * a.Nq + ri] = lg; }
                 T* dQ = static_cast<T*>(a.dq.p) + b * a.dq.batch + h * a.dq.head + (long)row * a.dq.row;
                 seq_row4<T, DT>(o[0], a.d, g, [&](int c, float4 v) { st4(dQ + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
             }

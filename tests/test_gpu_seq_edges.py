@@ -1,4 +1,5 @@
-"""GPU tests of the sequence attention at the edges of its definition: table entries of -inf and of very large magnitude over whole key tiles.
+"""GPU tests of the sequence attention at the edges of its definition: table entries of -inf and of very large magnitude over whole key tiles, and
+their gradients.
 
 Bounds as in test_gpu_seq_ops.py (u = 2^-24, r = 2^-8 for bf16 operands and results). A table entry b of magnitude 1e8 and more takes every score
 |s| < ulp(b) / 2 up whole: s + b rounds to b, so all keys of such entries weigh alike; against keys of ordinary entries their weight is 0 exactly. What is
@@ -9,7 +10,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_seq_ops import BF, F, R, U, buckets, rnd, within
+from test_gpu_seq_ops import BF, F, R, U, buckets, check, rnd, within
 
 pytestmark = pytest.mark.gpu
 DT = pytest.mark.parametrize("dtype", [torch.float32, BF], ids=["f32", "bf16"])
@@ -31,7 +32,7 @@ def cb(built_lib):
 T = lambda x: x.transpose(-1, -2).contiguous()  # noqa: E731
 
 
-def check_table(cb, dtype, B, Nq, Nk, H, d, rel, table, causal=False, q_pos=None, kv_mask=None, scale=None, amp=1.0, seed=0, grad=True):
+def check_table(cb, dtype, B, Nq, Nk, H, d, rel, table, causal=False, q_pos=None, kv_mask=None, scale=None, amp=1.0, seed=0):
     """forward and backward with the given table against 64 bits (one key head a query head)"""
     lib, ctx = cb
     dev = _dev()
@@ -88,8 +89,6 @@ def check_table(cb, dtype, B, Nq, Nk, H, d, rel, table, causal=False, q_pos=None
     assert not heads(out)[none].any() and (tape.lse[none] == -math.inf).all() and torch.isfinite(tape.lse[~none]).all()
     bare = lib.seq_attention(ctx, q, k, v, scale=scale, causal=causal, q_pos=pos32, kv_mask=kv_mask, relpos=rp, table=table)
     assert torch.equal(bare, out)
-    if not grad:
-        return
     g = lib.seq_attention_backward(ctx, tape, do)
     for name, got, want, bnd in (("dq", g.dq, dq, dqb), ("dk", g.dk, dk, dkb), ("dv", g.dv, dv, dvb)):
         within(name, got, heads(want), heads(bnd + rT * (want.abs() + bnd)))
@@ -125,9 +124,9 @@ def test_outermost_bucket_hidden(cb, dtype, value, B, Nq, Nk, H):
     """a window: keys past the table's range carry -inf (or next to nothing) while near ones are ordinary; small and large scores"""
     for rel, causal in (((32, 64, True), False), ((32, 64, False), True)):
         t = _table(rel, H, value, "outer")
-        check_table(cb, dtype, B, Nq, Nk, H, 64, rel, t, causal=causal, grad=value == -math.inf)
+        check_table(cb, dtype, B, Nq, Nk, H, 64, rel, t, causal=causal)
         if value != -1e9:                      # (scores of hundreds are not absorbed by 1e9)
-            check_table(cb, dtype, B, Nq, Nk, H, 64, rel, t, causal=causal, amp=6.0, scale=1.0, grad=value == -math.inf)
+            check_table(cb, dtype, B, Nq, Nk, H, 64, rel, t, causal=causal, amp=6.0, scale=1.0)
 
 
 @DT
@@ -137,20 +136,40 @@ def test_rows_that_see_only_hidden_buckets(cb, dtype, value):
     rel = (32, 64, True)
     t = _table(rel, 2, value, "outer")
     for Nk in (100, 200, 700):
-        check_table(cb, dtype, 4, 70, Nk, 2, 64, rel, t, q_pos=[0, 2000, -2000, 300], grad=value == -math.inf)
+        check_table(cb, dtype, 4, 70, Nk, 2, 64, rel, t, q_pos=[0, 2000, -2000, 300])
         m = torch.zeros(2, Nk, dtype=torch.bool, device=_dev())
         m[:, Nk - 20:] = True
-        check_table(cb, dtype, 2, Nk - 10, Nk, 2, 64, rel, t, kv_mask=m, grad=value == -math.inf)
-    check_table(cb, dtype, 16, 520, 700, 16, 40, rel, _table(rel, 16, value, "outer"), q_pos=[1500] * 8 + [0] * 8, grad=value == -math.inf)
+        check_table(cb, dtype, 2, Nk - 10, Nk, 2, 64, rel, t, kv_mask=m)
+    check_table(cb, dtype, 16, 520, 700, 16, 40, rel, _table(rel, 16, value, "outer"), q_pos=[1500] * 8 + [0] * 8)
 
 
 @DT
 @pytest.mark.parametrize("value", [LOWEST, -1e30, -1e9, 1e9, -math.inf])
 @pytest.mark.parametrize("B,Nq,Nk,H", SHAPES)
 def test_every_bucket_alike(cb, dtype, value, B, Nq, Nk, H):
-    """all entries take the scores up whole: every visible key weighs the same"""
-    rel, g = (32, 64, True), value == -math.inf
-    check_table(cb, dtype, B, Nq, Nk, H, 64, rel, _table(rel, H, value, "all"), grad=g)
-    check_table(cb, dtype, B, Nq, Nk, H, 40, (16, 700, False), _table((16, 700, False), H, value, "all"), causal=True, grad=g)
+    """all entries take the scores up whole: every visible key weighs the same, in the gradients too"""
+    rel = (32, 64, True)
+    check_table(cb, dtype, B, Nq, Nk, H, 64, rel, _table(rel, H, value, "all"))
+    check_table(cb, dtype, B, Nq, Nk, H, 40, (16, 700, False), _table((16, 700, False), H, value, "all"), causal=True)
     if abs(value) != 1e9:
-        check_table(cb, dtype, B, Nq, Nk, H, 64, rel, _table(rel, H, value, "all"), amp=6.0, scale=1.0, grad=g)
+        check_table(cb, dtype, B, Nq, Nk, H, 64, rel, _table(rel, H, value, "all"), amp=6.0, scale=1.0)
+
+
+@DT
+def test_one_token_row_of_lowest_entries(cb, dtype):
+    """the one-token kernel's statistics in the tile kernels' backward"""
+    rel = (32, 64, True)
+    for value in (LOWEST, -1e9, -math.inf):
+        for Nk in (90, 600, 3000):
+            check_table(cb, dtype, 3, 1, Nk, 2, 64, rel, _table(rel, 2, value, "all"), q_pos=[0, 50, 4000])
+            check_table(cb, dtype, 3, 1, Nk, 2, 64, rel, _table(rel, 2, value, "outer"), q_pos=[0, 50, 4000])
+
+
+@DT
+@pytest.mark.parametrize("amp", [12.0, 24.0])
+@pytest.mark.parametrize("rel", [None, (32, 64, True)])
+def test_scores_of_thousands(cb, dtype, amp, rel):
+    """ordinary rows on both sides of the magnitude at which the backward pass makes its statistics anew"""
+    check(cb, dtype, 1, 130, 100, 2, 2, 64, amp=amp, scale=1.0, rel=rel)
+    check(cb, dtype, 2, 130, 260, 2, 1, 64, amp=amp, scale=1.0, rel=rel, causal=True, kv_len=[260, 201])
+    check(cb, dtype, 1, 70, 900, 2, 2, 80, amp=amp, scale=1.0, rel=rel)
