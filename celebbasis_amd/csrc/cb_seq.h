@@ -231,6 +231,8 @@ __device__ __forceinline__ void seq_row4(const SeqRow<T, DT>& acc, int d, int g,
     }
 }
 
+// v times f, or zeros where a row sees nothing: selected, since what it was multiplied with may not be finite
+__device__ __forceinline__ float4 seq_scaled(float4 v, float f, bool none) { return none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
 // the bias of head h at distance rel (within +-D), times log2(e). The entries stay finite in the log2 domain (a table may hold its type's lowest
 // value): held to +-1e37; minus infinity and NaN are kept.
 __device__ __forceinline__ float seq_bias_of(const SeqArgs& a, int h, int rel) {

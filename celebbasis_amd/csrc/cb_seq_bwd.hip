@@ -254,7 +254,8 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
     for (int qb = 0; qb < QB; ++qb) {
         const int row = q0 + 16 * qb + l15;
         // with a table: the exact sum over this part of the keys; else the one from the output
-        const float D = BIAS ? seq_group_sum(own[qb]) : split == 0 ? dsum[qb] : 0.f;
+        const bool none = lse2[qb] == INFINITY;
+        const float sum = BIAS ? seq_group_sum(own[qb]) : split == 0 ? dsum[qb] : 0.f, D = none ? 0.f : sum;
         if (row >= a.Nq) continue;
         if (g == 0) {
             const long ri = (long)bh * a.Nq + row, n = (long)a.B * a.H * a.Nq;
@@ -263,11 +264,11 @@ __global__ __launch_bounds__(256, QB > 1 ? 2 : 1) void seq_dq_kernel(const SeqAr
         }
         if (a.ksplit > 1) {
             float* P = a.partq + (((long)split * a.B * a.H + bh) * a.Nq + row) * a.d;
-            seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(P + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
+            seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(P + c, seq_scaled(v, a.scale, none)); });
             continue;
         }
         T* dQ = static_cast<T*>(a.dq.p) + b * a.dq.batch + h * a.dq.head + (long)row * a.dq.row;
-        seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(dQ + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
+        seq_row4<T, DT>(acc[qb], a.d, g, [&](int c, float4 v) { st4(dQ + c, seq_scaled(v, a.scale, none)); });
     }
 #endif
 }

@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256, DT > 8 ? 1 : 2) void seq_fwd_kernel(const SeqA
         T* O = static_cast<T*>(a.o.p) + b * a.o.batch + h * a.o.head + (long)row * a.o.row;
         float* O32 = a.o32 ? a.o32 + (((long)b * a.Nq + row) * a.H + h) * a.d : nullptr;
         seq_row4<T, DT>(o[qb], a.d, g, [&](int c, float4 v) {
-            v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+            v = seq_scaled(v, inv, none);
             st4(O + c, v);
             if (O32) st4(O32 + c, v);
         });

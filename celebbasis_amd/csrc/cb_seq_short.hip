@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
             next();
             if (row < a.Nq) {
                 T* O = static_cast<T*>(a.o.p) + b * a.o.batch + h * a.o.head + (long)row * a.o.row;
-                seq_row4<T, DT>(o[0], a.d, g, [&](int c, float4 v) { st4(O + c, make_float4(none ? 0.f : v.x * inv, none ? 0.f : v.y * inv, none ? 0.f : v.z * inv, none ? 0.f : v.w * inv)); });
+                seq_row4<T, DT>(o[0], a.d, g, [&](int c, float4 v) { st4(O + c, seq_scaled(v, inv, none)); });
                 if (g == 0 && a.lse) a.lse[ri] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * SEQ_LN2;
             }
         } else {
@@ -208,7 +208,9 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
                         D = __builtin_fmaf(s[t][0][kt][r], dp[t][kt][r], D);
                     }
                 }
+            const bool none = m2 == INFINITY;
             D = seq_group_sum(D);
+            D = none ? 0.f : D;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
             if (row < a.Nq) {
                 if (g == 0) { a.dvec[ri] = D; a.stat[ri] = m2; a.stat[(long)a.B * a.H * a.Nq + ri] = lg; }
                 T* dQ = static_cast<T*>(a.dq.p) + b * a.dq.batch + h * a.dq.head + (long)row * a.dq.row;
-                seq_row4<T, DT>(o[0], a.d, g, [&](int c, float4 v) { st4(dQ + c, make_float4(v.x * a.scale, v.y * a.scale, v.z * a.scale, v.w * a.scale)); });
+                seq_row4<T, DT>(o[0], a.d, g, [&](int c, float4 v) { st4(dQ + c, seq_scaled(v, a.scale, none)); });
             }
         }
     }

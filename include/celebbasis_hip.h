@@ -198,8 +198,9 @@ typedef struct { void* p; int64_t row, head, batch; } cb_seq_tensor; /* [batch][
  *   j < kv_len[b], kv_mask[b][j] != 0, causal: j <= q_pos[b] + i; i < q_len[b].
  * Query rows without a visible key, and rows at or beyond q_len[b], give o = 0, lse = -inf and take part in no gradient; gradients of keys
  * that are not visible are 0. What K, V hold in places hidden by kv_len or kv_mask, and Q, dout in rows beyond q_len, is never used (it may be
- * NaN). A table entry of -inf hides its bucket; finite ones of any magnitude count (held
- * to +-1e37): scale q.k + entry is rounded to fp32, in the backward pass as in the forward. A one-token call over a cache: Nq = 1, q_pos[b] = kv_len[b] - 1.
+ * NaN). Causal order hides scores alone: a V that is not finite at a key behind a query that sees others may reach it (0 x inf). A table entry of
+ * -inf hides its bucket; finite ones of any magnitude count (held to +-1e37): scale q.k + entry is rounded to fp32, in the backward pass as in the
+ * forward. A one-token call over a cache: Nq = 1, q_pos[b] = kv_len[b] - 1.
  * kv_heads divides heads; head h reads key / value head h / (heads / kv_heads). d % 8 == 0, d <= 160. Pointers 16-byte aligned, strides
  * multiples of 16 bytes, row strides below 2^22 elements; out, dq, dk, dv must not overlap themselves, and their address ranges not those of
  * the inputs (dq, dk and dv may be slices of one buffer). Inputs may have stride 0. The backward call reads the inputs again, lengths and mask

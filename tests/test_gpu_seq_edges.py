@@ -173,3 +173,23 @@ def test_scores_of_thousands(cb, dtype, amp, rel):
     check(cb, dtype, 1, 130, 100, 2, 2, 64, amp=amp, scale=1.0, rel=rel)
     check(cb, dtype, 2, 130, 260, 2, 1, 64, amp=amp, scale=1.0, rel=rel, causal=True, kv_len=[260, 201])
     check(cb, dtype, 1, 70, 900, 2, 2, 80, amp=amp, scale=1.0, rel=rel)
+
+
+@DT
+@pytest.mark.parametrize("rel", [None, (32, 64, True)])
+@pytest.mark.parametrize("Nq,Nk,H", [(100, 77, 2), (100, 200, 2), (100, 700, 2), (520, 700, 64), (1, 700, 2)])
+def test_rows_without_keys_are_zero_beside_values_that_overflowed(cb, dtype, rel, Nq, Nk, H):
+    """rows behind q_len, and rows before the first key in causal order, give 0 and take 0 where a value that other rows see is infinite"""
+    lib, ctx = cb
+    q, k, v = (rnd(2, n, H, 64, seed=i, dtype=dtype) for i, n in enumerate((Nq, Nk, Nk)))
+    v[:, 3] = math.inf
+    do = rnd(2, Nq, H, 64, seed=3, dtype=dtype)
+    extra = dict(relpos=lib.RelPos(ctx, *rel), table=rnd(rel[0], H, seed=4)) if rel else {}
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=_dev())              # noqa: E731
+    for kw, rows in ((dict(q_len=i32(Nq - Nq // 3 - 1, Nq)), [(0, slice(Nq - Nq // 3 - 1, Nq)), (1, slice(0, 0))]),
+                     (dict(causal=True, q_pos=i32(-(Nq // 3) - 1, 8)), [(0, slice(0, Nq // 3 + 1)), (1, slice(0, 0))])):
+        out, tape = lib.seq_attention(ctx, q, k, v, need_grad=True, **kw, **extra)
+        g = lib.seq_attention_backward(ctx, tape, do)
+        for b, r in rows:
+            assert not out[b, r].any() and (tape.lse[b, :, r] == -math.inf).all() and not g.dq[b, r].any()
+        assert not torch.isfinite(out[1, :, :]).all()                               # the infinity shows where it is seen
