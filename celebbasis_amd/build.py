@@ -28,7 +28,7 @@ EXTRA = {src: (["-mllvm", "-amdgpu-mfma-vgpr-form"] if os.environ.get("CB_MFMA_V
 NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 for _src in ("cb_seq_fwd.hip", "cb_seq_bwd.hip", "cb_seq_short.hip"):
     EXTRA[_src] = EXTRA["cb_flash.hip"] + NO_PACKED
-for _src in ("cb_seq_token.hip", "cb_seq_short.hip", "cb_norm_i8.hip", "cb_gemm_i8.hip"):
+for _src in ("cb_seq_token.hip", "cb_norm_i8.hip", "cb_gemm_i8.hip"):
     EXTRA[_src] = NO_PACKED
 # Kernels whose software pipeline COUNTS its outstanding VMEM instructions (`s_waitcnt vmcnt(N)` + raw `s_barrier`,
 # cb_gemm_glds.hip): a register spill would add scratch loads / stores to that count and let a tile be read before it has landed.
