@@ -24,7 +24,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-u
 EXTRA = {src: (["-mllvm", "-amdgpu-mfma-vgpr-form"] if os.environ.get("CB_MFMA_VGPR_FORM", "1") != "0" else [])
          for src in ("cb_flash.hip", "cb_flash_bf16.hip", "cb_flash_bf16_v2.hip")}
 # Packed fp32 instructions are kept out of these files: hipcc forms them from ordinary float code, and some of their forms have given wrong
-# results on this part. (The host pass does not know the feature and says so.)
+# results on this part. A compiler that does not take this flag builds none of them; the tuning flags above are left out where they are not
+# known. (The host pass does not know the feature and says so.)
 NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 for _src in ("cb_seq_fwd.hip", "cb_seq_bwd.hip", "cb_seq_short.hip"):
     EXTRA[_src] = EXTRA["cb_flash.hip"] + NO_PACKED
@@ -127,17 +128,23 @@ def build(verbose=True, force=False):
 def _build_locked(verbose, force):
     hdrs = [os.path.join(CSRC, h) for h in HEADERS]
     hipcc = _hipcc()
-    for flags in {tuple(v) for v in EXTRA.values() if v}:          # probe once, before the worker threads share the cache
+    tuning = {tuple(v[:-len(NO_PACKED)] if v[-len(NO_PACKED):] == NO_PACKED else v) for v in EXTRA.values()}
+    for flags in {f for f in tuning if f} | {tuple(NO_PACKED)}:    # probe once, before the worker threads share the cache
         _flag_supported(hipcc, flags)
 
     def compile_one(src):
         import hashlib
         s = os.path.join(CSRC, src)
-        extra = list(EXTRA.get(src, []))
+        extra, needed = list(EXTRA.get(src, [])), []
+        if extra[-len(NO_PACKED):] == NO_PACKED:
+            extra, needed = extra[:-len(NO_PACKED)], NO_PACKED
+        if needed and not _flag_supported(hipcc, needed):
+            raise RuntimeError(f"{src}: {hipcc} rejects {' '.join(needed)}, which keeps packed fp32 instructions out of its kernels")
         if extra and not _flag_supported(hipcc, extra):
             print(f"[celebbasis_amd.build] WARNING: {hipcc} rejects {' '.join(extra)}; building {src} without it "
                   "(attention accumulators in AGPR form: correct, a few percent slower)", flush=True)
             extra = []
+        extra += needed
         guard, fatal = {**NO_SCRATCH, **NO_SCRATCH_I8}.get(src, (None, False))
         if guard:
             extra += ["-Rpass-analysis=kernel-resource-usage"]
