@@ -193,3 +193,48 @@ def test_rows_without_keys_are_zero_beside_values_that_overflowed(cb, dtype, rel
         for b, r in rows:
             assert not out[b, r].any() and (tape.lse[b, :, r] == -math.inf).all() and not g.dq[b, r].any()
         assert not torch.isfinite(out[1, :, :]).all()                               # the infinity shows where it is seen
+
+
+def _key_block(cb, B, Nq, Nk, H, Hkv, d, nb):
+    """keys a block of the dK/dV kernel takes (64 or 128), told from what its parts of dtable need: whole key axes, so parts = blocks of keys"""
+    import ctypes as C
+    lib, ctx = cb
+    rp = lib.RelPos(ctx, nb, 64, True)
+    t = torch.zeros(16, device=_dev())
+    D = lib.SeqAttentionDesc()
+    D.dtype, D.B, D.Nq, D.Nk, D.heads, D.kv_heads, D.d, D.scale = lib.DTYPE_BF16, B, Nq, Nk, H, Hkv, d, 1.0
+    D.relpos, D.table = rp.h, t.data_ptr()
+    sizes = []
+    for dtable in (None, t.data_ptr()):
+        D.dtable = dtable
+        n = C.c_int64()
+        lib.check(lib.load().cb_seq_attention_workspace(ctx.h, C.byref(D), 1, C.byref(n)))
+        sizes.append(n.value)
+    parts = [b for b in (64, 128) if abs(sizes[1] - sizes[0] - B * H * -(-Nk // b) * nb * 4) < 256]
+    assert len(parts) == 1, sizes
+    return parts[0]
+
+
+@pytest.mark.parametrize("d", [32, 40, 64])
+@pytest.mark.parametrize("kind", ["causal", "two_sided", "shared", "plain"])
+def test_backward_of_wide_blocks(cb, d, kind):
+    """bf16, enough work for the backward kernels that hold 32 rows a wave (both take the same rule, on queries and on keys), odd lengths"""
+    B, N, H, Hkv, kw = 11, 650, 12, 12, {}
+    lens = [650, 1, 64, 65, 333, 640, 0, 512, 649, 129, 650]
+    if kind == "causal":
+        kw = dict(rel=(32, 64, False), causal=True, kv_len=lens, q_len=lens)
+    elif kind == "two_sided":
+        m = torch.rand(B, N, generator=torch.Generator().manual_seed(5)) < 0.6
+        m[3] = False
+        m[4, :300] = False
+        kw = dict(rel=(32, 64, True), kv_mask=m.to(_dev()))
+    elif kind == "shared":
+        H, Hkv = 24, 12
+        kw = dict(rel=(16, 128, True), kv_len=lens)
+    else:
+        kw = dict(kv_len=lens, causal=True, q_pos=[0, 5, 700, 0, -30, 0, 0, 100, 0, 0, 1])
+    nb = kw.get("rel", (32,))[0]
+    assert _key_block(cb, B, N, N, H, Hkv, d, nb) == 128 and _key_block(cb, 10, N, N, 12, 12, d, nb) == 64
+    check(cb, BF, B, N, N, H, Hkv, d, **kw)
+    if kind == "two_sided":
+        check_table(cb, BF, B, N, N, H, d, kw["rel"], _table(kw["rel"], H, LOWEST, "outer"), kv_mask=kw["kv_mask"])
