@@ -234,7 +234,8 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
 
 // ---------------------------------------------------------------- host side
 // (fp32 heads beyond 128: 128 keys and the bias do not fit LDS)
-bool seq_short_takes(const SeqArgs& a) { return a.Nk > 0 && a.Nk <= (a.dt == DT_F32 && a.d > 128 ? 64 : SEQ_SHORT); }
+template <typename T, int DT> constexpr int SHORT_KEYS = sizeof(T) == 4 && DT > 8 ? 64 : SEQ_SHORT;
+bool seq_short_takes(const SeqArgs& a) { return a.Nk > 0 && a.Nk <= (a.dt == DT_F32 && a.d > 128 ? SHORT_KEYS<float, 10> : SEQ_SHORT); }
 template <typename T, int DT, int NT, bool BWD>
 static void short_go(const Launch& L, const SeqArgs& a) {
     // blocks of 16 rows a wave: as many as leave 2 blocks (of 4 waves) a CU, at most 8. 64 heads, 4096 x 77, forward / dQ: 2 rows of blocks 30 / 40 us,
@@ -259,8 +260,10 @@ static void short_go(const Launch& L, const SeqArgs& a) {
 template <typename T, int DT>
 static void short_pick(const Launch& L, const SeqArgs& a, bool bwd) {
     constexpr int ONE = 64 / SeqGeo<T, DT>::TK;
-    if (a.Nk <= 64) { if (bwd) short_go<T, DT, ONE, true>(L, a); else short_go<T, DT, ONE, false>(L, a); }
-    else { if (bwd) short_go<T, DT, 2 * ONE, true>(L, a); else short_go<T, DT, 2 * ONE, false>(L, a); }
+    if constexpr (SHORT_KEYS<T, DT> > 64) {
+        if (a.Nk > 64) { if (bwd) short_go<T, DT, 2 * ONE, true>(L, a); else short_go<T, DT, 2 * ONE, false>(L, a); return; }
+    }
+    if (bwd) short_go<T, DT, ONE, true>(L, a); else short_go<T, DT, ONE, false>(L, a);
 }
 void seq_short(const Launch& L, const SeqArgs& a, bool bwd) {
     CB_DT_SWITCH(a.dt, T, SEQ_DT_SWITCH(a.d, DT, short_pick<T, DT>(L, a, bwd)));
