@@ -1113,6 +1113,41 @@ static void seq_apart(const std::vector<SeqRange>& written, const std::vector<Se
         for (auto& r : read)
             CB_CHECK(w.lo >= r.hi || r.lo >= w.hi || w.lo == w.hi || r.lo == r.hi, CB_ERR_ARG, "seq attention: %s overlaps %s", w.what, r.what);
 }
+// two written operands may be slices of one buffer: whether some element belongs to both. `dims`: (stride, extents), the larger strides first;
+// `delta`: where the second begins behind the first. Where slices interleave so much that this would take long, they count as overlapping.
+struct SeqDim { int64_t stride, n1, n2, w1, w2; };          // w: what the inner dimensions span
+static bool seq_meets(const std::vector<SeqDim>& dims, size_t at, int64_t delta, int64_t d, int& visits) {
+    if (at == dims.size()) return delta < d && -delta < d;
+    const SeqDim& m = dims[at];
+    const auto down = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };
+    // inner offsets delta + k stride, k the second's index less the first's, that lie within the inner spans
+    const int64_t k0 = std::max(-(m.n1 - 1), down(-m.w2 - delta, m.stride) + 1), k1 = std::min(m.n2 - 1, down(m.w1 - 1 - delta, m.stride));
+    for (int64_t k = k0; k <= k1; ++k)
+        if (++visits > 4096 || seq_meets(dims, at + 1, delta + k * m.stride, d, visits)) return true;
+    return false;
+}
+static void seq_disjoint(const char* what1, const SeqT& a, int N1, int H1, const char* what2, const SeqT& b, int N2, int H2, DType dt, int B, int d) {
+    const SeqRange ra = seq_range(what1, a, dt, B, N1, H1, d), rb = seq_range(what2, b, dt, B, N2, H2, d);
+    if (!a.p || !b.p || ra.lo == ra.hi || rb.lo == rb.hi || ra.hi <= rb.lo || rb.hi <= ra.lo) return;       // tensors of their own
+    std::vector<SeqDim> dims;
+    const auto add = [&](int64_t stride, int64_t n, bool second) {
+        if (n <= 1) return;
+        for (auto& x : dims)
+            if (x.stride == stride && (second ? x.n2 : x.n1) == 1) { (second ? x.n2 : x.n1) = n; return; }
+        dims.push_back({stride, second ? 1 : n, second ? n : 1, 0, 0});
+    };
+    add(a.row, N1, false); add(a.head, H1, false); add(a.batch, B, false);
+    add(b.row, N2, true); add(b.head, H2, true); add(b.batch, B, true);
+    std::sort(dims.begin(), dims.end(), [](const SeqDim& x, const SeqDim& y) { return x.stride > y.stride; });
+    int64_t w1 = d, w2 = d;
+    for (size_t i = dims.size(); i-- > 0;) {
+        dims[i].w1 = w1; dims[i].w2 = w2;
+        w1 += dims[i].stride * (dims[i].n1 - 1); w2 += dims[i].stride * (dims[i].n2 - 1);
+    }
+    const int64_t delta = (int64_t)(reinterpret_cast<intptr_t>(b.p) - reinterpret_cast<intptr_t>(a.p)) / (int64_t)dt_size(dt);
+    int visits = 0;
+    CB_CHECK(!seq_meets(dims, 0, delta, d, visits), CB_ERR_ARG, "seq attention: %s overlaps %s", what1, what2);
+}
 static SeqArgs seq_args(const cb_ctx* ctx, const cb_seq_attention_desc* d, bool bwd, bool pointers) {
     const Ctx& c = ctx->c;
     CB_CHECK(d->struct_size == (int)sizeof(cb_seq_attention_desc), CB_ERR_ARG, "seq attention: desc.struct_size %d != %d — caller built against "
@@ -1161,6 +1196,9 @@ static SeqArgs seq_args(const cb_ctx* ctx, const cb_seq_attention_desc* d, bool 
         const std::vector<SeqRange> grads = {q_side("dq", a.dq), k_side("dk", a.dk), k_side("dv", a.dv)};
         seq_apart(grads, in);
         seq_apart(grads, {q_side("out", a.o), q_side("dout", a.dout)});
+        seq_disjoint("dq", a.dq, d->Nq, d->heads, "dk", a.dk, d->Nk, d->kv_heads, a.dt, d->B, d->d);
+        seq_disjoint("dq", a.dq, d->Nq, d->heads, "dv", a.dv, d->Nk, d->kv_heads, a.dt, d->B, d->d);
+        seq_disjoint("dk", a.dk, d->Nk, d->kv_heads, "dv", a.dv, d->Nk, d->kv_heads, a.dt, d->B, d->d);
     }
     return a;
 }

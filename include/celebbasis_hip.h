@@ -203,8 +203,8 @@ typedef struct { void* p; int64_t row, head, batch; } cb_seq_tensor; /* [batch][
  * forward. A one-token call over a cache: Nq = 1, q_pos[b] = kv_len[b] - 1.
  * kv_heads divides heads; head h reads key / value head h / (heads / kv_heads). d % 8 == 0, d <= 160. Pointers 16-byte aligned, strides
  * multiples of 16 bytes, row strides below 2^22 elements; out, dq, dk, dv must not overlap themselves, and their address ranges not those of
- * the inputs (dq, dk and dv may be slices of one buffer). Inputs may have stride 0. The backward call reads the inputs again, lengths and mask
- * included: they hold what the forward call saw. */
+ * the inputs; dq, dk and dv may be slices of one buffer that do not meet. Inputs may have stride 0. The backward call reads the inputs again,
+ * lengths and mask included: they hold what the forward call saw. */
 typedef struct {
     int struct_size;                             /* = sizeof(cb_seq_attention_desc) */
     int dtype;                                   /* cb_dtype of q, k, v, out, dout, dq, dk, dv */
