@@ -127,7 +127,18 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsArgs a) {
             for (int e = 0; e < 8; ++e) s = __builtin_fmaf(v[j][e], v[j][e], s);
             ss += s;
         }
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(ss, sh) / (float)C + a.eps);
+        const float ms = row_sum<TPR>(ss, sh) / (float)C;
+        float rstd = 1.f / sqrtf(ms + a.eps);
+        // squares beyond fp32's range, or so small that they lost bits beside no greater eps: once more, of the row times 2^-100 or 2^100
+        if (!(ms < 3e38f) || ms + a.eps < 0x1p-90f) {
+            const float f = ms + a.eps < 0x1p-90f ? 0x1p100f : 0x1p-100f;
+            ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { const float x = v[j][e] * f; ss = __builtin_fmaf(x, x, ss); }
+            rstd = f / sqrtf(row_sum<TPR>(ss, sh) / (float)C + a.eps * f * f);
+        }
         if (t == 0 && a.rstd) a.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {

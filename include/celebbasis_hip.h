@@ -227,9 +227,9 @@ int cb_seq_attention_fwd(cb_ctx* ctx, const cb_seq_attention_desc* d);
 int cb_seq_attention_bwd(cb_ctx* ctx, const cb_seq_attention_desc* d);
 
 /* Root-mean-square norm with the residual's addition (beside cb_layernorm_*): h = round_dtype(x + residual) is the residual stream as it is
- * held; rstd = 1 / sqrt(mean(h^2) + eps); y = h rstd gamma, in dtype or in 8 bits: scale = max|y| / 127, y_i8 = rint(y 127 / max|y|) of the
- * unrounded y, columns C .. ceil16(C) zeroed (what cb_gemm_i8 reads). A row that holds a NaN or an infinity gets it as its scale and zeros
- * as its values; a row whose largest magnitude is below 2^-119 gets scale 0.
+ * held; rstd = 1 / sqrt(mean(h^2) + eps), for rows of any finite magnitude; y = h rstd gamma, in dtype or in 8 bits: scale = max|y| / 127,
+ * y_i8 = rint(y 127 / max|y|) of the unrounded y, columns C .. ceil16(C) zeroed (what cb_gemm_i8 reads). A row that holds a NaN or an infinity
+ * gets a scale that is not finite and zeros as its values; a row whose largest magnitude is below 2^-119 gets scale 0.
  * Backward: dh = rstd (dy gamma - h rstd^2 mean(dy gamma h)) + dres, the gradient of x and of the residual alike;
  * dgamma = sum over rows of dy h rstd, written, in a fixed order. x, h, residual may be one buffer, and dh may be dy or dres.
  * 1 <= C <= 16384, any row strides >= C; rows of whole aligned 16-byte pieces (C % 8 == 0) take the fast path. */
