@@ -395,11 +395,11 @@ static I8Plan i8_plan(const GemmI8Args& a) {
     // 8192) 26.2 / 22.6, 2^32 (64, 4096 x 16384) 50.6 / 27.5
     if (a.M <= 64 && (long)a.M * a.N * a.K <= 3L << 29) { p.kind = I8_FEW; return p; }
     // 256 against 128 tiles (us of a call): 128 of them (1024 x 8192 x 4096) 48.4 / 41.1, 160 (2560 x 4096 x 4096) 50.8 / 60.1, 196 (3584 x 3584 x
-    // 4096) 55.0 / 70.4
-    if (t256 >= 160) { p.kind = I8_256; return p; }
+    // 4096) 55.0 / 70.4. Only where a tile's rows are more than half there: 192 tiles of N = 49152, K = 4096 with 128 rows 56.3 / 52.0, with 129 57.4 / 74.0
+    if (t256 >= 160 && a.M > 128) { p.kind = I8_256; return p; }
     // 128 against 64 tiles: 192 of them (128 x 24576 x 4096) 68 / 34, 256 (512 x 8192 x 4096) 33.8 / 35.2, (512 x 8192 x 8192) 61 / 66, 384 (256 x 24576
-    // x 4096) 45.6 / 62
-    p.kind = t128 >= 256 ? I8_128 : I8_64;
+    // x 4096) 45.6 / 62. With rows enough for both: N = 49152, K = 4096, 64 rows 47.8 / 43.3, 65 rows 47.6 / 61.4; N = 40960, K = 2048 25.2 / 20.4, 25.0 / 32.2
+    p.kind = t128 >= 256 && a.M > 64 ? I8_128 : I8_64;
     const long t = p.kind == I8_128 ? t128 : t64;
     // fewer tiles than CUs: K is split into runs of at least 8 k-tiles for two blocks a CU. 64 x 4096 x 4096 (64 tiles) whole / 4 runs of 8 / 8 of 4:
     // 26.0 / 17.9 / 20.9; 64 x 8192 x 8192 (128 tiles) whole / 4 / 8: 50 / 26 / 31. As many 64 tiles as CUs: four runs where K is long (128 x 8192 x 8192
