@@ -427,6 +427,9 @@ template <typename T> static void i8_any(const Launch& L, GemmI8Args a, void* ws
     const I8Plan p = i8_plan(a);
     a.nsplit = p.nsplit;
     a.part = static_cast<int*>(ws);
+    const long bm = p.kind == I8_256 ? 256 : p.kind == I8_128 ? 128 : 64;
+    const long threads = p.kind == I8_FEW ? 512l * cdiv(a.N, a.M <= 32 ? 16 : 32) : (p.kind == I8_256 ? 512l : 256l) * cdiv(a.M, bm) * cdiv(a.N, bm);
+    CB_CHECK(threads < (1l << 32), CB_ERR_SHAPE, "gemm_i8: %d x %d outputs are too many for one call", a.M, a.N);
     L.count(p.nsplit > 1 ? 2 : 1);
     if (L.stats) { L.stats->gemm_flops += 2.0 * a.M * a.N * (double)a.K; L.stats->gemm_launches++; }
     if (L.dry) return;

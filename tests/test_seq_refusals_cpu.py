@@ -1,4 +1,4 @@
-"""CPU tests of the sequence attention's refusal of gradients laid over each other (a dry context: no GPU, all checks)."""
+"""CPU tests of what the sequence operators refuse: gradients laid over each other, and grids beyond a launch (a dry context: no GPU, all checks)."""
 import itertools
 
 import pytest
@@ -91,3 +91,16 @@ def test_every_small_layout_against_its_addresses(dry):
             if idx(a, 0) & idx(b, off):
                 with pytest.raises(lib.CBError, match="overlaps"):
                     lib.seq_attention_backward(ctx, tape, do, dk=dk, dv=dv)
+
+
+def test_product_grids_beyond_a_launch_are_refused(dry):
+    """a launch holds fewer than 2^32 threads; 2^31 - 1 rows onto one channel would be 2^23 blocks of 512"""
+    import ctypes as C
+    lib, ctx = dry
+    for m, n, ok in (((1 << 31) - 1, 1, False), ((1 << 31) - 600, 1, True), (1, 1 << 27, True), (1 << 30, 1, True)):
+        d = lib.GemmI8Desc()
+        d.M, d.N, d.K, d.lda, d.ldb, d.ldc = m, n, 16, 16, 16, n
+        for name in ("A", "B", "C", "a_scale", "b_scale"):
+            setattr(d, name, 0x1000)
+        rc = lib.load().cb_gemm_i8(ctx.h, C.byref(d))
+        assert (rc == 0) == ok and (ok or rc == -3 and b"too many" in lib.load().cb_last_error()), (m, n, rc, lib.load().cb_last_error())
