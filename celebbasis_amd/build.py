@@ -38,7 +38,7 @@ for _src in ("cb_seq_token.hip", "cb_norm_i8.hip", "cb_gemm_i8.hip"):
 if os.environ.get("CB_FLASH_ABL"):       # timing ablations of the fp32 attention backward (cb_flash.hip, FL_ABL): results are wrong under them
     EXTRA["cb_flash.hip"] = EXTRA["cb_flash.hip"] + ["-DFL_ABL=" + str(int(os.environ["CB_FLASH_ABL"]))]
 NO_SCRATCH = {"cb_gemm_glds.hip": ("gemm_glds", True), "cb_gemm_bf16_p8.hip": ("gemm_bf16_p8", True), "cb_flash_bf16_v2.hip": ("f2_", False)}
-NO_SCRATCH_I8 = {"cb_gemm_i8.hip": ("_p8_", True)}
+NO_SCRATCH_I8 = {"cb_gemm_i8.hip": ("_p8_", True)}      # the same guard for the 8-bit product; NO_SCRATCH stays the set of the step's own files, which tests name
 
 
 def source_digest():

@@ -16,9 +16,10 @@
 // for itself, one row index g after the other, so that no two lanes meet: the order of all additions is fixed. A wave's sums are folded by
 // bucket at the end of each head. (Measured, this kernel on 8 x 12 heads, 512 x 512, where half of the tiles are near: by columns of a copy
 // shifted row by row 54 us, by ds_add_f32 134 us, with a copy of the sums for each g, which costs the third block a CU, 43 us, so 32 us.)
-// What bounds them: vector instructions, as in the forward pass, and with 32 rows a wave two waves a SIMD to hide everything else. 2 x 12 heads, 4096
-// causal, d 64, bf16, with bias and dtable: dQ 113 - 124 us, dK/dV 166 us (scores and dP formed in both: 180 GFLOP, 0.63 PFLOP/s); fp32, 16 heads, 1023 x 333, d 80: 37 and 54 us
-// (6.1 GFLOP for both, 40 us at the rate of a large fp32 product).
+// What bounds them: vector and matrix instructions one after the other, with two waves a SIMD to overlap them (32 rows a wave take over 200 registers).
+// 2 x 12 heads, 4096 causal, d 64, bf16, with bias and dtable: dQ 107 - 117 us (vector units 53 % of the time, matrix units 33 %), dK/dV 156 - 171 us (45 %,
+// 30 %; LDS 29 %; scores and dP formed in both kernels: 180 GFLOP, 0.68 PFLOP/s). fp32, 16 heads, 1023 x 333, d 80: 37 and 54 us, matrix units 49 and 45 %: one
+// wave a SIMD, whose exponentials nothing runs under (6.1 GFLOP for both, 40 us at the rate of a large fp32 product).
 #include "cb_seq.h"
 #include <algorithm>
 
@@ -627,15 +628,15 @@ SeqBwdPlan seq_bwd_plan(const SeqArgs& a, bool want_dtable) {
     SeqBwdPlan p;
     const bool wide = a.dt == DT_BF16 && a.d <= 64;                  // what the registers hold for 32 rows a wave
     const long bh = (long)a.B * a.H, bk = (long)a.B * a.Hkv;
-    // measured, 16 against 32 rows a wave, with a table. dQ: 384 blocks of 128 queries (8 x 12 heads, 512 x 512) 24.0 / 27.9 us, 768 (2 x 12 heads, 4096
-    // causal) 128 / 125 us. dK, dV: 384 blocks of 128 keys 31 / 36 us, 768 188 / 173 us
+    // measured, the whole call with a table. dQ with 16 / 32 rows a wave: 384 blocks of 128 queries (8 x 12 heads, 512 x 512) 53.7 / 56.3 us, 600 (10 x 12
+    // heads, 600 x 600) 92.5 / 98.0, 768 (2 x 12 heads, 4096 causal) 257 / 247. dK, dV: 384 blocks of 128 keys 53.7 / 56.9 us, 600 92.5 / 100.9, 768 262 / 247
     p.qb = wide && bh * cdiv(a.Nq, 128) >= 768 ? 2 : 1;
     p.kb = wide && bk * cdiv(a.Nk, 128) >= 768 ? 2 : 1;
     p.nqb = (int)cdiv(a.Nq, 64 * p.qb);
     const bool brief = seq_short_takes(a);
     p.nkb = (int)cdiv(a.Nk, 64 * p.kb);
-    // few blocks of keys (or queries): the other axis is split into runs of at least 4 tiles. 128 blocks (64 heads, 4096 x 77, d 40): 102 us whole,
-    // 26 + 5 us in 8 parts
+    // few blocks of keys (or queries): the other axis is split into runs of at least 4 tiles. 128 blocks (64 heads, 4096 x 77, d 40), whole call:
+    // 99 us unsplit, 55 us in 8 parts
     const long fill = a.dt == DT_BF16 ? 1024 : 512;
     const long kblocks = bk * cdiv(a.Nk, 64 * p.kb), steps = (long)a.G * cdiv(a.Nq, 64);
     p.qsplit = kblocks < 384 && steps >= 8 ? (int)std::min<long>(fill / std::max(kblocks, 1l), steps / 4) : 1;

@@ -3,7 +3,8 @@
 // All keys and values of one (sample, head) stay in LDS, and the scores of a row over all of them in registers: the softmax needs no running
 // maximum, and the row sums of the backward pass come from the probabilities in fp32 on the spot (exact; neither output is read). After K and V
 // have arrived once, the waves of a block run by themselves, each over blocks of 16 rows, with the rows of the next block in flight: bound by
-// reading Q (and dO) and writing O (dQ). Measured on 64 heads, 4096 x 77, d 40, bf16 (forward / dQ): tile kernels 27 / 41 us, these 28 / 32.
+// reading Q (and dO) and writing O (dQ) and by what a turn of 16 rows takes. Measured on 64 heads, 4096 x 77, d 40, bf16 (forward / dQ): 22 / 25 us, vector
+// units 51 / 48 % of the time, 2 waves a SIMD.
 #include "cb_seq.h"
 #include <algorithm>
 
@@ -127,7 +128,8 @@ __global__ __launch_bounds__(256) void seq_short_kernel(const SeqArgs a, const i
 #pragma unroll
         for (int t = 0; t < G::DA; ++t) o[0][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
         // The rows that were fetched for the next turn are waited for before this turn's results are stored: stores count as outstanding memory
-        // operations too, and a wait behind them would last until they are done (measured: forward 30 us with it, 64 heads, 4096 x 77)
+        // operations too, and a wait behind them would last until they are done (measured: forward 30 us with it, 28 without, 64 heads, 4096 x 77, before the
+        // accumulators lay beside the vector registers)
         auto next = [&]() {
 #pragma unroll
             for (int s2 = 0; s2 < KS; ++s2) {
@@ -238,8 +240,9 @@ template <typename T, int DT> constexpr int SHORT_KEYS = sizeof(T) == 4 && DT > 
 bool seq_short_takes(const SeqArgs& a) { return a.Nk > 0 && a.Nk <= (a.dt == DT_F32 && a.d > 128 ? SHORT_KEYS<float, 10> : SEQ_SHORT); }
 template <typename T, int DT, int NT, bool BWD>
 static void short_go(const Launch& L, const SeqArgs& a) {
-    // blocks of 16 rows a wave: as many as leave 2 blocks (of 4 waves) a CU, at most 8. 64 heads, 4096 x 77, forward / dQ: 2 rows of blocks 30 / 40 us,
-    // 4 29 / 36, 8 28 / 32, 16 (one block a CU) 46 / 51
+    // blocks of 16 rows a wave: as many as leave 2 blocks (of 4 waves) a CU, at most 8. Forward / whole backward call, us, by turns: 64 heads, 4096 x 77, d 40,
+    // bf16 2: 21 / 57, 4: 19 / 55, 8: 21 / 54, 16: 32 / 66; fp32 2: 59 / 195, 4: 54 / 189, 8: 51 / 187, 16: 63 / 199; 32 heads (2 blocks a CU at 4) bf16
+    // 2: 12.2 / 39.5, 4: 12.6 / 37.8, 8: 18 / 44
     const long heads = (long)a.B * a.H, rbs = cdiv(a.Nq, 16);
     const int turns = (int)std::max(1l, std::min<long>(8, heads * rbs / (4 * 512)));
     const int nqb = (int)cdiv(rbs, 4 * turns);

@@ -833,7 +833,7 @@ def seq_attention(ctx, q, k, v, scale=None, causal=False, q_pos=None, q_len=None
     head dim (slices of a fused projection, transposed caches); scale defaults to d ** -0.5.
     causal: key j is visible to query i where j <= q_pos[b] + i. q_pos, q_len, kv_len: int32 [B] on the device (0, Nq, Nk by default).
     kv_mask: bool or uint8 [B, Nk], non-zero = visible. relpos + table [num_buckets, heads]: learned bias by the distance key - query.
-    Rows at or beyond q_len and rows that see no key are 0.
+    Rows at or beyond q_len and rows that see no key are 0. Sums are fp32; bf16 rounds the probabilities to bf16 for the product with v.
     Returns out [B, Nq, heads, d] (or `out`, written), with need_grad (out, tape) for seq_attention_backward. The backward call reads the
     inputs again: they, lengths and masks included, must still hold what the forward call saw."""
     head, mid, key = _seq_inputs(ctx, q, k, v, scale, causal, q_pos, q_len, kv_len, kv_mask, relpos, table)
@@ -1005,7 +1005,8 @@ def quantize_rows(ctx, x):
 
 def linear_i8(ctx, a, a_scale, w, w_scale, bias=None, residual=None, dtype="bf16"):
     """a_scale * w_scale * (a . w^T) + bias + residual (cb_gemm_i8): a int8 [..., K], w int8 [N, K] (K padded by quantize_rows / rms_norm),
-    a_scale [...], w_scale [N], bias float32 [N], residual [..., N] of the output's dtype -> [..., N]"""
+    a_scale [...], w_scale [N], bias float32 [N], residual [..., N] of the output's dtype -> [..., N]. Forward only: there is no gradient of a,
+    so a tower that is trained through keeps float projections."""
     _place(ctx, a=a, a_scale=a_scale, w=w, w_scale=w_scale, bias=bias, residual=residual)
     code = dtype_code(dtype)
     if w.dim() != 2:

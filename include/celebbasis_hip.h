@@ -201,6 +201,8 @@ typedef struct { void* p; int64_t row, head, batch; } cb_seq_tensor; /* [batch][
  * NaN). Causal order hides scores alone: a V that is not finite at a key behind a query that sees others may reach it (0 x inf). A table entry of
  * -inf hides its bucket; finite ones of any magnitude count (held to +-1e37): scale q.k + entry is rounded to fp32, in the backward pass as in the
  * forward. A one-token call over a cache: Nq = 1, q_pos[b] = kv_len[b] - 1.
+ * Scores, softmax statistics and all sums are fp32. bf16 rounds the probabilities (and, backward, p (dP - D)) to bf16 for the matrix products that
+ * follow them; one-token calls (heads / kv_heads <= 8) and fp32 round nothing but the results.
  * kv_heads divides heads; head h reads key / value head h / (heads / kv_heads). d % 8 == 0, d <= 160. Pointers 16-byte aligned, strides
  * multiples of 16 bytes, row strides below 2^22 elements; out, dq, dk, dv must not overlap themselves, and their address ranges not those of
  * the inputs; dq, dk and dv may be slices of one buffer that do not meet. Inputs may have stride 0. The backward call reads the inputs again,
@@ -255,7 +257,8 @@ int cb_rmsnorm_bwd(cb_ctx* ctx, const cb_rmsnorm_desc* d);
 int cb_quantize_rows(cb_ctx* ctx, int dtype, const void* x, int64_t ldx, int64_t rows, int C, int8_t* q, int64_t ldq, float* scale);
 /* C[m][n] = a_scale[m] b_scale[n] sum_k A[m][k] B[n][k] + bias[n] + R[m][n] (beside cb_gemm): 8-bit integers with a scale per token and per
  * output channel, summed exactly in 32 bits. K % 16 == 0 (pad rows with zeros: cb_quantize_rows does), K <= 131056; A and B 16-byte aligned,
- * lda % 16 == 0, ldb % 16 == 0, both below 2^23; any N, ldc, ldr. A scale of NaN or infinity makes its row or column NaN. C may be R. */
+ * lda % 16 == 0, ldb % 16 == 0, both below 2^23; any N, ldc, ldr. A scale of NaN or infinity makes its row or column NaN. C may be R.
+ * Forward only: a tower that is trained through (its weights frozen, the gradient passing to its inputs) keeps cb_gemm for its projections. */
 typedef struct {
     int struct_size;                             /* = sizeof(cb_gemm_i8_desc) */
     int dtype;                                   /* cb_dtype of C and R */
