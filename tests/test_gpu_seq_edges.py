@@ -238,3 +238,37 @@ def test_backward_of_wide_blocks(cb, d, kind):
     check(cb, BF, B, N, N, H, Hkv, d, **kw)
     if kind == "two_sided":
         check_table(cb, BF, B, N, N, H, d, kw["rel"], _table(kw["rel"], H, LOWEST, "outer"), kv_mask=kw["kv_mask"])
+
+
+@DT
+@pytest.mark.parametrize("d", [8, 40, 128, 160])
+@pytest.mark.parametrize("Nk", [60, 120, 300, 900])
+def test_large_entries_with_shared_heads(cb, dtype, d, Nk):
+    """key / value heads shared by three query heads, lengths, a mask, causal order: the call with the heads repeated gives the same rows, and the
+    gradients of the shared heads are the sums of its own (each stored with one rounding, the sum with another, in at most 4 more of fp32)"""
+    lib, ctx = cb
+    B, Nq, Hkv, G = 2, 90, 2, 3
+    H, rel = Hkv * G, (32, 64, False)
+    q, k, v = rnd(B, Nq, H, d, seed=1, dtype=dtype), rnd(B, Nk, Hkv, d, seed=2, dtype=dtype), rnd(B, Nk, Hkv, d, seed=3, dtype=dtype)
+    do, rp = rnd(B, Nq, H, d, seed=4, dtype=dtype), lib.RelPos(ctx, *rel)
+    m = torch.rand(B, Nk, generator=torch.Generator().manual_seed(6)).to(_dev()) < 0.7
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=_dev())              # noqa: E731
+    t = rnd(rel[0], H, seed=5)
+    t[:, 1], t[rel[0] - 1, 2], t[:, 4], t[3, 5] = LOWEST, -1e9, 3e9, -math.inf      # heads of one group differ
+    kw = dict(causal=True, q_pos=i32(Nk - Nq + 20, 10), q_len=i32(Nq, 77), kv_len=i32(Nk, Nk - 9), kv_mask=m, relpos=rp, table=t, need_grad=True)
+    out, tape = lib.seq_attention(ctx, q, k, v, **kw)
+    g = lib.seq_attention_backward(ctx, tape, do)
+    ke, ve = k.repeat_interleave(G, 2), v.repeat_interleave(G, 2)
+    want, tape2 = lib.seq_attention(ctx, q, ke, ve, **kw)
+    w = lib.seq_attention_backward(ctx, tape2, do)
+    for x in (out, tape.lse.nan_to_num(neginf=0.0), g.dq, g.dk, g.dv, g.dtable):
+        assert torch.isfinite(x).all()
+    assert torch.equal(tape.lse == -math.inf, tape2.lse == -math.inf)
+    rt = R if dtype == BF else U
+    near = lambda a, b, bound: ((a.double() - b.double()).abs() <= bound).all()     # noqa: E731
+    # (how the axes are split may differ between the two calls: bf16 probabilities stay, fp32 sums move by their own rounding)
+    assert near(out, want, 2 * rt * want.double().abs() + 2 * (Nk + 8) * U * v.double().abs().max())
+    assert near(g.dq, w.dq, 2 * rt * w.dq.double().abs() + 2 * rt * w.dq.double().abs().amax(-1, keepdim=True) + 2 * (Nk + 64) * U * w.dq.double().abs().max())
+    for a, b in ((g.dk, w.dk), (g.dv, w.dv)):
+        parts = b.double().view(B, Nk, Hkv, G, d)
+        assert near(a, parts.sum(3), rt * parts.abs().sum(3) + rt * a.double().abs() + 2 * (G * Nq + 64) * U * parts.abs().max())
